@@ -209,6 +209,61 @@ int lmh_bn_apply(const float* z, int64_t rows, int K, const float* scale, const 
  * scalars in order, out[2] = regularization = reg_a + reg_b (NULL = 0), out[0] = total = no_reg + regularization. */
 int lmh_loss_sums(const float* const* terms, int n, const float* reg_a, const float* reg_b, float* out,
                   lmh_stream_t stream);
+/* ---------------------------------------------------------------- row-wise operators of a trained head --
+ * (no reference call: luminoth normalises with slim.batch_norm only and reads tf.nn.softmax's probabilities, rcnn.py:222.)
+ * Rows of `cols` values, `ld*` values apart (>= cols; any alignment of the type), in fp32, f16 or bf16; statistics and sums in
+ * fp32, one rounding at the end.  Results are rows of exactly `cols` values behind each other.  rows = 0 writes nothing
+ * but zero sums. */
+enum lmh_dtype { LMH_DTYPE_F32 = 0, LMH_DTYPE_F16 = 1, LMH_DTYPE_BF16 = 2 };
+#define LMH_ROW_MAX_COLS (1 << 30)
+/* Layer norm over the last dimension: mean, rstd (rows, fp32: kept for the backward), y = (x - mean) rstd gamma + beta; gamma /
+ * beta (cols, of param_dtype = fp32 or the rows' type) may be NULL (1 / 0).
+ * Backward: dx = rstd (t - mean(t) - xh mean(t xh)) (+ addend), t = dy gamma, xh = (x - mean) rstd; dgamma = sum_rows dy xh and
+ * dbeta = sum_rows dy (param_dtype) are WRITTEN, summed in a fixed order; dx, dgamma, dbeta, addend may each be NULL. */
+int lmh_layer_norm_fwd(const void* x, int64_t ldx, const void* gamma, const void* beta, int dtype, int param_dtype, int64_t rows,
+                       int cols, float eps, void* y, float* mean, float* rstd, lmh_stream_t stream);
+size_t lmh_layer_norm_bwd_workspace_bytes(int64_t rows, int cols, int dtype);
+int lmh_layer_norm_bwd(const void* dy, int64_t lddy, const void* x, int64_t ldx, const void* addend, int64_t ldadd, const float* mean,
+                       const float* rstd, const void* gamma, int dtype, int param_dtype, int64_t rows, int cols, void* dx,
+                       void* dgamma, void* dbeta, void* ws, size_t ws_bytes, lmh_stream_t stream);
+/* Log probabilities of the given classes: logp[r] = x[r][targets[r]] - lse[r] (targets: int32, or int64 when index64; may be
+ * NULL together with logp), entropy[r] = -sum p log p, lse[r], and the `top` (<= LMH_LOG_PROBS_MAX_TOP, <= cols) largest
+ * classes of every row with their log probabilities, larger first, equal ones in the order of their index (-0 equals 0;
+ * not-a-number comes first).  A target < 0 is not asked for: logp 0, no gradient; one >= cols gives not-a-number.  Classes of
+ * -inf have p = 0; in a row of -inf alone every log probability and lse are -inf, entropy and gradient 0.
+ * Backward: dx = g_logp (1[target] - p) + sum_i g_top[i] (1[top_index[i]] - p) - g_entropy p (log p + entropy); g_logp, g_entropy
+ * may be NULL, top = 0: no alternatives. */
+#define LMH_LOG_PROBS_MAX_TOP 64
+size_t lmh_log_probs_workspace_bytes(int64_t rows, int cols, int dtype, int top);
+int lmh_log_probs_fwd(const void* x, int64_t ldx, int dtype, const void* targets, int index64, int64_t rows, int cols, int top,
+                      float* logp, float* entropy, float* lse, float* top_logp, int64_t* top_index, void* ws, size_t ws_bytes,
+                      lmh_stream_t stream);
+int lmh_log_probs_bwd(const void* x, int64_t ldx, int dtype, const void* targets, int index64, const float* lse,
+                      const float* entropy, const float* g_logp, const float* g_entropy, const int64_t* top_index,
+                      const float* g_top, int64_t rows, int cols, int top, void* dx, lmh_stream_t stream);
+/* Orthogonalised updates (the Muon optimizer, beside lmh_optimizer_step) for a list of matrices (rows, cols) at a time:
+ * O(U) = `steps` Newton-Schulz steps X <- (a I + b A + c A A) X, A = X X' (a, b, c = 3.4445, -4.7750, 2.0315) on X = U / max(|U|_F,
+ * eps), in products of fp32 accuracy.
+ * lmh_orthogonalize: out = O(g); g and out of `dtype`.
+ * lmh_muon_step (fp32): g' = (g gscale + wd w) * factor, v = momentum v + g', U = nesterov ? g' + momentum v : v,
+ * w -= lr scale O(U); `factor`: one float on the device (a clip factor of lmh_grad_clip_factors) or NULL. */
+#define LMH_MUON_MAX_JOBS 65536
+#define LMH_MUON_MAX_DIM 32768
+#define LMH_MUON_MAX_STEPS 64
+typedef struct lmh_muon_job {
+  const void* g;
+  float* v;
+  float* w;
+  void* out;
+  const float* factor;
+  int32_t rows, cols;
+  float wd, scale;
+} lmh_muon_job;
+size_t lmh_muon_workspace_bytes(const lmh_muon_job* jobs, int count);
+int lmh_orthogonalize(const lmh_muon_job* jobs, int count, int dtype, int steps, float eps, void* ws, size_t ws_bytes,
+                      lmh_stream_t stream);
+int lmh_muon_step(const lmh_muon_job* jobs, int count, int steps, float eps, float gscale, float momentum, int nesterov, float lr,
+                  void* ws, size_t ws_bytes, lmh_stream_t stream);
 void* lmh_event_create(void);
 void lmh_event_destroy(void* e);
 float lmh_event_elapsed_ms(void* e0, void* e1);

@@ -90,6 +90,11 @@ class WgradTail(ctypes.Structure):
                 ('reserved', ctypes.c_int32)]
 
 
+class MuonJob(ctypes.Structure):
+    _fields_ = [(n, ctypes.c_void_p) for n in ('g', 'v', 'w', 'out', 'factor')] + \
+               [('rows', ctypes.c_int32), ('cols', ctypes.c_int32), ('wd', ctypes.c_float), ('scale', ctypes.c_float)]
+
+
 P = ctypes.POINTER
 SIGNATURES = {
     # name: (restype, argtypes)   -- lists EVERY symbol include/luminoth_hip.h declares
@@ -213,6 +218,16 @@ SIGNATURES = {
     'lmh_grad_clip_workspace_bytes': (c_sz, [c_i]),
     'lmh_grad_clip_factors': (c_i, [c_f, c_f, c_i64, c_f, c_f, c_i, c_fl, c_fl, c_f, c_f, c_sz, c_f]),
     'lmh_optimizer_step': (c_i, [c_i, c_f, c_f, c_f, c_f, c_f, c_i64, c_f, c_f, c_f, c_i, c_fl, c_fl, c_fl, c_fl, c_fl, c_f]),
+    'lmh_layer_norm_fwd': (c_i, [c_f, c_i64, c_f, c_f, c_i, c_i, c_i64, c_i, c_fl, c_f, c_f, c_f, c_f]),
+    'lmh_layer_norm_bwd_workspace_bytes': (c_sz, [c_i64, c_i, c_i]),
+    'lmh_layer_norm_bwd': (c_i, [c_f, c_i64, c_f, c_i64, c_f, c_i64, c_f, c_f, c_f, c_i, c_i, c_i64, c_i, c_f, c_f, c_f, c_f, c_sz,
+                                 c_f]),
+    'lmh_log_probs_workspace_bytes': (c_sz, [c_i64, c_i, c_i, c_i]),
+    'lmh_log_probs_fwd': (c_i, [c_f, c_i64, c_i, c_f, c_i, c_i64, c_i, c_i, c_f, c_f, c_f, c_f, c_f, c_f, c_sz, c_f]),
+    'lmh_log_probs_bwd': (c_i, [c_f, c_i64, c_i, c_f, c_i, c_f, c_f, c_f, c_f, c_f, c_f, c_i64, c_i, c_i, c_f, c_f]),
+    'lmh_muon_workspace_bytes': (c_sz, [P(MuonJob), c_i]),
+    'lmh_orthogonalize': (c_i, [P(MuonJob), c_i, c_i, c_i, c_fl, c_f, c_sz, c_f]),
+    'lmh_muon_step': (c_i, [P(MuonJob), c_i, c_i, c_fl, c_fl, c_fl, c_i, c_fl, c_f, c_sz, c_f]),
     'lmh_dropout': (c_i, [c_f, c_i64, c_fl, ctypes.c_uint32, c_f, c_f]),
     'lmh_l2_reg_workspace_bytes': (c_sz, []),
     'lmh_l2_reg_loss': (c_i, [c_f, c_i64, c_f, c_f, c_i, c_f, c_f, c_sz, c_f]),

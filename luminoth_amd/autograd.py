@@ -6,6 +6,7 @@ into the flat gradient buffer (luminoth_amd/params.py) — autograd routes
 activation gradients between Functions and nothing else.
 """
 import torch
+from torch.autograd.function import once_differentiable
 
 from luminoth_amd import kernels as K
 
@@ -131,6 +132,59 @@ class RcnnLossFn(torch.autograd.Function):
     def backward(ctx, g):
         d_cls, d_off = ctx.saved_tensors
         return d_cls * g[0], d_off * g[1], None, None, None, None, None, None
+
+
+class LayerNormFn(torch.autograd.Function):
+    """Layer norm over the last dimension (kernels.layer_norm_fwd / _bwd)."""
+
+    @staticmethod
+    def forward(ctx, x, gamma, beta, eps):
+        y, mean, rstd = K.layer_norm_fwd(x, gamma, beta, eps)
+        ctx.save_for_backward(x, gamma, mean, rstd)
+        ctx.param_dtype = (gamma if gamma is not None else beta).dtype if gamma is not None or beta is not None else None
+        return y
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, dy):
+        x, gamma, mean, rstd = ctx.saved_tensors
+        need_x, need_g, need_b = ctx.needs_input_grad[0], ctx.needs_input_grad[1], ctx.needs_input_grad[2]
+        dgamma = torch.empty_like(gamma) if need_g else None
+        dbeta = torch.empty((x.shape[-1],), dtype=ctx.param_dtype, device=x.device) if need_b else None
+        dx = K.layer_norm_bwd(dy.contiguous(), x, mean, rstd, gamma, dgamma, dbeta, need_dx=need_x)
+        return dx, dgamma, dbeta, None
+
+
+def layer_norm(x, gamma=None, beta=None, eps=1e-5):
+    """Differentiable layer norm of x (..., D); gamma / beta (D,) float32 or x's type."""
+    return LayerNormFn.apply(x, gamma, beta, float(eps))
+
+
+class LogProbsFn(torch.autograd.Function):
+    """kernels.log_probs_fwd / _bwd; the alternatives' indices carry no gradient."""
+
+    @staticmethod
+    def forward(ctx, logits, targets, top_k):
+        logp, entropy, top, index, lse = K.log_probs_fwd(logits, targets, top_k)
+        ctx.save_for_backward(logits, targets, lse, entropy, index)
+        if index is not None:
+            ctx.mark_non_differentiable(index)
+        ctx.set_materialize_grads(False)
+        return logp, entropy, top, index
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, g_logp, g_entropy, g_top, _):
+        logits, targets, lse, entropy, index = ctx.saved_tensors
+        if g_logp is None and g_entropy is None and g_top is None:
+            return None, None, None
+        c = [None if g is None else g.contiguous() for g in (g_logp, g_entropy, g_top)]
+        return K.log_probs_bwd(logits, targets, lse, entropy, c[0], c[1], index if c[2] is not None else None, c[2]), None, None
+
+
+def log_probs(logits, targets=None, top_k=0):
+    """Differentiable -> (logp, entropy, top_logp, top_index) of kernels.log_probs_fwd."""
+    return LogProbsFn.apply(logits, targets, top_k)
 
 
 class MaxPoolFn(torch.autograd.Function):

@@ -10,7 +10,7 @@ OBJS=""
 pids=""
 # objects built with other flags (e.g. a probe build) are stale whatever their age
 if [ "$(cat .build_flags 2>/dev/null)" != "$FLAGS" ]; then rm -f *.o; echo "$FLAGS" > .build_flags; fi
-for f in api plan proposals detect targets roi loss optim elementwise bnorm ssd tail halfstore conv conv_x3; do
+for f in api plan proposals detect targets roi loss optim elementwise bnorm lnorm logprobs muon ssd tail halfstore conv conv_x3; do
   stale=0
   if [ ! -f "$f.o" ] || [ "$f.hip" -nt "$f.o" ]; then stale=1; fi
   for h in *.h ../../include/luminoth_hip.h; do

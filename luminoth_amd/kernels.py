@@ -6,6 +6,7 @@ that merely own the memory.  Nothing in this file computes with torch ops, and
 nothing falls back to the CPU: tensors must live on a ROCm device.
 """
 import ctypes
+import functools
 import threading
 import os
 
@@ -1212,6 +1213,193 @@ def softmax(x):
     return y
 
 
+# ------------------------------------------- row-wise operators of a trained head ----
+ROW_DTYPES = {torch.float32: 0, torch.float16: 1, torch.bfloat16: 2}     # enum lmh_dtype
+
+
+def _refuse(cond, text, *args):
+    if cond:
+        raise _lib.LuminothHipError(text % args if args else text)
+
+
+def _row_dtype(t, what):
+    _refuse(t.dtype not in ROW_DTYPES, '%s: float32, float16 or bfloat16 expected, got %s', what, t.dtype)
+    return ROW_DTYPES[t.dtype]
+
+
+def _rows_of(t, what):
+    """(..., cols) -> (rows, cols, row stride): evenly spaced rows whose values lie behind each other."""
+    _refuse(t.dim() == 0 or t.shape[-1] == 0, '%s: at least one column expected, got shape %s', what, tuple(t.shape))
+    cols = t.shape[-1]
+    rows = t.numel() // cols
+    if rows == 0:
+        return 0, cols, cols
+    try:
+        v = t.view(rows, cols)
+    except RuntimeError:
+        v = None
+    _refuse(v is None or (cols > 1 and v.stride(1) != 1) or (rows > 1 and v.stride(0) < cols),
+            '%s: rows of contiguous values at an even distance expected, got shape %s with strides %s', what, tuple(t.shape),
+            tuple(t.stride()))
+    return rows, cols, v.stride(0) if rows > 1 else cols
+
+
+def _pr(t):
+    """Device pointer of rows that _rows_of has checked (no contiguity asked for)."""
+    if t is None:
+        return None
+    keep = _TLS.keep
+    if keep is not None:
+        keep.append(t)
+    return ctypes.c_void_p(t.data_ptr())
+
+
+def _same_device(first, *others):
+    _refuse(not first.is_cuda, 'luminoth_amd kernels need ROCm device tensors (got %s); there is no CPU fallback', first.device)
+    for t in others:
+        _refuse(t is not None and t.device != first.device, 'tensors on %s and %s in one call', first.device,
+                t.device if t is not None else None)
+
+
+def _new(shape, dtype, device):
+    """Uninitialised memory of the stream this module launches on (scratch and results of ONE call: nothing is shared
+    between calls, streams or captured graphs)."""
+    if _stream_override_obj is not None:
+        with torch.cuda.stream(_stream_override_obj):
+            return torch.empty(shape, dtype=dtype, device=device)
+    return torch.empty(shape, dtype=dtype, device=device)
+
+
+def _on_device_of(fn):
+    """The call runs with the device of its first tensor as the current one (its current stream is the launch stream)."""
+    @functools.wraps(fn)
+    def call(first, *args, **kwargs):
+        t = first if torch.is_tensor(first) else first[0] if len(first) else None
+        if t is None or not t.is_cuda or t.device.index == torch.cuda.current_device():
+            return fn(first, *args, **kwargs)
+        with torch.cuda.device(t.device):
+            return fn(first, *args, **kwargs)
+    return call
+
+
+def _ln_params(x, cols, what, *params):
+    """gamma / beta / dgamma / dbeta: (cols,) of one type, float32 or the rows' own -> enum lmh_dtype"""
+    dtype = None
+    for t in params:
+        if t is None:
+            continue
+        _refuse(tuple(t.shape) != (cols,), '%s: parameters of shape (%d,) expected, got %s', what, cols, tuple(t.shape))
+        _refuse(t.dtype not in (torch.float32, x.dtype), '%s: parameters in float32 or %s expected, got %s', what, x.dtype, t.dtype)
+        _refuse(dtype is not None and t.dtype != dtype, '%s: parameters of two types, %s and %s', what, dtype, t.dtype)
+        dtype = t.dtype
+    return ROW_DTYPES[torch.float32 if dtype is None else dtype]
+
+
+@_on_device_of
+def layer_norm_fwd(x, gamma=None, beta=None, eps=1e-5):
+    """y = (x - mean) * rstd * gamma + beta over the last dimension of x (..., D) in float32, float16 or bfloat16 -> (y like x
+    but contiguous, mean, rstd: float32 of shape (...)).  Rows may lie in a wider buffer."""
+    lib = _lib.load()
+    dtype = _row_dtype(x, 'layer_norm')
+    rows, cols, ld = _rows_of(x, 'layer_norm')
+    pdtype = _ln_params(x, cols, 'layer_norm', gamma, beta)
+    _same_device(x, gamma, beta)
+    y = _new(x.shape, x.dtype, x.device)
+    mean = _new(x.shape[:-1], torch.float32, x.device)
+    rstd = _new(x.shape[:-1], torch.float32, x.device)
+    check(lib.lmh_layer_norm_fwd(_pr(x), ld, _p(gamma), _p(beta), dtype, pdtype, rows, cols, float(eps), _p(y), _p(mean), _p(rstd),
+                                 _stream()), 'lmh_layer_norm_fwd')
+    return y, mean, rstd
+
+
+@_on_device_of
+def layer_norm_bwd(dy, x, mean, rstd, gamma=None, dgamma=None, dbeta=None, addend=None, need_dx=True):
+    """-> dx (contiguous; + addend, the gradient of x from its other consumers); dgamma / dbeta (D,), float32 or x's type, are
+    written when given (sums over all rows in a fixed order)."""
+    lib = _lib.load()
+    dtype = _row_dtype(x, 'layer_norm')
+    rows, cols, ldx = _rows_of(x, 'layer_norm')
+    lds = {}
+    for name, t in (('dy', dy), ('addend', addend)):
+        _refuse(t is not None and (t.shape != x.shape or t.dtype != x.dtype), 'layer_norm: %s like x expected (%s, %s)', name,
+                tuple(x.shape), x.dtype)
+        lds[name] = _rows_of(t, 'layer_norm: ' + name)[2] if t is not None else 0
+    for name, t in (('mean', mean), ('rstd', rstd)):
+        _refuse(t.shape != x.shape[:-1] or t.dtype != torch.float32, 'layer_norm: %s of the forward expected', name)
+    _refuse(addend is not None and not need_dx, 'layer_norm: an addend needs dx')
+    pdtype = _ln_params(x, cols, 'layer_norm', gamma, dgamma, dbeta)
+    _same_device(x, dy, mean, rstd, gamma, dgamma, dbeta, addend)
+    dx = _new(x.shape, x.dtype, x.device) if need_dx else None
+    ws = None
+    if dgamma is not None or dbeta is not None:
+        ws = _new((lib.lmh_layer_norm_bwd_workspace_bytes(rows, cols, dtype),), torch.uint8, x.device)
+    check(lib.lmh_layer_norm_bwd(_pr(dy), lds['dy'], _pr(x), ldx, _pr(addend), lds['addend'], _p(mean), _p(rstd), _p(gamma), dtype,
+                                 pdtype, rows, cols, _p(dx), _p(dgamma), _p(dbeta), _p(ws),
+                                 ctypes.c_size_t(0 if ws is None else ws.numel()), _stream()), 'lmh_layer_norm_bwd')
+    return dx
+
+
+LOG_PROBS_MAX_TOP = 64
+
+
+def _lp_args(logits, targets, top_k):
+    dtype = _row_dtype(logits, 'log_probs')
+    rows, cols, ld = _rows_of(logits, 'log_probs')
+    _refuse(not 0 <= int(top_k) <= min(LOG_PROBS_MAX_TOP, cols), 'log_probs: 0 to %d alternatives of %d classes, not %s',
+            min(LOG_PROBS_MAX_TOP, cols), cols, top_k)
+    if targets is not None:
+        _refuse(targets.shape != logits.shape[:-1] or targets.dtype not in (torch.int32, torch.int64),
+                'log_probs: one int32 or int64 target per row expected, got %s of %s', targets.dtype, tuple(targets.shape))
+    return dtype, rows, cols, ld
+
+
+@_on_device_of
+def log_probs_fwd(logits, targets=None, top_k=0):
+    """logits (..., C) in float32, float16 or bfloat16, targets (...) int32 / int64 or None -> (logp, entropy, top_logp, top_index,
+    lse): log p of the targets (None without them), entropy -sum p log p and log sum exp of every row (float32), and the top_k
+    (<= 64) most probable classes with their log p, (..., top_k) float32 / int64, equal ones in the order of their index (None
+    with top_k = 0).  A target -1 is not asked for (0), one that is no class gives nan.  Classes of -inf have p = 0; a row of -inf
+    alone has log p = lse = -inf and entropy 0.  include/luminoth_hip.h lmh_log_probs_fwd."""
+    lib = _lib.load()
+    k = int(top_k)
+    dtype, rows, cols, ld = _lp_args(logits, targets, k)
+    _same_device(logits, targets)
+    dev, lead = logits.device, logits.shape[:-1]
+    logp = _new(lead, torch.float32, dev) if targets is not None else None
+    entropy, lse = _new(lead, torch.float32, dev), _new(lead, torch.float32, dev)
+    top = _new(lead + (k,), torch.float32, dev) if k else None
+    index = _new(lead + (k,), torch.int64, dev) if k else None
+    ws = _new((lib.lmh_log_probs_workspace_bytes(rows, cols, dtype, k),), torch.uint8, dev)
+    check(lib.lmh_log_probs_fwd(_pr(logits), ld, dtype, _p(targets), int(targets is not None and targets.dtype == torch.int64), rows,
+                                cols, k, _p(logp), _p(entropy), _p(lse), _p(top), _p(index), _p(ws), ctypes.c_size_t(ws.numel()),
+                                _stream()), 'lmh_log_probs_fwd')
+    return logp, entropy, top, index, lse
+
+
+@_on_device_of
+def log_probs_bwd(logits, targets, lse, entropy, g_logp=None, g_entropy=None, top_index=None, g_top=None):
+    """-> gradient of the logits (their type, contiguous) from the gradients of log_probs_fwd's logp, entropy and top_logp (each
+    may be None)."""
+    lib = _lib.load()
+    k = 0 if top_index is None or g_top is None else top_index.shape[-1]
+    dtype, rows, cols, ld = _lp_args(logits, targets, k)
+    lead = logits.shape[:-1]
+    for name, t in (('lse', lse), ('entropy', entropy), ('g_logp', g_logp), ('g_entropy', g_entropy)):
+        _refuse(t is not None and (t.shape != lead or t.dtype != torch.float32), 'log_probs: float32 %s of shape %s expected', name,
+                tuple(lead))
+    _refuse(lse is None or (g_entropy is not None and entropy is None) or (g_logp is not None and targets is None),
+            'log_probs: the backward needs lse, entropy for its gradient, and targets for theirs')
+    if k:
+        _refuse(top_index.shape != lead + (k,) or top_index.dtype != torch.int64 or g_top.shape != top_index.shape or
+                g_top.dtype != torch.float32, 'log_probs: int64 alternatives and their float32 gradients of one shape expected')
+    _same_device(logits, targets, lse, entropy, g_logp, g_entropy, top_index if k else None, g_top if k else None)
+    dx = _new(logits.shape, logits.dtype, logits.device)
+    check(lib.lmh_log_probs_bwd(_pr(logits), ld, dtype, _p(targets), int(targets is not None and targets.dtype == torch.int64), _p(lse),
+                                _p(entropy), _p(g_logp), _p(g_entropy), _p(top_index) if k else None, _p(g_top) if k else None, rows,
+                                cols, k, _p(dx), _stream()), 'lmh_log_probs_bwd')
+    return dx
+
+
 # ------------------------------------------------------------- optimizer ----
 def sgd_momentum(w, g, v, seg_offset, seg_wd, lr, momentum, gscale=1.0):
     lib = _lib.load()
@@ -1245,6 +1433,100 @@ def optimizer_step(kind, w, g, slot1, slot2, seg_offset, seg_wd, seg_factor, lr,
     check(lib.lmh_optimizer_step(int(kind), _p(w), _p(g), _p(slot1), _p(slot2), _p(slot3), w.numel(), _p(seg_offset),
                                  _p(seg_wd), _p(seg_factor), seg_wd.numel(), float(lr), float(p1), float(p2),
                                  float(eps), float(gscale), _stream()), 'lmh_optimizer_step')
+
+
+MUON_MAX_DIM = 32768
+
+
+def _matrix_of(t, what):
+    """(..., out) weights as the matrix (inputs, out): HWIO kernels flattened like a Linear's (in, out)."""
+    _refuse(t.dim() < 2 or t.numel() == 0, '%s: matrices expected, got shape %s', what, tuple(t.shape))
+    rows, cols = t.numel() // t.shape[-1], t.shape[-1]
+    _refuse(max(rows, cols) > MUON_MAX_DIM, '%s: at most %d rows and columns, got %d x %d', what, MUON_MAX_DIM, rows, cols)
+    return rows, cols
+
+
+@_on_device_of
+def orthogonalize(mats, steps=5, eps=1e-7):
+    """O(U) of every matrix of the list (one type: float32, float16 or bfloat16; (..., out) weights count as (inputs, out)): `steps`
+    Newton-Schulz steps that take the singular values to about 1 -> list of new tensors.  One set of launches for all of
+    them.  include/luminoth_hip.h lmh_orthogonalize."""
+    lib = _lib.load()
+    _refuse(not 1 <= int(steps) <= 64 or not float(eps) > 0, 'orthogonalize: 1 to 64 steps and eps > 0 expected')
+    mats = list(mats)
+    if not mats:
+        return []
+    dtype = _row_dtype(mats[0], 'orthogonalize')
+    jobs = (_lib.MuonJob * len(mats))()
+    out = []
+    for j, u in zip(jobs, mats):
+        _refuse(u.dtype != mats[0].dtype, 'orthogonalize: matrices of one type expected, got %s and %s', mats[0].dtype, u.dtype)
+        j.rows, j.cols = _matrix_of(u, 'orthogonalize')
+    _same_device(*mats)
+    for j, u in zip(jobs, mats):
+        o = _new(u.shape, u.dtype, u.device)
+        out.append(o)
+        j.g, j.out = _p(u).value, _p(o).value
+    ws = _new((lib.lmh_muon_workspace_bytes(jobs, len(mats)),), torch.uint8, mats[0].device)
+    check(lib.lmh_orthogonalize(jobs, len(mats), dtype, int(steps), float(eps), _p(ws), ctypes.c_size_t(ws.numel()), _stream()),
+          'lmh_orthogonalize')
+    return out
+
+
+class MuonJobs(object):
+    """Weights, gradients and momentum (lists of float32 tensors of one shape each) as the descriptors of lmh_muon_step, made
+    once by an optimizer whose buffers stay where they are.  weight_decay: a number or one per matrix; scale: one factor of
+    the update per matrix, by default 0.2 sqrt(max(rows, cols)) - an orthogonal matrix then has the root mean square of an
+    Adam update, 0.2; factors: (n,) float32 device tensor of gradient factors (grad_clip_factors) or None."""
+
+    def __init__(self, params, grads, moms, weight_decay=0.0, scale=None, factors=None):
+        params, grads, moms = list(params), list(grads), list(moms)
+        n = len(params)
+        _refuse(n == 0 or len(grads) != n or len(moms) != n, 'muon: as many gradients and momenta as weights expected')
+        _refuse(factors is not None and (tuple(factors.shape) != (n,) or factors.dtype != torch.float32),
+                'muon: float32 factors of shape (%d,) expected', n)
+        self.tensors = params + grads + moms + ([factors] if factors is not None else [])
+        self.jobs, self.count = (_lib.MuonJob * n)(), n
+        for t in self.tensors:
+            _refuse(t.dtype != torch.float32, 'muon: float32 expected, got %s', t.dtype)
+        for i, (j, w, g, v) in enumerate(zip(self.jobs, params, grads, moms)):
+            _refuse(w.shape != g.shape or w.shape != v.shape, 'muon: weights, gradient and momentum of one shape expected, got %s, %s, %s',
+                    tuple(w.shape), tuple(g.shape), tuple(v.shape))
+            j.rows, j.cols = _matrix_of(w, 'muon')
+            j.wd = float(weight_decay[i]) if isinstance(weight_decay, (list, tuple)) else float(weight_decay)
+            j.scale = float(scale[i]) if scale is not None else 0.2 * max(j.rows, j.cols) ** 0.5
+        _same_device(*self.tensors)
+        for i, (j, w, g, v) in enumerate(zip(self.jobs, params, grads, moms)):
+            j.w, j.g, j.v = _p(w).value, _p(g).value, _p(v).value
+            j.factor = factors.data_ptr() + 4 * i if factors is not None else None
+        # what is written must be nobody else's: a matrix given twice, or overlapping views, would be updated by two blocks at a time
+        spans = sorted((t.data_ptr(), t.data_ptr() + 4 * t.numel()) for t in params + moms)
+        _refuse(any(a[1] > b[0] for a, b in zip(spans, spans[1:])), 'muon: weights and momenta overlap')
+        self.ws_bytes = _lib.load().lmh_muon_workspace_bytes(self.jobs, n)
+
+    def __len__(self):
+        return self.count
+
+    def __getitem__(self, i):
+        return self.tensors[i]
+
+
+@_on_device_of
+def muon_jobs_step(jobs, lr, momentum=0.95, nesterov=True, steps=5, eps=1e-7, gscale=1.0):
+    """One step of lmh_muon_step over the matrices of a MuonJobs, in place: g' = (gscale g + wd w) factor, v = momentum v + g',
+    w -= lr scale O(nesterov ? g' + momentum v : v)."""
+    _refuse(not 1 <= int(steps) <= 64 or not float(eps) > 0, 'muon: 1 to 64 steps and eps > 0 expected')
+    lib = _lib.load()
+    plan_keep(*jobs.tensors)
+    ws = _new((jobs.ws_bytes,), torch.uint8, jobs.tensors[0].device)
+    check(lib.lmh_muon_step(jobs.jobs, jobs.count, int(steps), float(eps), float(gscale), float(momentum), int(bool(nesterov)),
+                            float(lr), _p(ws), ctypes.c_size_t(ws.numel()), _stream()), 'lmh_muon_step')
+
+
+def muon_step(params, grads, moms, lr, momentum=0.95, nesterov=True, weight_decay=0.0, scale=None, factors=None, steps=5, eps=1e-7,
+              gscale=1.0):
+    """muon_jobs_step for lists of tensors (see MuonJobs)."""
+    muon_jobs_step(MuonJobs(params, grads, moms, weight_decay, scale, factors), lr, momentum, nesterov, steps, eps, gscale)
 
 
 def dropout(x, keep_prob, seed):

@@ -1,0 +1,161 @@
+"""Newton-Schulz products (kernels.orthogonalize) and the optimizer step on them (kernels.muon_step, train.optimizer.type: muon)
+against the formulas in float64.
+
+Tolerance of O(U).  A product of m x k by k x n numbers with operands of error 2^-24 and fp32 accumulation is off, in the 2-norm
+of its entries, by at most d |L|_F |R|_2 with d = 2^-22 (1 + sqrt(k) / 64) (operands 2 * 2^-24, three partial products, k / 16
+rounded additions that add up like a random walk).  What is off by e in X is off by 3.4445 e at most one step later (the
+quintic's largest slope, at 0), and |X_k|_F <= min(3.4445^k, 1.25 sqrt(m)).  Five steps: at most (5 + 1) 3.4445^5 d = 2910 d in
+all, and the result is rounded once to its type."""
+import math
+
+import pytest
+import torch
+
+from luminoth_amd import kernels as K
+
+pytestmark = pytest.mark.gpu
+
+COEF = (3.4445, -4.7750, 2.0315)
+SHAPES = [(1, 1), (1, 9), (7, 1), (3, 5), (16, 16), (64, 64), (65, 63), (33, 200), (200, 33), (128, 128), (129, 257), (130, 100),
+          (300, 1000), (1024, 320), (72, 2304), (2304, 64), (512, 512)]
+
+
+def ns(u, steps=5, eps=1e-7):
+    u = u.double()
+    x = u / max(float(torch.linalg.norm(u)), eps)
+    tall = x.shape[0] > x.shape[1]
+    x = x.t() if tall else x
+    for _ in range(steps):
+        g = x @ x.t()
+        x = COEF[0] * x + (COEF[1] * g + COEF[2] * (g @ g)) @ x
+    return x.t() if tall else x
+
+
+def bound(u, steps=5):
+    d = 2.0 ** -22 * (1 + math.sqrt(max(u.shape)) / 64)
+    return (steps + 1) * 3.4445 ** steps * d
+
+
+def close(got, u, steps=5, eps=1e-7):
+    want = ns(u, steps, eps)
+    err = float(torch.linalg.norm(got.cpu().double() - want))
+    half = torch.finfo(got.dtype).eps / 2
+    assert err <= bound(u, steps) + half * float(torch.linalg.norm(want)) + (2.0 ** -25 * want.numel() ** 0.5 if got.dtype == torch.float16 else 0), \
+        (tuple(u.shape), err, bound(u, steps))
+
+
+def make(rows, cols, seed=0, scale=1.0):
+    g = torch.Generator().manual_seed(seed + rows * 101 + cols)
+    r = min(4, rows, cols)
+    return scale * (0.3 * torch.randn((rows, r), generator=g) @ torch.randn((r, cols), generator=g) + torch.randn((rows, cols), generator=g))
+
+
+@pytest.mark.parametrize('dtype', [torch.float32, torch.float16, torch.bfloat16])
+@pytest.mark.parametrize('rows,cols', SHAPES)
+def test_orthogonalize(rows, cols, dtype):
+    u = make(rows, cols).to(dtype)
+    out, = K.orthogonalize([u.cuda()])
+    assert out.dtype == dtype and out.shape == u.shape
+    close(out, u)
+
+
+def test_many_matrices_at_once():
+    """More shapes and matrices than one launch takes; HWIO kernels count as (inputs, out); the result of each is the same alone."""
+    mats = [make(5 + 3 * (i % 31), 4 + 7 * (i % 29), seed=i) for i in range(101)] + [make(288, 40).view(3, 3, 32, 40)]
+    got = K.orthogonalize([m.cuda() for m in mats])
+    for m, o in zip(mats, got):
+        assert o.shape == m.shape
+        close(o.view(-1, o.shape[-1]), m.view(-1, m.shape[-1]))
+    alone, = K.orthogonalize([mats[50].cuda()])
+    assert torch.equal(alone, got[50])
+    assert K.orthogonalize([]) == []
+
+
+@pytest.mark.parametrize('scale', [1e-30, 1e-3, 1e18, 1e37])
+def test_scales(scale):
+    """|U|^2 leaves float32's range; below eps the quotient is U / eps, as defined."""
+    u = make(40, 90, scale=scale)
+    out, = K.orthogonalize([u.cuda()])
+    close(out, u)
+
+
+def test_zero_steps_eps_and_not_a_number():
+    z = torch.zeros((70, 30), device='cuda')
+    assert (K.orthogonalize([z])[0] == 0).all()
+    bad = make(70, 30)
+    bad[3, 4] = math.nan
+    good = make(70, 30)
+    a, b = K.orthogonalize([bad.cuda(), good.cuda()])
+    assert torch.isnan(a).all()
+    close(b, good)
+    for steps in (1, 2, 3, 8):
+        close(K.orthogonalize([good.cuda()], steps=steps)[0], good, steps=steps)
+    close(K.orthogonalize([good.cuda()], eps=1e3)[0], good, eps=1e3)
+
+
+@pytest.mark.parametrize('nesterov', [True, False])
+def test_step(nesterov):
+    """Two steps with everything on: weight decay, gradient factors and scale, a rate per matrix; tensors are views of one buffer."""
+    shapes = [(96, 64), (3, 3, 16, 40), (200, 300), (64, 64), (5, 2)]
+    n = [math.prod(s) for s in shapes]
+    g = torch.Generator().manual_seed(3)
+    w, v, gr = (torch.randn(sum(n) + 8, generator=g) for _ in range(3))
+
+    def views(flat):
+        out, at = [], 4
+        for s, k in zip(shapes, n):
+            out.append(flat[at:at + k].view(s))
+            at += k
+        return out
+    dw, dv, dg = w.cuda(), v.cuda(), gr.cuda()
+    wd, scale = [0.0, 0.1, 0.01, 0.0, 0.3], [1.0, 0.5, 2.0, 0.1, 1.0]
+    factors = torch.tensor([1.0, 0.5, 0.25, 1.0, 0.125])
+    rw, rv, rg = ([t.double() for t in views(f)] for f in (w, v, gr))
+    tol = [0.0] * 5
+    for _ in range(2):
+        K.muon_step(views(dw), views(dg), views(dv), lr=0.3, momentum=0.9, nesterov=nesterov, weight_decay=wd, scale=scale,
+                    factors=factors.cuda(), gscale=0.5)
+        for i in range(5):
+            gp = (0.5 * rg[i] + wd[i] * rw[i]) * float(factors[i])
+            rv[i] = 0.9 * rv[i] + gp
+            u = (gp + 0.9 * rv[i] if nesterov else rv[i]).reshape(-1, shapes[i][-1])
+            # the update's input is off by some roundings of its terms too: 4 * 2^-24 of its norm, times the slope
+            tol[i] += 0.3 * scale[i] * 2 * bound(u)
+            rw[i] = rw[i] - 0.3 * scale[i] * ns(u).reshape(shapes[i])
+    for i in range(5):
+        a, b = views(dw)[i].cpu().double(), views(dv)[i].cpu().double()
+        assert float(torch.linalg.norm(a - rw[i])) <= tol[i] + 2.0 ** -22 * float(torch.linalg.norm(rw[i]))
+        assert float(torch.linalg.norm(b - rv[i])) <= 2.0 ** -21 * float(torch.linalg.norm(rv[i])) + wd[i] * tol[i]
+    assert torch.equal(dg.cpu(), gr)
+    for flat, start in ((dw, w), (dv, v)):                 # what lies around the matrices
+        assert torch.equal(flat[:4].cpu(), start[:4]) and torch.equal(flat[-4:].cpu(), start[-4:])
+
+
+def test_same_bits_streams_and_graph():
+    mats = [make(300, 200).cuda(), make(64, 640).cuda(), make(20, 10).cuda()]
+    want = K.orthogonalize(mats)
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        got = K.orthogonalize(mats)
+    with K.launch_on(side):
+        again = K.orthogonalize(mats)
+    torch.cuda.synchronize()
+    for a, b, c in zip(want, got, again):
+        assert torch.equal(a, b) and torch.equal(a, c)
+    # two captured graphs and eager calls in turn: no scratch memory is shared
+    other = [make(300, 200, seed=5).cuda(), make(64, 640, seed=6).cuda()]
+    graphs, outs = [], []
+    for inputs in (mats, other):
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            outs.append(K.orthogonalize(inputs))
+        graphs.append(graph)
+    for seed in range(3):
+        mats[0].copy_(make(300, 200, seed=seed))
+        graphs[0].replay()
+        graphs[1].replay()
+        torch.cuda.synchronize()
+        for inputs, got in ((mats, outs[0]), (other, outs[1])):
+            for a, b in zip(got, K.orthogonalize(inputs)):
+                assert torch.equal(a, b)
