@@ -5,7 +5,10 @@ set -e
 cd "$(dirname "$0")"
 HIPCC=${HIPCC:-/opt/rocm/bin/hipcc}
 if [ "${LMH_PROBES:-0}" != 0 ]; then PROBES="-DLMH_PROBES"; fi   # timing probes in the convolution kernels (scripts/r5_*sweep*, r5_epilogue_decomp)
-FLAGS="--offload-arch=gfx950 $PROBES -O3 -std=c++17 -fPIC -ffp-contract=off -munsafe-fp-atomics -fhip-fp32-correctly-rounded-divide-sqrt -Wno-unused-result"
+FLAGS="--offload-arch=gfx950 $PROBES -O3 -std=c++17 -fPIC -ffp-contract=off -munsafe-fp-atomics -fhip-fp32-correctly-rounded-divide-sqrt -Wno-unused-result -Wno-unused-command-line-argument"
+# packed fp32 instructions (v_pk_add/mul/fma_f32), which -O3 makes of ordinary float code by itself, have given wrong results
+# now and then on this hardware: the device pass is told that there are none (the host pass says it does not know the feature)
+FLAGS="$FLAGS -Xclang -target-feature -Xclang -packed-fp32-ops"
 OBJS=""
 pids=""
 # objects built with other flags (e.g. a probe build) are stale whatever their age
