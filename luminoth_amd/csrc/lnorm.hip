@@ -122,7 +122,7 @@ k_ln_fwd_long(const T* __restrict__ x, int64_t ldx, const P* __restrict__ gamma,
   }
 }
 
-// part: [gridDim.x][2][D] partial sums of dgamma / dbeta (NULL: not wanted); dx NULL: not wanted.
+// part: [gridDim.x][2][E][TPR] partial sums of dgamma / dbeta (NULL: not wanted); dx NULL: not wanted.
 template <typename T, typename P, int TPR, int NC, int BT, bool PF>
 __global__ void __launch_bounds__(BT)
 k_ln_bwd(const T* __restrict__ dy, int64_t lddy, const T* __restrict__ x, int64_t ldx, const T* __restrict__ addend, int64_t ldadd,
@@ -130,7 +130,7 @@ k_ln_bwd(const T* __restrict__ dy, int64_t lddy, const T* __restrict__ x, int64_
          float* __restrict__ part, int64_t rows, int D, float inv_d) {
   constexpr int VEC = row_type<T>::VEC, GPB = BT / TPR, E = NC * VEC;
   __shared__ float red[2][2][BT / 64];
-  extern __shared__ float sums[];       // [2][D] when the block holds several rows at a time
+  extern __shared__ float sums[];       // [GPB / 2][2][E][TPR]
   const int lane = threadIdx.x & (TPR - 1), grp = threadIdx.x / TPR;
   float ga[E], dg[E], db[E];
 #pragma unroll
@@ -225,35 +225,36 @@ k_ln_bwd(const T* __restrict__ dy, int64_t lddy, const T* __restrict__ x, int64_
     }
   }
   if (!part) return;
-  float* out = part + (size_t)blockIdx.x * 2 * D;
-  if constexpr (GPB > 1) {                 // the block's rows, one group after the other
-    for (int g = 0; g < GPB; ++g) {
-      if (grp == g) {
-#pragma unroll
-        for (int c = 0; c < NC; ++c)
-#pragma unroll
-          for (int e = 0; e < VEC; ++e) {
-            const int col = (c * TPR + lane) * VEC + e, i = c * VEC + e;
-            if (col < D) {
-              sums[col] = g ? sums[col] + dg[i] : dg[i];
-              sums[D + col] = g ? sums[D + col] + db[i] : db[i];
-            }
-          }
-      }
+  // the block's groups, halved in turn: a fixed tree.  A thread's column i lies at [i][lane]: lanes side by side in LDS and in
+  // the partial row (k_ln_params puts the columns in order)
+  if constexpr (GPB > 1) {
+    for (int half = GPB / 2; half > 0; half >>= 1) {
+      float* s = sums + (size_t)(grp & (half - 1)) * 2 * E * TPR;
       __syncthreads();
-    }
-    for (int i = threadIdx.x; i < 2 * D; i += BT) out[i] = sums[i];
-  } else {
+      if (grp >= half && grp < 2 * half) {
 #pragma unroll
-    for (int c = 0; c < NC; ++c)
-#pragma unroll
-      for (int e = 0; e < VEC; ++e) {
-        const int col = (c * TPR + lane) * VEC + e, i = c * VEC + e;
-        if (col < D) {
-          out[col] = dg[i];
-          out[D + col] = db[i];
+        for (int i = 0; i < E; ++i) {
+          s[i * TPR + lane] = dg[i];
+          s[(E + i) * TPR + lane] = db[i];
         }
       }
+      __syncthreads();
+      if (grp < half) {
+#pragma unroll
+        for (int i = 0; i < E; ++i) {
+          dg[i] += s[i * TPR + lane];
+          db[i] += s[(E + i) * TPR + lane];
+        }
+      }
+    }
+  }
+  if (grp == 0) {
+    float* out = part + (size_t)blockIdx.x * 2 * E * TPR;
+#pragma unroll
+    for (int i = 0; i < E; ++i) {
+      out[i * TPR + lane] = dg[i];
+      out[(E + i) * TPR + lane] = db[i];
+    }
   }
 }
 
@@ -322,26 +323,29 @@ k_ln_cols_long(const T* __restrict__ dy, int64_t lddy, const T* __restrict__ x, 
     }
 }
 
-// dgamma | dbeta from nb partial rows: 64 columns a block, 16 threads a column (slice s takes rows s, s + 16, ...), joined
-// in slice order.  nb = 0 (no rows): zeros.
+// dgamma | dbeta from nb partial rows of [2][W] columns: 64 a block, 16 threads a column (slice s takes rows s, s + 16, ...),
+// joined in slice order.  tpr: place p of a partial row is column ((p / tpr / vec) tpr + p % tpr) vec + (p / tpr) % vec, 0: column
+// p.  nb = 0 (no rows): zeros.
 template <typename P>
 __global__ void __launch_bounds__(1024)
-k_ln_params(const float* __restrict__ part, int nb, int D, P* __restrict__ dgamma, P* __restrict__ dbeta) {
+k_ln_params(const float* __restrict__ part, int nb, int D, int W, int tpr, int vec, P* __restrict__ dgamma, P* __restrict__ dbeta) {
   __shared__ float red[16][65];
-  const int64_t i = (int64_t)blockIdx.x * 64 + (threadIdx.x & 63);      // column of [dgamma | dbeta]
+  const int64_t i = (int64_t)blockIdx.x * 64 + (threadIdx.x & 63);      // place in [dgamma | dbeta]
   const int s = threadIdx.x >> 6;
   float a = 0.f;
-  if (i < 2 * (int64_t)D) {
-#pragma unroll 4
-    for (int r = s; r < nb; r += 16) a += part[(size_t)r * 2 * D + i];
+  if (i < 2 * (int64_t)W) {
+#pragma unroll 8
+    for (int r = s; r < nb; r += 16) a += part[(size_t)r * 2 * W + i];
   }
   red[s][threadIdx.x & 63] = a;
   __syncthreads();
-  if (s == 0 && i < 2 * (int64_t)D) {
+  if (s == 0 && i < 2 * (int64_t)W) {
 #pragma unroll
     for (int r = 1; r < 16; ++r) a += red[r][threadIdx.x];
-    P* out = i < D ? dgamma : dbeta;
-    if (out) out[i < D ? i : i - D] = from_f32<P>(a);
+    P* out = i < W ? dgamma : dbeta;
+    int p = (int)(i < W ? i : i - W);
+    if (tpr) p = (p / tpr / vec * tpr + p % tpr) * vec + p / tpr % vec;
+    if (out && p < D) out[p] = from_f32<P>(a);
   }
 }
 
@@ -362,8 +366,14 @@ static int ln_bwd_blocks(int64_t rows, int D, int vec) {
   if (D > LN_MAX_REG_COLS) return (int)(rows < LN_LONG_SLICES ? rows : LN_LONG_SLICES);
   const ln_shape s = ln_pick(D, vec);
   const int bt = ln_bwd_threads(s.tpr), gpb = bt / s.tpr;
-  const int64_t need = (rows + gpb - 1) / gpb, cap = s.tpr == 1024 ? 256 : 512;
+  // a group walks over four rows at least: what a block leaves (its sums, a partial row) costs as much as some rows
+  const int64_t need = (rows + 4 * gpb - 1) / (4 * gpb), cap = s.tpr == 1024 ? 256 : 512;
   return (int)(need < cap ? need : cap);
+}
+static int ln_part_cols(int D, int vec) {         // columns of a partial row
+  if (D > LN_MAX_REG_COLS) return D;
+  const ln_shape s = ln_pick(D, vec);
+  return s.tpr * s.nc * vec;
 }
 
 static bool ln_dtype_ok(int d) { return d == LMH_F32 || d == LMH_F16 || d == LMH_BF16; }
@@ -425,13 +435,16 @@ static void ln_bwd_launch(const void* dy, int64_t lddy, const void* x, int64_t l
     float* p = params ? part : nullptr;
 #define LN_BWD(T_, P_, TPR_, NC_)                                                                                              \
   lmh_launch((k_ln_bwd<T_, P_, TPR_, NC_, (TPR_ == 1024 ? 1024 : 512), (TPR_ < 1024)>), dim3((unsigned)nb), dim3(ln_bwd_threads(TPR_)),     \
-             (unsigned)(TPR_ == 1024 ? 0 : 2 * sizeof(float) * D), st, (const T_*)dy, lddy, (const T_*)x, ldx, (const T_*)addend, ldadd, \
+             (unsigned)(TPR_ == 1024 ? 0 : 512 / TPR_ / 2 * 2 * sizeof(float) * NC_ * row_type<T_>::VEC * TPR_), st, (const T_*)dy, lddy, (const T_*)x, ldx, (const T_*)addend, ldadd, \
              mean, rstd, (const P_*)gamma, (T_*)dx, p, rows, D, inv_d)
     LN_PICK(LN_BWD, T, P);
 #undef LN_BWD
   }
-  if (params)
-    lmh_launch((k_ln_params<P>), dim3((unsigned)((2 * (int64_t)D + 63) / 64)), dim3(1024), 0, st, (const float*)part, nb, D, (P*)dgamma, (P*)dbeta);
+  if (params) {
+    const int W = ln_part_cols(D, row_type<T>::VEC), tpr = D > LN_MAX_REG_COLS ? 0 : ln_pick(D, row_type<T>::VEC).tpr;
+    lmh_launch((k_ln_params<P>), dim3((unsigned)((2 * (int64_t)W + 63) / 64)), dim3(1024), 0, st, (const float*)part, nb, D, W, tpr,
+               row_type<T>::VEC, (P*)dgamma, (P*)dbeta);
+  }
 }
 
 #define LN_TYPES(FN, ...)                                                                                      \
@@ -455,7 +468,7 @@ extern "C" int lmh_layer_norm_fwd(const void* x, int64_t ldx, const void* gamma,
 
 extern "C" size_t lmh_layer_norm_bwd_workspace_bytes(int64_t rows, int D, int dtype) {
   if (rows <= 0 || D <= 0 || D > LMH_ROW_MAX_COLS || !ln_dtype_ok(dtype)) return 256;
-  return lmh_align_up((size_t)ln_bwd_blocks(rows, D, ln_vec(dtype)) * 2 * D * sizeof(float), 256);
+  return lmh_align_up((size_t)ln_bwd_blocks(rows, D, ln_vec(dtype)) * 2 * ln_part_cols(D, ln_vec(dtype)) * sizeof(float), 256);
 }
 
 extern "C" int lmh_layer_norm_bwd(const void* dy, int64_t lddy, const void* x, int64_t ldx, const void* addend, int64_t ldadd,

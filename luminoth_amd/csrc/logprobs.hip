@@ -10,14 +10,14 @@
 // thread: 16384 classes in 16 bits), so the logits are read once for all of it.  A short row is one wave's.  The maximum
 // of the segment is known before the first exponential, so there is ONE exponential a class.  Alternatives: the k-th
 // largest of a wave's 64 lane maxima is a lower bound of the k-th largest value (bit by bit with ballots: 32 compares);
-// what reaches the best wave's bound goes into a list of LDS - some dozens of entries - and an entry's place is the
-// number of larger ones.  Value and index make one 64-bit key (larger value first, then lower index): all keys differ, so
+// the vectors that reach the best wave's bound go into a list of LDS, of those the values that do - some dozens - into a
+// second one, and an entry's place is the number of larger ones.  Value and index make one 64-bit key (larger value first, then lower index): all keys differ, so
 // the order in which lanes append does not matter.  Segments of one row are joined by a second launch.
 #include "rowops.h"
 
 #define LP_MAX_TOP LMH_LOG_PROBS_MAX_TOP
-#define LP_LIST 1024             // candidates of a segment; more (only if the row is built for it) take k rounds of a block-wide maximum
 #define LP_SEG_VECS 8
+#define LP_JOIN_LDS 4096
 
 typedef unsigned long long u64;
 
@@ -32,23 +32,36 @@ __device__ __forceinline__ float lp_unkey(uint32_t k) {
 }
 __device__ __forceinline__ u64 lp_pair(uint32_t key, uint32_t index) { return ((u64)key << 32) | (uint32_t)~index; }
 
-// The k-th largest of the 64 lanes' keys (k <= 64): the largest value that k lanes reach, bit by bit.
+// A lower bound of the k-th largest of the 64 lanes' keys (k <= 64): the largest value that k lanes reach, bit by bit, as far as
+// the upper 16 bits (of fp32 values: 7 bits of the mantissa; a looser bound only lengthens the list).
 __device__ __forceinline__ uint32_t lp_kth_of_wave(uint32_t key, int k) {
   uint32_t t = 0;
 #pragma unroll
-  for (int b = 31; b >= 0; --b) {
+  for (int b = 31; b >= 16; --b) {
     const uint32_t c = t | (1u << b);
     if (__popcll(__ballot(key >= c)) >= k) t = c;
   }
   return t;
 }
 
+template <int CTRL> __device__ __forceinline__ uint32_t dpp_max_u32(uint32_t v) {
+  const uint32_t w = (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, CTRL, 0xf, 0xf, true);
+  return w > v ? w : v;
+}
+__device__ __forceinline__ uint32_t wave_max_u32(uint32_t v) {
+  v = dpp_max_u32<0xB1>(v);
+  v = dpp_max_u32<0x4E>(v);
+  v = dpp_max_u32<0x141>(v);
+  v = dpp_max_u32<0x140>(v);
+  auto s = __builtin_amdgcn_permlane16_swap(v, v, false, false);
+  v = s[0] > s[1] ? s[0] : s[1];
+  s = __builtin_amdgcn_permlane32_swap(v, v, false, false);
+  return s[0] > s[1] ? s[0] : s[1];
+}
 __device__ __forceinline__ u64 wave_max_u64(u64 v) {
-  for (int o = 32; o > 0; o >>= 1) {
-    const u64 w = __shfl_xor(v, o);
-    v = w > v ? w : v;
-  }
-  return v;
+  const uint32_t hi = wave_max_u32((uint32_t)(v >> 32));
+  const uint32_t lo = wave_max_u32((uint32_t)(v >> 32) == hi ? (uint32_t)v : 0);
+  return ((u64)hi << 32) | lo;
 }
 
 struct lp_out {
@@ -75,6 +88,26 @@ __device__ __forceinline__ bool lp_target(const T* x, const I* targets, int64_t 
   return true;
 }
 
+template <typename T> __device__ __forceinline__ raw16 load_classes(const T* row, int col, int end) {
+  constexpr int VEC = row_type<T>::VEC;
+  if (col + VEC <= end) return load16(row + col);
+  const uint32_t none = __is_same(T, f32_t) ? 0xff800000u : __is_same(T, f16_t) ? 0xfc00fc00u : 0xff80ff80u;
+  raw16 r = {none, none, none, none};
+  if (col < end) {
+#pragma unroll
+    for (int e = 0; e < VEC; ++e)
+      if (col + e < end) {
+        if constexpr (VEC == 4) {
+          r[e] = __float_as_uint(row[col + e].v);
+        } else {
+          const uint32_t b = __builtin_bit_cast(uint16_t, row[col + e]), sh = 16 * (e & 1);
+          r[e >> 1] = (r[e >> 1] & ~(0xffffu << sh)) | (b << sh);
+        }
+      }
+  }
+  return r;
+}
+
 // TPR threads a row or segment (64: one wave, no block-wide step; 256: the block), NV vectors a thread.
 // Partial results of a segment: stats[(row * segs + seg) * 3] and, sorted, best[(row * segs + seg) * k].
 template <typename T, typename I, int TPR, int NV>
@@ -82,12 +115,13 @@ __global__ void __launch_bounds__(256)
 k_log_probs(const T* __restrict__ x, int64_t ldx, const I* __restrict__ targets, int64_t rows, int V, int k, int segs, lp_out out,
             float* __restrict__ stats, u64* __restrict__ best) {
   constexpr int VEC = row_type<T>::VEC, SEG = TPR * NV * VEC, GPB = 256 / TPR, WPG = TPR / 64;
-  constexpr int LIST = TPR == 64 ? 256 : LP_LIST;
+  constexpr int LIST = TPR == 64 ? 128 : 512, VLIST = TPR == 64 ? 64 : 256;
   __shared__ float red[3][4];
   __shared__ uint32_t red_key[4];
   __shared__ u64 list[GPB][LIST];
   __shared__ u64 winner[4];
-  __shared__ int count[GPB];
+  __shared__ raw16 vlist[GPB][VLIST];
+  __shared__ int vcol[GPB][VLIST], vcount[GPB], count[GPB];
   const int lane = threadIdx.x & (TPR - 1), grp = threadIdx.x / TPR;
   const int64_t unit = (int64_t)blockIdx.x * GPB + grp;         // (row, segment)
   const int64_t row = unit / segs;
@@ -96,28 +130,24 @@ k_log_probs(const T* __restrict__ x, int64_t ldx, const I* __restrict__ targets,
   const int first = seg * SEG;
   const T* xr = x + (live ? row : 0) * ldx;
   const int end = live ? V : 0;
+  // (behind the end: -inf, which no maximum and no sum sees)
   raw16 r[NV];
 #pragma unroll
-  for (int v = 0; v < NV; ++v) r[v] = load_cols(xr, first + (v * TPR + lane) * VEC, end);
-  if (lane == 0) count[grp] = 0;
+  for (int v = 0; v < NV; ++v) r[v] = load_classes(xr, first + (v * TPR + lane) * VEC, end);
+  if (lane == 0) count[grp] = vcount[grp] = 0;
 
-  // ---- maximum
-  float mine = -INFINITY;
-  bool nan = false;
+  // ---- maximum, of every vector and of all (fmaxf passes over not-a-number: those rows show in S)
+  float vmax[NV], mine = -INFINITY;
 #pragma unroll
-  for (int v = 0; v < NV; ++v)
+  for (int v = 0; v < NV; ++v) {
+    vmax[v] = elem<T>(r[v], 0);
 #pragma unroll
-    for (int e = 0; e < VEC; ++e) {
-      const int col = first + (v * TPR + lane) * VEC + e;
-      const float f = elem<T>(r[v], e);
-      if (col < end) {
-        mine = fmaxf(mine, f);
-        nan |= f != f;
-      }
-    }
+    for (int e = 1; e < VEC; ++e) vmax[v] = fmaxf(vmax[v], elem<T>(r[v], e));
+    mine = fmaxf(mine, vmax[v]);
+  }
   float m = reduce64(mine, op_max());
   uint32_t bound = 0;
-  if (k > 0) bound = lp_kth_of_wave(nan ? 0xffffffffu : lp_key(mine), k);
+  if (k > 0) bound = lp_kth_of_wave(lp_key(mine), k);
   if constexpr (TPR > 64) {
     if ((threadIdx.x & 63) == 0) {
       red[0][threadIdx.x >> 6] = m;
@@ -135,24 +165,21 @@ k_log_probs(const T* __restrict__ x, int64_t ldx, const I* __restrict__ targets,
   // ---- sums, and the entries of the list
   float S = 0.f, W = 0.f;
 #pragma unroll
-  for (int v = 0; v < NV; ++v)
+  for (int v = 0; v < NV; ++v) {
 #pragma unroll
     for (int e = 0; e < VEC; ++e) {
-      const int col = first + (v * TPR + lane) * VEC + e;
-      const float f = elem<T>(r[v], e);
-      if (col < end) {
-        const float z = f - m0, p = __expf(z);
-        S += p;
-        W = fmaf(p > 0.f ? z : 0.f, p, W);
-        if (k > 0) {
-          const uint32_t key = lp_key(f);
-          if (key >= bound) {
-            const int at = atomicAdd(&count[grp], 1);
-            if (at < LIST) list[grp][at] = lp_pair(key, (uint32_t)col);
-          }
-        }
+      const float z = elem<T>(r[v], e) - m0, p = __expf(z);
+      S += p;
+      W = fmaf(fmaxf(z, -200.f), p, W);          // (p = 0 below -104: -inf must not meet it)
+    }
+    if (k > 0 && lp_key(vmax[v]) >= bound) {       // the vector goes to the list whole
+      const int at = atomicAdd(&vcount[grp], 1);
+      if (at < VLIST) {
+        vlist[grp][at] = r[v];
+        vcol[grp][at] = first + (v * TPR + lane) * VEC;
       }
     }
+  }
   S = reduce64(S, op_add());
   W = reduce64(W, op_add());
   if constexpr (TPR > 64) {
@@ -191,8 +218,21 @@ k_log_probs(const T* __restrict__ x, int64_t ldx, const I* __restrict__ targets,
       best[unit * k + rank] = pair;
     }
   };
-  const int n = count[grp];
-  if (n <= LIST) {
+  const int nv = vcount[grp];
+  int n = LIST + 1;
+  if (nv <= VLIST) {
+    for (int i = lane; i < nv * VEC; i += TPR) {
+      const int col = vcol[grp][i / VEC] + i % VEC;
+      const uint32_t key = lp_key(to_f32(reinterpret_cast<const T*>(&vlist[grp][0])[i]));
+      if (key >= bound && col < end) {
+        const int at = atomicAdd(&count[grp], 1);
+        if (at < LIST) list[grp][at] = lp_pair(key, (uint32_t)col);
+      }
+    }
+    if constexpr (TPR > 64) __syncthreads();
+    n = count[grp];
+  }
+  if (n <= LIST && S == S) {
     for (int i = lane; i < n; i += TPR) {
       const u64 p = list[grp][i];
       int rank = 0;
@@ -203,7 +243,7 @@ k_log_probs(const T* __restrict__ x, int64_t ldx, const I* __restrict__ targets,
       for (int i = n + lane; i < k; i += TPR) emit(i, 0);
     return;
   }
-  // many equal values, or most large ones in few lanes: k times the largest key below the last one
+  // many equal values, most large ones in few lanes, or not-a-number among them: k times the largest key below the last one
   u64 last = ~0ull;
   for (int rank = 0; rank < k; ++rank) {
     u64 mx = 0;
@@ -230,13 +270,22 @@ k_log_probs(const T* __restrict__ x, int64_t ldx, const I* __restrict__ targets,
   }
 }
 
-// One wave a row: joins the segments' sums, then k times the largest of the lists' heads (every list is sorted).
+// One block a row: the segments' lists go to LDS (every list is sorted), then the first wave joins the sums and takes k times
+// the largest of the lists' heads.
 template <typename T, typename I>
-__global__ void __launch_bounds__(64)
+__global__ void __launch_bounds__(256)
 k_log_probs_join(const T* __restrict__ x, int64_t ldx, const I* __restrict__ targets, int64_t rows, int V, int k, int segs, lp_out out,
                  const float* __restrict__ stats, const u64* __restrict__ best) {
+  extern __shared__ u64 lists[];        // [segs][k] when that is at most LP_JOIN_LDS entries
   const int64_t row = blockIdx.x;
   const int lane = threadIdx.x;
+  const u64* b = best + row * segs * k;
+  const bool in_lds = segs <= 64 && segs * k <= LP_JOIN_LDS;
+  if (in_lds) {
+    for (int i = threadIdx.x; i < segs * k; i += blockDim.x) lists[i] = b[i];
+    if (blockDim.x > 64) __syncthreads();
+  }
+  if (threadIdx.x >= 64) return;
   const float* st = stats + row * segs * 3;
   float m = -INFINITY;
   for (int s = lane; s < segs; s += 64) m = fmaxf(m, st[3 * s]);
@@ -260,39 +309,36 @@ k_log_probs_join(const T* __restrict__ x, int64_t ldx, const I* __restrict__ tar
   }
   if (k == 0) return;
   const float log_s = S == 0.f ? 0.f : logf(S);
-  const u64* b = best + row * segs * k;
-  u64 last = ~0ull;
-  if (segs <= 64) {
+  auto emit = [&](int rank, u64 pair) {
+    const uint32_t key = (uint32_t)(pair >> 32);
+    out.index[row * k + rank] = (int64_t)(uint32_t)~(uint32_t)pair;
+    out.top[row * k + rank] = key == 0xffffffffu ? NAN : (lp_unkey(key) - m0) - log_s;
+  };
+  u64 last = ~0ull, mine = 0;           // lane r keeps the alternative of rank r (k <= 64)
+  if (in_lds) {
     int pos = 0;
-    u64 head = lane < segs ? b[lane * k] : 0;
+    u64 head = lane < segs ? lists[lane * k] : 0;
     for (int rank = 0; rank < k; ++rank) {
       const u64 mx = wave_max_u64(head);
-      if (lane == 0) {
-        const uint32_t key = (uint32_t)(mx >> 32);
-        out.index[row * k + rank] = (int64_t)(uint32_t)~(uint32_t)mx;
-        out.top[row * k + rank] = key == 0xffffffffu ? NAN : (lp_unkey(key) - m0) - log_s;
-      }
+      if (lane == rank) mine = mx;
       if (head == mx && lane < segs) {
         ++pos;
-        head = pos < k ? b[lane * k + pos] : 0;
+        head = pos < k ? lists[lane * k + pos] : 0;
       }
     }
-    return;
-  }
-  for (int rank = 0; rank < k; ++rank) {        // more than 64 segments: the entries below the last winner
-    u64 mx = 0;
-    for (int64_t i = lane; i < (int64_t)segs * k; i += 64) {
-      const u64 p = b[i];
-      if (p < last && p > mx) mx = p;
+  } else {
+    for (int rank = 0; rank < k; ++rank) {      // the largest entry below the last one
+      u64 mx = 0;
+      for (int64_t i = lane; i < (int64_t)segs * k; i += 64) {
+        const u64 p = b[i];
+        if (p < last && p > mx) mx = p;
+      }
+      mx = wave_max_u64(mx);
+      if (lane == rank) mine = mx;
+      last = mx;
     }
-    mx = wave_max_u64(mx);
-    if (lane == 0) {
-      const uint32_t key = (uint32_t)(mx >> 32);
-      out.index[row * k + rank] = (int64_t)(uint32_t)~(uint32_t)mx;
-      out.top[row * k + rank] = key == 0xffffffffu ? NAN : (lp_unkey(key) - m0) - log_s;
-    }
-    last = mx;
   }
+  if (lane < k) emit(lane, mine);
 }
 
 // Gradient: a thread's vectors of one row, then the given classes' own entries, written whole (p, entropy and every
@@ -357,9 +403,9 @@ static lp_plan lp_pick(int64_t rows, int V, int vec) {
 }
 
 extern "C" size_t lmh_log_probs_workspace_bytes(int64_t rows, int V, int dtype, int top) {
-  if (rows <= 0 || V <= 0 || V > LMH_ROW_MAX_COLS || top < 0 || top > LP_MAX_TOP) return 256;
+  if (rows <= 0 || V <= 0 || V > LMH_ROW_MAX_COLS || top < 0 || top > LP_MAX_TOP) return 0;
   const lp_plan p = lp_pick(rows, V, dtype == LMH_F32 ? 4 : 8);
-  if (p.segs == 1) return 256;
+  if (p.segs == 1) return 0;
   return lmh_align_up((size_t)rows * p.segs * 3 * sizeof(float), 256) + lmh_align_up((size_t)rows * p.segs * top * sizeof(u64), 256) + 256;
 }
 
@@ -379,8 +425,9 @@ static void lp_fwd_launch(const void* x, int64_t ldx, const void* targets, int64
   else if (p.nv == 4) LP_FWD(256, 4);
   else LP_FWD(256, 8);
 #undef LP_FWD
-  if (p.segs > 1)
-    lmh_launch((k_log_probs_join<T, I>), dim3((unsigned)rows), dim3(64), 0, st, (const T*)x, ldx, (const I*)targets, rows, V, k, p.segs, o,
+  if (p.segs > 1)       // few entries: one wave a row
+    lmh_launch((k_log_probs_join<T, I>), dim3((unsigned)rows), dim3(p.segs * k > 512 ? 256 : 64),
+               (unsigned)(p.segs <= 64 && p.segs * k <= LP_JOIN_LDS ? p.segs * k * sizeof(u64) : 0), st, (const T*)x, ldx, (const I*)targets, rows, V, k, p.segs, o,
                (const float*)stats, (const u64*)best);
 }
 
@@ -428,7 +475,8 @@ extern "C" int lmh_log_probs_fwd(const void* x, int64_t ldx, int dtype, const vo
   LMH_CHECK_ARG(lp_args_ok(dtype, rows, V, ldx, top));
   if (rows == 0) return LMH_OK;
   LMH_CHECK_ARG(x && entropy && lse && (!targets == !logp) && (top == 0 || (top_logp && top_index)));
-  if (!ws || ws_bytes < lmh_log_probs_workspace_bytes(rows, V, dtype, top)) {
+  const size_t need = lmh_log_probs_workspace_bytes(rows, V, dtype, top);
+  if (need && (!ws || ws_bytes < need)) {
     lmh_set_error("lmh_log_probs_fwd: workspace too small");
     return LMH_ERR_WORKSPACE;
   }

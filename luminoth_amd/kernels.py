@@ -1229,36 +1229,52 @@ def _row_dtype(t, what):
 
 def _rows_of(t, what):
     """(..., cols) -> (rows, cols, row stride): evenly spaced rows whose values lie behind each other."""
-    _refuse(t.dim() == 0 or t.shape[-1] == 0, '%s: at least one column expected, got shape %s', what, tuple(t.shape))
-    cols = t.shape[-1]
+    shape = t.shape
+    cols = shape[-1] if len(shape) else 0
+    if cols == 0:
+        raise _lib.LuminothHipError('%s: at least one column expected, got shape %s' % (what, tuple(shape)))
     rows = t.numel() // cols
-    if rows == 0:
-        return 0, cols, cols
-    try:
-        v = t.view(rows, cols)
-    except RuntimeError:
-        v = None
-    _refuse(v is None or (cols > 1 and v.stride(1) != 1) or (rows > 1 and v.stride(0) < cols),
-            '%s: rows of contiguous values at an even distance expected, got shape %s with strides %s', what, tuple(t.shape),
-            tuple(t.stride()))
+    if t.is_contiguous() or rows == 0:
+        return rows, cols, cols
+    v = t
+    if len(shape) != 2:
+        try:
+            v = t.view(rows, cols)
+        except RuntimeError:
+            v = None
+    if v is None or (cols > 1 and v.stride(1) != 1) or (rows > 1 and v.stride(0) < cols):
+        raise _lib.LuminothHipError('%s: rows of contiguous values at an even distance expected, got shape %s with strides %s' %
+                                    (what, tuple(shape), tuple(t.stride())))
     return rows, cols, v.stride(0) if rows > 1 else cols
 
 
 def _pr(t):
-    """Device pointer of rows that _rows_of has checked (no contiguity asked for)."""
+    """Device pointer of a tensor whose layout and device have been checked (None: NULL)."""
     if t is None:
         return None
-    keep = _TLS.keep
-    if keep is not None:
-        keep.append(t)
-    return ctypes.c_void_p(t.data_ptr())
+    if _TLS.keep is not None:
+        _TLS.keep.append(t)
+    return t.data_ptr()
+
+
+def _flat(t, what):
+    """Device pointer of a contiguous tensor of the call's device (None: NULL)."""
+    if t is None:
+        return None
+    if not t.is_contiguous():
+        raise _lib.LuminothHipError('%s: contiguous tensor expected, got strides %s' % (what, tuple(t.stride())))
+    return _pr(t)
 
 
 def _same_device(first, *others):
-    _refuse(not first.is_cuda, 'luminoth_amd kernels need ROCm device tensors (got %s); there is no CPU fallback', first.device)
+    """All tensors (or None) on the first one's GPU -> its index."""
+    dev = first.get_device()
+    if dev < 0 or not first.is_cuda:
+        raise _lib.LuminothHipError('luminoth_amd kernels need ROCm device tensors (got %s); there is no CPU fallback' % first.device)
     for t in others:
-        _refuse(t is not None and t.device != first.device, 'tensors on %s and %s in one call', first.device,
-                t.device if t is not None else None)
+        if t is not None and t.get_device() != dev:
+            raise _lib.LuminothHipError('tensors on %s and %s in one call' % (first.device, t.device))
+    return dev
 
 
 def _new(shape, dtype, device):
@@ -1270,28 +1286,45 @@ def _new(shape, dtype, device):
     return torch.empty(shape, dtype=dtype, device=device)
 
 
+def _new_like(t):
+    if _stream_override_obj is not None or not t.is_contiguous():
+        return _new(t.shape, t.dtype, t.device)
+    return torch.empty_like(t)
+
+
+_get_device = getattr(torch._C, '_cuda_getDevice', torch.cuda.current_device)      # (~10x cheaper than current_device())
+
+
 def _on_device_of(fn):
     """The call runs with the device of its first tensor as the current one (its current stream is the launch stream)."""
     @functools.wraps(fn)
     def call(first, *args, **kwargs):
-        t = first if torch.is_tensor(first) else first[0] if len(first) else None
-        if t is None or not t.is_cuda or t.device.index == torch.cuda.current_device():
+        t = first if isinstance(first, torch.Tensor) else first[0] if len(first) else None
+        if t is None or not t.is_cuda or t.get_device() == _get_device():
             return fn(first, *args, **kwargs)
         with torch.cuda.device(t.device):
             return fn(first, *args, **kwargs)
     return call
 
 
-def _ln_params(x, cols, what, *params):
+def _row_stream(dev):
+    if _stream_override is not None:
+        return _stream_override
+    return _raw_stream(dev) if _raw_stream is not None else torch.cuda.current_stream(dev).cuda_stream
+
+
+def _ln_params(x, cols, *params):
     """gamma / beta / dgamma / dbeta: (cols,) of one type, float32 or the rows' own -> enum lmh_dtype"""
     dtype = None
     for t in params:
         if t is None:
             continue
-        _refuse(tuple(t.shape) != (cols,), '%s: parameters of shape (%d,) expected, got %s', what, cols, tuple(t.shape))
-        _refuse(t.dtype not in (torch.float32, x.dtype), '%s: parameters in float32 or %s expected, got %s', what, x.dtype, t.dtype)
-        _refuse(dtype is not None and t.dtype != dtype, '%s: parameters of two types, %s and %s', what, dtype, t.dtype)
-        dtype = t.dtype
+        if t.dim() != 1 or t.shape[0] != cols:
+            raise _lib.LuminothHipError('layer_norm: parameters of shape (%d,) expected, got %s' % (cols, tuple(t.shape)))
+        if t.dtype is not dtype:
+            _refuse(t.dtype not in (torch.float32, x.dtype), 'layer_norm: parameters in float32 or %s expected, got %s', x.dtype, t.dtype)
+            _refuse(dtype is not None, 'layer_norm: parameters of two types, %s and %s', dtype, t.dtype)
+            dtype = t.dtype
     return ROW_DTYPES[torch.float32 if dtype is None else dtype]
 
 
@@ -1299,16 +1332,15 @@ def _ln_params(x, cols, what, *params):
 def layer_norm_fwd(x, gamma=None, beta=None, eps=1e-5):
     """y = (x - mean) * rstd * gamma + beta over the last dimension of x (..., D) in float32, float16 or bfloat16 -> (y like x
     but contiguous, mean, rstd: float32 of shape (...)).  Rows may lie in a wider buffer."""
-    lib = _lib.load()
     dtype = _row_dtype(x, 'layer_norm')
     rows, cols, ld = _rows_of(x, 'layer_norm')
-    pdtype = _ln_params(x, cols, 'layer_norm', gamma, beta)
-    _same_device(x, gamma, beta)
-    y = _new(x.shape, x.dtype, x.device)
+    pdtype = _ln_params(x, cols, gamma, beta)
+    dev = _same_device(x, gamma, beta)
+    y = _new_like(x)
     mean = _new(x.shape[:-1], torch.float32, x.device)
-    rstd = _new(x.shape[:-1], torch.float32, x.device)
-    check(lib.lmh_layer_norm_fwd(_pr(x), ld, _p(gamma), _p(beta), dtype, pdtype, rows, cols, float(eps), _p(y), _p(mean), _p(rstd),
-                                 _stream()), 'lmh_layer_norm_fwd')
+    rstd = _new_like(mean)
+    check(_lib.load().lmh_layer_norm_fwd(_pr(x), ld, _flat(gamma, 'layer_norm'), _flat(beta, 'layer_norm'), dtype, pdtype, rows, cols,
+                                         eps, _pr(y), _pr(mean), _pr(rstd), _row_stream(dev)), 'lmh_layer_norm_fwd')
     return y, mean, rstd
 
 
@@ -1319,23 +1351,25 @@ def layer_norm_bwd(dy, x, mean, rstd, gamma=None, dgamma=None, dbeta=None, adden
     lib = _lib.load()
     dtype = _row_dtype(x, 'layer_norm')
     rows, cols, ldx = _rows_of(x, 'layer_norm')
-    lds = {}
-    for name, t in (('dy', dy), ('addend', addend)):
-        _refuse(t is not None and (t.shape != x.shape or t.dtype != x.dtype), 'layer_norm: %s like x expected (%s, %s)', name,
-                tuple(x.shape), x.dtype)
-        lds[name] = _rows_of(t, 'layer_norm: ' + name)[2] if t is not None else 0
-    for name, t in (('mean', mean), ('rstd', rstd)):
-        _refuse(t.shape != x.shape[:-1] or t.dtype != torch.float32, 'layer_norm: %s of the forward expected', name)
-    _refuse(addend is not None and not need_dx, 'layer_norm: an addend needs dx')
-    pdtype = _ln_params(x, cols, 'layer_norm', gamma, dgamma, dbeta)
-    _same_device(x, dy, mean, rstd, gamma, dgamma, dbeta, addend)
-    dx = _new(x.shape, x.dtype, x.device) if need_dx else None
-    ws = None
+    _refuse(dy.shape != x.shape or dy.dtype != x.dtype, 'layer_norm: dy like x expected (%s, %s)', tuple(x.shape), x.dtype)
+    lddy, ldadd = _rows_of(dy, 'layer_norm: dy')[2], 0
+    if addend is not None:
+        _refuse(addend.shape != x.shape or addend.dtype != x.dtype, 'layer_norm: addend like x expected (%s, %s)', tuple(x.shape), x.dtype)
+        _refuse(not need_dx, 'layer_norm: an addend needs dx')
+        ldadd = _rows_of(addend, 'layer_norm: addend')[2]
+    lead = x.shape[:-1]
+    _refuse(mean.shape != lead or mean.dtype is not torch.float32, 'layer_norm: mean of the forward expected')
+    _refuse(rstd.shape != lead or rstd.dtype is not torch.float32, 'layer_norm: rstd of the forward expected')
+    pdtype = _ln_params(x, cols, gamma, dgamma, dbeta)
+    dev = _same_device(x, dy, mean, rstd, gamma, dgamma, dbeta, addend)
+    dx = _new_like(x) if need_dx else None
+    ws, nbytes = None, 0
     if dgamma is not None or dbeta is not None:
-        ws = _new((lib.lmh_layer_norm_bwd_workspace_bytes(rows, cols, dtype),), torch.uint8, x.device)
-    check(lib.lmh_layer_norm_bwd(_pr(dy), lds['dy'], _pr(x), ldx, _pr(addend), lds['addend'], _p(mean), _p(rstd), _p(gamma), dtype,
-                                 pdtype, rows, cols, _p(dx), _p(dgamma), _p(dbeta), _p(ws),
-                                 ctypes.c_size_t(0 if ws is None else ws.numel()), _stream()), 'lmh_layer_norm_bwd')
+        nbytes = lib.lmh_layer_norm_bwd_workspace_bytes(rows, cols, dtype)
+        ws = _new((nbytes,), torch.uint8, x.device)
+    check(lib.lmh_layer_norm_bwd(_pr(dy), lddy, _pr(x), ldx, _pr(addend), ldadd, _flat(mean, 'layer_norm'), _flat(rstd, 'layer_norm'),
+                                 _flat(gamma, 'layer_norm'), dtype, pdtype, rows, cols, _pr(dx), _flat(dgamma, 'layer_norm'),
+                                 _flat(dbeta, 'layer_norm'), _pr(ws), nbytes, _row_stream(dev)), 'lmh_layer_norm_bwd')
     return dx
 
 
@@ -1345,12 +1379,15 @@ LOG_PROBS_MAX_TOP = 64
 def _lp_args(logits, targets, top_k):
     dtype = _row_dtype(logits, 'log_probs')
     rows, cols, ld = _rows_of(logits, 'log_probs')
-    _refuse(not 0 <= int(top_k) <= min(LOG_PROBS_MAX_TOP, cols), 'log_probs: 0 to %d alternatives of %d classes, not %s',
-            min(LOG_PROBS_MAX_TOP, cols), cols, top_k)
+    if not 0 <= top_k <= LOG_PROBS_MAX_TOP or top_k > cols:
+        raise _lib.LuminothHipError('log_probs: 0 to %d alternatives of %d classes, not %s' % (min(LOG_PROBS_MAX_TOP, cols), cols, top_k))
+    index64 = 0
     if targets is not None:
-        _refuse(targets.shape != logits.shape[:-1] or targets.dtype not in (torch.int32, torch.int64),
-                'log_probs: one int32 or int64 target per row expected, got %s of %s', targets.dtype, tuple(targets.shape))
-    return dtype, rows, cols, ld
+        index64 = int(targets.dtype is torch.int64)
+        if targets.shape != logits.shape[:-1] or not (index64 or targets.dtype is torch.int32):
+            raise _lib.LuminothHipError('log_probs: one int32 or int64 target per row expected, got %s of %s' %
+                                        (targets.dtype, tuple(targets.shape)))
+    return dtype, rows, cols, ld, index64
 
 
 @_on_device_of
@@ -1362,17 +1399,18 @@ def log_probs_fwd(logits, targets=None, top_k=0):
     alone has log p = lse = -inf and entropy 0.  include/luminoth_hip.h lmh_log_probs_fwd."""
     lib = _lib.load()
     k = int(top_k)
-    dtype, rows, cols, ld = _lp_args(logits, targets, k)
-    _same_device(logits, targets)
-    dev, lead = logits.device, logits.shape[:-1]
-    logp = _new(lead, torch.float32, dev) if targets is not None else None
-    entropy, lse = _new(lead, torch.float32, dev), _new(lead, torch.float32, dev)
-    top = _new(lead + (k,), torch.float32, dev) if k else None
-    index = _new(lead + (k,), torch.int64, dev) if k else None
-    ws = _new((lib.lmh_log_probs_workspace_bytes(rows, cols, dtype, k),), torch.uint8, dev)
-    check(lib.lmh_log_probs_fwd(_pr(logits), ld, dtype, _p(targets), int(targets is not None and targets.dtype == torch.int64), rows,
-                                cols, k, _p(logp), _p(entropy), _p(lse), _p(top), _p(index), _p(ws), ctypes.c_size_t(ws.numel()),
-                                _stream()), 'lmh_log_probs_fwd')
+    dtype, rows, cols, ld, index64 = _lp_args(logits, targets, k)
+    dev = _same_device(logits, targets)
+    device, lead = logits.device, logits.shape[:-1]
+    entropy = _new(lead, torch.float32, device)
+    lse = _new_like(entropy)
+    logp = _new_like(entropy) if targets is not None else None
+    top = _new(lead + (k,), torch.float32, device) if k else None
+    index = _new(lead + (k,), torch.int64, device) if k else None
+    nbytes = lib.lmh_log_probs_workspace_bytes(rows, cols, dtype, k)
+    ws = _new((nbytes,), torch.uint8, device) if nbytes else None
+    check(lib.lmh_log_probs_fwd(_pr(logits), ld, dtype, _flat(targets, 'log_probs'), index64, rows, cols, k, _pr(logp), _pr(entropy),
+                                _pr(lse), _pr(top), _pr(index), _pr(ws), nbytes, _row_stream(dev)), 'lmh_log_probs_fwd')
     return logp, entropy, top, index, lse
 
 
@@ -1381,22 +1419,25 @@ def log_probs_bwd(logits, targets, lse, entropy, g_logp=None, g_entropy=None, to
     """-> gradient of the logits (their type, contiguous) from the gradients of log_probs_fwd's logp, entropy and top_logp (each
     may be None)."""
     lib = _lib.load()
-    k = 0 if top_index is None or g_top is None else top_index.shape[-1]
-    dtype, rows, cols, ld = _lp_args(logits, targets, k)
+    if top_index is None or g_top is None:
+        top_index = g_top = None
+    k = 0 if g_top is None else top_index.shape[-1]
+    dtype, rows, cols, ld, index64 = _lp_args(logits, targets, k)
     lead = logits.shape[:-1]
     for name, t in (('lse', lse), ('entropy', entropy), ('g_logp', g_logp), ('g_entropy', g_entropy)):
-        _refuse(t is not None and (t.shape != lead or t.dtype != torch.float32), 'log_probs: float32 %s of shape %s expected', name,
-                tuple(lead))
+        if t is not None and (t.shape != lead or t.dtype is not torch.float32):
+            raise _lib.LuminothHipError('log_probs: float32 %s of shape %s expected' % (name, tuple(lead)))
     _refuse(lse is None or (g_entropy is not None and entropy is None) or (g_logp is not None and targets is None),
             'log_probs: the backward needs lse, entropy for its gradient, and targets for theirs')
     if k:
-        _refuse(top_index.shape != lead + (k,) or top_index.dtype != torch.int64 or g_top.shape != top_index.shape or
-                g_top.dtype != torch.float32, 'log_probs: int64 alternatives and their float32 gradients of one shape expected')
-    _same_device(logits, targets, lse, entropy, g_logp, g_entropy, top_index if k else None, g_top if k else None)
-    dx = _new(logits.shape, logits.dtype, logits.device)
-    check(lib.lmh_log_probs_bwd(_pr(logits), ld, dtype, _p(targets), int(targets is not None and targets.dtype == torch.int64), _p(lse),
-                                _p(entropy), _p(g_logp), _p(g_entropy), _p(top_index) if k else None, _p(g_top) if k else None, rows,
-                                cols, k, _p(dx), _stream()), 'lmh_log_probs_bwd')
+        _refuse(top_index.shape != lead + (k,) or top_index.dtype is not torch.int64 or g_top.shape != top_index.shape or
+                g_top.dtype is not torch.float32, 'log_probs: int64 alternatives and their float32 gradients of one shape expected')
+    dev = _same_device(logits, targets, lse, entropy, g_logp, g_entropy, top_index, g_top)
+    dx = _new_like(logits)
+    what = 'log_probs'
+    check(lib.lmh_log_probs_bwd(_pr(logits), ld, dtype, _flat(targets, what), index64, _flat(lse, what), _flat(entropy, what),
+                                _flat(g_logp, what), _flat(g_entropy, what), _flat(top_index, what), _flat(g_top, what), rows, cols, k,
+                                _pr(dx), _row_stream(dev)), 'lmh_log_probs_bwd')
     return dx
 
 

@@ -82,7 +82,7 @@ def test_c_entries_refuse_before_they_launch():
     for bad in (dict(x=None), dict(ld=7), dict(dt=-1), dict(t=p), dict(lp=p), dict(top=9), dict(cols=100, ld=100, top=65), dict(top=-1),
                 dict(top=2, tl=None), dict(top=2, ti=None), dict(rows=-3), dict(rows=2 ** 40)):
         assert lp(**bad) == -1, bad
-    assert lp(n=0) == -3 and lp(ws=None) == -3 and lp(rows=0) == 0
+    assert lp(cols=40000, ld=40000, n=0) == -3 and lp(cols=40000, ld=40000, ws=None) == -3 and lp(rows=0) == 0
     lb = lambda **k: lib.lmh_log_probs_bwd(p, 8, 0, k.get('t', None), 1, k.get('lse', p), k.get('h', p), k.get('gl', None),      # noqa: E731
                                            k.get('gh', None), k.get('ti', None), k.get('gt', None), 2, 8, k.get('top', 0), p, None)
     for bad in (dict(lse=None), dict(gl=p), dict(gh=p, h=None), dict(top=2), dict(top=2, ti=p)):
