@@ -248,7 +248,7 @@ int lmh_log_probs_bwd(const void* x, int64_t ldx, int dtype, const void* targets
  * lmh_muon_step (fp32): g' = (g gscale + wd w) * factor, v = momentum v + g', U = nesterov ? g' + momentum v : v,
  * w -= lr scale O(U); `factor`: one float on the device (a clip factor of lmh_grad_clip_factors) or NULL. */
 #define LMH_MUON_MAX_JOBS 65536
-#define LMH_MUON_MAX_DIM 32768
+#define LMH_MUON_MAX_DIM (1 << 17)      /* rows and columns; rows * cols <= 2^30 */
 #define LMH_MUON_MAX_STEPS 64
 typedef struct lmh_muon_job {
   const void* g;

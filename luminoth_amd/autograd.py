@@ -160,6 +160,26 @@ def layer_norm(x, gamma=None, beta=None, eps=1e-5):
     return LayerNormFn.apply(x, gamma, beta, float(eps))
 
 
+class StoredLayerNormFn(torch.autograd.Function):
+    """Layer norm with variables of the parameter store: (gamma, beta, their places in the gradient buffer); `anchor` makes
+    autograd call the backward where the input needs no gradient (like ConvFn)."""
+
+    @staticmethod
+    def forward(ctx, x, anchor, norm):
+        x = x.contiguous()
+        y, mean, rstd = K.layer_norm_fwd(x, norm[0], norm[1])
+        ctx.save_for_backward(x, mean, rstd)
+        ctx.norm, ctx.need_dx = norm, ctx.needs_input_grad[0]
+        return y
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, dy):
+        x, mean, rstd = ctx.saved_tensors
+        gamma, _, dgamma, dbeta = ctx.norm
+        return K.layer_norm_bwd(dy.contiguous(), x, mean, rstd, gamma, dgamma, dbeta, need_dx=ctx.need_dx), None, None
+
+
 class LogProbsFn(torch.autograd.Function):
     """kernels.log_probs_fwd / _bwd; the alternatives' indices carry no gradient."""
 

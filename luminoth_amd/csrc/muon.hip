@@ -1,24 +1,31 @@
 // Orthogonalised updates by Newton-Schulz products, for a whole list of matrices at a time (gfx950, matrix cores).
 //
-//   X = U / max(|U|_F, eps), taken wide (m x n, m <= n);   `steps` times:  A = X X',  X <- (a I + b A + c A A) X
+//   X = U / max(|U|_F, eps), taken wide (m x n, m <= n);   `steps` times:  A = X X',  X <- p(A) X,  p(A) = a I + b A + c A A
 //   a = 3.4445, b = -4.7750, c = 2.0315 (the published quintic: every singular value is driven to about 1)
 //   optimizer:  g' = gscale g + wd w,  v = mu v + g',  U = g' + mu v (Nesterov) or v,  w -= lr scale X
 //
 // Arithmetic.  Small singular values grow by a = 3.44 a step, 485 times in five: 16-bit products would return noise in those
 // directions, so the products have fp32 accuracy.  Every operand is held as the sum of two f16 values, hi = f16(x) and
-// lo = f16(x - hi): 11 + 1 + 11 bits of x, an error of 2^-24 of its binade.  A product takes three matrix instructions (hi hi,
-// hi lo, lo hi; lo lo is below 2^-24) with fp32 accumulation: 3 instead of the 6 of a bf16 split, and 2500 / 3 TFLOP/s
-// against 157 of the fp32 instructions.  f16's range is enough because everything here is bounded: |X|_2 <= 1.25,
-// |A| <= 1.6, |b I + c A| <= 4.8, |a I + b A + c A A| <= 3.5 (spectral norms, which bound the entries); fixed powers of two put those just below 65504, so lo keeps its
-// bits down to entries of 2^-24 of the bound.
+// lo = f16(x - hi): 11 + 1 + 11 bits of x, an error of 2^-24 of its binade.  A product takes three matrix instructions (hi lo,
+// lo hi, hi hi; lo lo is below 2^-24) with fp32 accumulation: 3 instead of the 6 of a bf16 split, and 2500 / 3 TFLOP/s
+// against 157 of the fp32 instructions.  f16's range is enough because everything here is bounded in the spectral norm, which
+// bounds the entries: |X| <= 1.25, |A| <= 1.6, |b I + c A| <= 4.8, |p| <= 3.5, products of three p <= 41; fixed powers of two
+// put those just below 65504, so lo keeps its bits down to entries of 2^-24 of the bound.
+//
+// Long matrices (n >= 2 m).  The steps are polynomials in A, which commute: A <- p A p and Q <- p Q take m x m products only, and
+// X <- Q X comes every second or third step: of 15 m m n multiplications in five steps 6 are left.  A's error grows by up to
+// a^2 = 11.9 a step where A is small (there p hardly depends on it: |b| / a of it), so A is taken anew from X after three
+// steps at most.  Shorter matrices go X by X: A has nothing to save there.
 //
 // Layout.  An operand lies in memory as the matrix instruction takes it ("planes"): [32 rows][16 k] units of hi then lo, 64
 // lanes x 16 bytes each, k units of one row block after each other.  Tiles go to LDS with lane-linear 16-byte DMA and come
 // back with ds_read_b128 at lane * 16: no bank conflicts, no address arithmetic.  A result leaves the accumulators as
 // planes again: with its own rows along k straight from the registers (two lane-half swaps), the other way round through
-// LDS.  All three products are then row . row products.  Rows and columns are padded with zeros to whole tiles.
+// LDS.  All products are then row . row products.  Rows and columns are padded with zeros to whole tiles.
 //
-// A and the polynomial in it are symmetric: only tiles on and above the diagonal are computed.
+// Everything m x m is symmetric: only tiles on and above the diagonal are computed.  Launches take all matrices of the list.
+// Products with too few tiles for the chip (a long k), and the tiles that a last round of blocks would leave over, are split
+// along k; their parts are joined, in order, by a launch of their own.
 #include <algorithm>
 #include <vector>
 
@@ -28,52 +35,48 @@
 #define MU_B -4.7750f
 #define MU_C 2.0315f
 // scales of what is stored as f16 pairs (powers of two)
-#define MU_SX 8192.f      // X, |.| <= 1.25
-#define MU_SG 8192.f      // A = X X'
+#define MU_SX 8192.f      // X
+#define MU_SG 8192.f      // A, p A
 #define MU_SC 8192.f      // b I + c A, eigenvalues in [b, b + 1.6 c]
-#define MU_SP 8192.f      // a I + b A + c A A
+#define MU_SP 8192.f      // p(A)
+#define MU_SQ 1024.f      // products of up to three of them
 #define MU_MAX_GROUPS 24  // of one launch (kernel arguments: under 4 KB together)
-#define MU_MAX_JOBS 48
-#define MU_NORM_BLOCKS 64
+#define MU_MAX_JOBS 44
+#define MU_NORM_BLOCKS 256
+#define MU_NORM_ELEMS 8192    // at least this many per block of k_mu_norm
 
 typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
 typedef float f32x16 __attribute__((ext_vector_type(16)));
 
-// Matrices of one padded shape: their planes lie `stride` bytes apart in the workspace.
-struct mu_group {
-  int64_t off, stride;
-  int32_t m, n, pm, pn;
-  int32_t count, tall, first, splits;
-  int32_t blk0, job_blocks;        // first block of the group in this launch, blocks of one matrix
+// The matrices of one shape in one launch.  Places in the workspace and sizes of buffers are counted in units of 256 bytes; a
+// matrix's buffers are given from its start (-1: none).
+struct mu_task {
+  uint32_t off, stride;
+  int32_t m, n, pm, pn, tall;
+  int32_t count, first;            // matrices, the first one's place in the table of pointers
+  int32_t l, r, d0, d1, norm, aux;
+  int32_t whole, splits;           // tiles (of all its matrices) before `whole` are not split along k
+  uint32_t slab;                   // partial tiles of the others
+  float s0, g0, s1, g1;            // what is stored: accumulator * s + (on the diagonal) g
 };
+// blk0: the tasks' first blocks, behind each other: the arguments lie in host memory, where a search that goes from task to task
+// waits for every one of them (10 us of a 14 us launch)
 struct mu_table {
-  int32_t groups, flip, last, pad;
-  mu_group g[MU_MAX_GROUPS];
+  int32_t blk0[MU_MAX_GROUPS];     // (unused: the largest integer)
+  int32_t tasks;
+  mu_task t[MU_MAX_GROUPS];
 };
-struct mu_ptrs { const void* g; float* v; float* w; void* out; const float* factor; float wd, scale; };
+struct mu_ptrs { const void* g; float* v; void* out; const float* factor; float wd, scale; };      // out: the weights, or the result
 struct mu_jobs { mu_ptrs p[MU_MAX_JOBS]; };
 
-// Buffers of one matrix, in bytes from its start.
-struct mu_buf { int64_t x, xt0, xt1, a, c, p, slab, norm, end; };
-__host__ __device__ inline mu_buf mu_layout(const mu_group& g) {
-  mu_buf b;
-  const int64_t mn = (int64_t)g.pm * g.pn * 4, mm = (int64_t)g.pm * g.pm * 4;
-  b.x = 0;
-  b.xt0 = b.x + mn;
-  b.xt1 = b.xt0 + mn;
-  b.a = b.xt1 + mn;
-  b.c = b.a + mm;
-  b.p = b.c + mm;
-  b.slab = b.p + mm;
-  b.norm = b.slab + (g.splits > 1 ? g.splits * mm : 0);
-  b.end = b.norm + MU_NORM_BLOCKS * (int64_t)sizeof(double);
-  return b;
-}
-
 __device__ __forceinline__ int mu_find(const mu_table& t, int blk) {
-  int i = 0;
-  while (i + 1 < t.groups && blk >= t.g[i + 1].blk0) ++i;
+  int i = -1;
+#pragma unroll
+  for (int k = 0; k < MU_MAX_GROUPS; ++k) i += blk >= t.blk0[k];
   return i;
+}
+__device__ __forceinline__ char* mu_at(char* ws, const mu_task& t, int job, int buffer) {
+  return ws + ((int64_t)t.off + (int64_t)job * t.stride + buffer) * 256;
 }
 
 __device__ __forceinline__ void mu_split(float x, uint16_t* hi, uint16_t* lo) {
@@ -83,74 +86,109 @@ __device__ __forceinline__ void mu_split(float x, uint16_t* hi, uint16_t* lo) {
 }
 
 // ---- momentum and the partial sums of the squares ----------------------------------------------------------
-// u: the matrix that is orthogonalised, row-major fp32 (the optimizer's; the plain call reads its input instead)
+// aux: blocks per matrix; d0: the matrix that is orthogonalised, row-major fp32 (the optimizer's; the plain call reads its input)
 template <typename T, bool OPT>
 __global__ void __launch_bounds__(256)
 k_mu_norm(mu_table tab, mu_jobs jobs, char* ws, float mu, int nesterov, float gscale) {
   __shared__ double red[4];
-  const int gi = mu_find(tab, blockIdx.x);
-  const mu_group& g = tab.g[gi];
-  const int local = blockIdx.x - g.blk0, job = local / g.job_blocks, b = local % g.job_blocks;
-  const mu_ptrs& p = jobs.p[g.first + job];
-  char* base = ws + g.off + job * g.stride;
-  const mu_buf buf = mu_layout(g);
-  float* u = (float*)(base + buf.xt1);
-  const int64_t n = (int64_t)g.m * g.n;
-  const float f = OPT && p.factor ? *p.factor : 1.f;
+  const int ti = mu_find(tab, blockIdx.x);
+  const mu_task& t = tab.t[ti];
+  const int local = blockIdx.x - tab.blk0[ti], job = local / t.aux, b = local % t.aux;
+  const mu_ptrs& p = jobs.p[t.first + job];
+  const int64_t n = (int64_t)t.m * t.n, stride = (int64_t)t.aux * 256;
   double acc = 0.0;
-  for (int64_t i = (int64_t)b * 256 + threadIdx.x; i < n; i += (int64_t)g.job_blocks * 256) {
-    float x;
-    if (OPT) {
-      const float gp = (((const float*)p.g)[i] * gscale + p.wd * p.w[i]) * f;
-      const float v = mu * p.v[i] + gp;
-      p.v[i] = v;
-      x = nesterov ? gp + mu * v : v;
-      u[i] = x;
+  if (OPT) {
+    float* u = (float*)mu_at(ws, t, job, t.d0);
+    const float* g = (const float*)p.g;
+    const float* w = (const float*)p.out;
+    const float f = p.factor ? *p.factor : 1.f, wd = p.wd;
+    auto one = [&](float gi, float wi, float* vi) {
+      const float gp = (gi * gscale + wd * wi) * f;
+      *vi = mu * *vi + gp;
+      const float x = nesterov ? gp + mu * *vi : *vi;
+      acc += (double)x * (double)x;
+      return x;
+    };
+    if ((((uintptr_t)g | (uintptr_t)w | (uintptr_t)p.v) & 15) == 0) {
+      const int64_t n4 = n >> 2;
+      for (int64_t i = (int64_t)b * 256 + threadIdx.x; i < n4; i += stride) {
+        const float4 gi = reinterpret_cast<const float4*>(g)[i], wi = reinterpret_cast<const float4*>(w)[i];
+        float4 vi = reinterpret_cast<const float4*>(p.v)[i], x;
+        x.x = one(gi.x, wi.x, &vi.x);
+        x.y = one(gi.y, wi.y, &vi.y);
+        x.z = one(gi.z, wi.z, &vi.z);
+        x.w = one(gi.w, wi.w, &vi.w);
+        reinterpret_cast<float4*>(p.v)[i] = vi;
+        reinterpret_cast<float4*>(u)[i] = x;
+      }
+      if (b == 0 && threadIdx.x < (n & 3)) {
+        const int64_t i = 4 * n4 + threadIdx.x;
+        float v = p.v[i];
+        u[i] = one(g[i], w[i], &v);
+        p.v[i] = v;
+      }
     } else {
-      x = to_f32(((const T*)p.g)[i]);
+      for (int64_t i = (int64_t)b * 256 + threadIdx.x; i < n; i += stride) {
+        float v = p.v[i];
+        u[i] = one(g[i], w[i], &v);
+        p.v[i] = v;
+      }
     }
-    acc += (double)x * (double)x;
+  } else {
+    constexpr int VEC = row_type<T>::VEC;
+    const T* g = (const T*)p.g;
+    for (int64_t i = ((int64_t)b * 256 + threadIdx.x) * VEC; i < n; i += stride * VEC) {
+      const raw16 r = load_cols(g + i, 0, (int)(n - i < VEC ? n - i : VEC));
+#pragma unroll
+      for (int e = 0; e < VEC; ++e) acc += (double)elem<T>(r, e) * (double)elem<T>(r, e);
+    }
   }
   for (int o = 32; o > 0; o >>= 1) acc += __shfl_xor(acc, o);
   if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = acc;
   __syncthreads();
-  if (threadIdx.x == 0) ((double*)(base + buf.norm))[b] = (red[0] + red[1]) + (red[2] + red[3]);
+  if (threadIdx.x == 0) ((double*)mu_at(ws, t, job, t.norm))[b] = (red[0] + red[1]) + (red[2] + red[3]);
 }
 
 // ---- X and X' as planes --------------------------------------------------------------------------------------
-// One block: 64 x 64 of the matrix as it is stored (rows x cols), padding included.
+// One block: 64 x 64 of the matrix as it is stored (rows x cols), padding included.  l: fp32 input (OPT), d0: X, d1: X'
 template <typename T, bool OPT>
 __global__ void __launch_bounds__(256)
-k_mu_planes(mu_table tab, mu_jobs jobs, char* ws, int norm_blocks, float eps) {
+k_mu_planes(mu_table tab, mu_jobs jobs, char* ws, float eps) {
   __shared__ float tile[64][65];
+  __shared__ double total;
   const int gi = mu_find(tab, blockIdx.x);
-  const mu_group& g = tab.g[gi];
-  const int local = blockIdx.x - g.blk0, job = local / g.job_blocks, t = local % g.job_blocks;
-  char* base = ws + g.off + job * g.stride;
-  const mu_buf buf = mu_layout(g);
+  const mu_task& g = tab.t[gi];
   const int rows = g.tall ? g.n : g.m, cols = g.tall ? g.m : g.n, prow = g.tall ? g.pn : g.pm, pcol = g.tall ? g.pm : g.pn;
+  const int local = blockIdx.x - tab.blk0[gi], per = (prow / 64) * (pcol / 64), job = local / per, t = local % per;
   const int r0 = (t / (pcol / 64)) * 64, c0 = (t % (pcol / 64)) * 64;
-  const double* part = (const double*)(base + buf.norm);
-  double ss = 0.0;
-  for (int i = 0; i < norm_blocks; ++i) ss += part[i];
-  double norm = sqrt(ss);
-  if (norm < (double)eps) norm = (double)eps;            // (not a number stays one)
-  const float inv = (float)((double)MU_SX / norm);
-  const void* src = OPT ? (const void*)(base + buf.xt1) : jobs.p[g.first + job].g;
-#pragma unroll 4
+  const void* src = OPT ? (const void*)mu_at(ws, g, job, g.l) : jobs.p[g.first + job].g;
+  float x[16];
+#pragma unroll
   for (int i = 0; i < 16; ++i) {
     const int r = i * 4 + (threadIdx.x >> 6), c = threadIdx.x & 63;
-    float x = 0.f;
+    x[i] = 0.f;
     if (r0 + r < rows && c0 + c < cols) {
       const int64_t at = (int64_t)(r0 + r) * cols + c0 + c;
-      x = OPT ? ((const float*)src)[at] : to_f32(((const T*)src)[at]);
+      x[i] = OPT ? ((const float*)src)[at] : to_f32(((const T*)src)[at]);
     }
-    tile[r][c] = x * inv;
+  }
+  if (threadIdx.x < 64) {                  // the matrix's partial sums, in a fixed order
+    const double* part = (const double*)mu_at(ws, g, job, g.norm);
+    double ss = 0.0;
+    for (int i = threadIdx.x; i < g.aux; i += 64) ss += part[i];
+    for (int o = 32; o > 0; o >>= 1) ss += __shfl_xor(ss, o);
+    if (threadIdx.x == 0) total = ss;
   }
   __syncthreads();
+  double norm = sqrt(total);
+  if (norm < (double)eps) norm = (double)eps;            // (not a number stays one)
+  const float inv = (float)((double)MU_SX / norm);
+#pragma unroll
+  for (int i = 0; i < 16; ++i) tile[i * 4 + (threadIdx.x >> 6)][threadIdx.x & 63] = x[i] * inv;
+  __syncthreads();
   // stored rows as rows (k = stored columns): X for a wide matrix, X' for a tall one; and the other way round
-  char* by_row = base + (g.tall ? buf.xt0 : buf.x);
-  char* by_col = base + (g.tall ? buf.x : buf.xt0);
+  char* by_row = mu_at(ws, g, job, g.tall ? g.d1 : g.d0);
+  char* by_col = mu_at(ws, g, job, g.tall ? g.d0 : g.d1);
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, l31 = lane & 31, h = lane >> 5;
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
@@ -174,8 +212,6 @@ k_mu_planes(mu_table tab, mu_jobs jobs, char* ws, int norm_blocks, float eps) {
 }
 
 // ---- products ------------------------------------------------------------------------------------------------
-enum { MU_GRAM = 0, MU_GRAM_SPLIT = 1, MU_GRAM_JOIN = 2, MU_POLY = 3, MU_APPLY = 4, MU_LAST = 5 };
-
 // The 32 x 32 accumulator (lane: column lane & 31, register i: row (i & 3) + 8 (i >> 2) + 4 (lane >> 5)) as planes whose rows
 // are its COLUMNS and whose k are its rows: two 16-k units at `out` (+ 2048).
 __device__ __forceinline__ void mu_store_cols(const float* v, char* out, int lane) {
@@ -222,54 +258,82 @@ __device__ __forceinline__ void mu_store_rows(const float* v, char* out, int lan
   __builtin_amdgcn_wave_barrier();
 }
 
-// One tile of (64 TW)^2 of C = L . R' (rows of L and R along k), 4 waves of (32 TW)^2.  Two stages of 32 k in LDS.
-template <typename T, int TW, int MODE, bool OPT>
-__global__ void __launch_bounds__(256)
-k_mu_gemm(mu_table tab, mu_jobs jobs, char* ws, float lr) {
-  constexpr int BT = 64 * TW, RB = 2 * TW, STAGE = RB * 4096;      // bytes of one operand's stage
-  __shared__ __attribute__((aligned(16))) char smem[4 * STAGE];
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, wr = wave >> 1, wc = wave & 1, l31 = lane & 31, h = lane >> 5;
-  const int gi = mu_find(tab, blockIdx.x);
-  const mu_group& g = tab.g[gi];
-  const int local = blockIdx.x - g.blk0, job = local / g.job_blocks;
-  int t = local % g.job_blocks;
-  char* base = ws + g.off + job * g.stride;
-  const mu_buf buf = mu_layout(g);
-  const int tm = g.pm / BT, tri = tm * (tm + 1) / 2;
-  const char* xt_in = base + (tab.flip ? buf.xt1 : buf.xt0);
-  char* xt_out = base + (tab.flip ? buf.xt0 : buf.xt1);
-  int split = 0, ti, tj, kunits, k0 = 0;
-  const char *L, *R;
-  if (MODE <= MU_POLY) {                     // symmetric: tile t of the upper triangle, row by row
-    split = MODE == MU_GRAM_SPLIT ? t / tri : 0;
-    t -= split * tri;
-    ti = 0;
-    int rest = t;
-    while (rest >= tm - ti) { rest -= tm - ti; ++ti; }
-    tj = ti + rest;
-    if (MODE == MU_POLY) {
-      L = base + buf.c;
-      R = base + buf.a;
-      kunits = g.pm / 16;
-    } else {
-      L = R = base + buf.x;
-      kunits = g.pn / 16;
-    }
-  } else {
-    // X' rows x polynomial rows; a wide matrix's last product the other way round: its lanes then run along stored rows
-    const bool turn = MODE == MU_LAST && !g.tall;
-    const int tn = g.pn / BT;
-    ti = turn ? t % tm : t / tm;
-    tj = turn ? t / tm : t % tm;
-    (void)tn;
-    L = turn ? base + buf.p : xt_in;
-    R = turn ? xt_in : base + buf.p;
-    kunits = g.pm / 16;
+// Tile t (row by row) of the upper triangle of tm x tm tiles.
+__device__ __forceinline__ void mu_triangle(int t, int tm, int* ti, int* tj) {
+  int i = 0;
+  while (t >= tm - i) t -= tm - i++;
+  *ti = i;
+  *tj = i + t;
+}
+
+// The accumulator of 32-blocks (rb, cb) of a symmetric result, scaled into its one or two buffers, and mirrored unless the
+// whole tile lies on the diagonal.
+__device__ __forceinline__ void mu_store_symmetric(const mu_task& g, char* ws, int job, const float* acc, int rb, int cb, bool mirror,
+                                                   int lane, float* turn) {
+  const int l31 = lane & 31, h = lane >> 5, units = g.pm / 16;
+#pragma unroll
+  for (int k = 0; k < 2; ++k) {
+    const int d = k ? g.d1 : g.d0;
+    if (d < 0) continue;
+    const float s = k ? g.s1 : g.s0, on = k ? g.g1 : g.g0;
+    float v[16];
+#pragma unroll
+    for (int i = 0; i < 16; ++i) v[i] = acc[i] * s + (rb == cb && (i & 3) + 8 * (i >> 2) + 4 * h == l31 ? on : 0.f);
+    char* out = mu_at(ws, g, job, d);
+    mu_store_cols(v, out + ((int64_t)cb * units + rb * 2) * 2048, lane);
+    if (mirror) mu_store_rows(v, out + ((int64_t)rb * units + cb * 2) * 2048, lane, turn);
   }
-  int stages = kunits / 2;
-  if (MODE == MU_GRAM_SPLIT) {               // splits share the stages evenly
-    k0 = (int)((int64_t)stages * split / g.splits);
-    stages = (int)((int64_t)stages * (split + 1) / g.splits) - k0;
+}
+
+enum { MU_SYM = 0, MU_APPLY = 1, MU_LAST = 2 };
+
+// One tile of (64 TW)^2 of C = L . R' (rows of L and R along k), 4 waves of (32 TW)^2; a ring of DEPTH stages of 16 KU k in LDS.
+//  MU_SYM: m x m, tiles of the upper triangle; kinds of operands by r: k runs over aux 16-units.
+//  MU_APPLY: l = X' (n x m), r = a polynomial (m x m) -> d0 = X (rows m), d1 = X' (rows n).
+//  MU_LAST: the same product into the result (a wide matrix the other way round: lanes then run along stored rows).
+template <typename T, int TW, int KU, int DEPTH, int MODE, bool OPT>
+__device__ __forceinline__ void mu_gemm_tile(const mu_table& tab, const mu_jobs* jobs, char* ws, float lr) {
+  constexpr int BT = 64 * TW, RB = 2 * TW, SU = KU * 2048, STAGE = RB * SU, NL = TW * KU;      // bytes of one operand's stage, its loads by a wave
+  __shared__ __attribute__((aligned(16))) char smem[2 * DEPTH * STAGE];
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, wr = wave >> 1, wc = wave & 1, l31 = lane & 31, h = lane >> 5;
+  // every eighth block runs on the same die: of 64 blocks, those of a die take eight tiles behind each other, which share operands
+  // in its L2
+  int blk = blockIdx.x;
+  if (blk < (int)(gridDim.x & ~63u)) blk = (blk & ~63) + (blk & 7) * 8 + ((blk >> 3) & 7);
+  const int gi = mu_find(tab, blk);
+  const mu_task& g = tab.t[gi];
+  int u = blk - tab.blk0[gi], split = 0, ti, tj, job;
+  const int tm = g.pm / BT, tn = g.pn / BT, per = MODE == MU_SYM ? tm * (tm + 1) / 2 : tm * tn;
+  if (MODE == MU_SYM && g.whole == 0) {      // all tiles split: a matrix's tiles of one part of k are neighbours
+    const int in = u % (per * g.splits);
+    job = u / (per * g.splits);
+    split = in / per;
+    u = job * per + in % per;
+  } else if (MODE == MU_SYM && u >= g.whole) {
+    split = (u - g.whole) % g.splits;
+    u = g.whole + (u - g.whole) / g.splits;
+  }
+  job = u / per;
+  const int t = u - job * per;
+  const bool turned = MODE == MU_LAST && !g.tall;
+  if (MODE == MU_SYM) {
+    mu_triangle(t, tm, &ti, &tj);
+  } else {
+    // (row, column) among tn x tm tiles: in strips of eight rows, a strip column by column; few columns: row by row
+    const int step = tm > 8 ? 8 : 1, strip = t / (step * tm), in = t - strip * step * tm, high = min(step, tn - strip * step);
+    const int row = strip * step + in % high, col = in / high;
+    ti = turned ? col : row;
+    tj = turned ? row : col;
+  }
+  const char* L = mu_at(ws, g, job, turned ? g.r : g.l);
+  const char* R = mu_at(ws, g, job, turned ? g.l : g.r);
+  const int kunits = g.aux;
+  int k0 = 0, stages = kunits / KU;
+  const bool part = MODE == MU_SYM && u >= g.whole;
+  if (part) {                                // splits share the stages evenly
+    const int all = stages;
+    k0 = (int)((int64_t)all * split / g.splits);
+    stages = (int)((int64_t)all * (split + 1) / g.splits) - k0;
   }
   f32x16 acc[TW][TW];
 #pragma unroll
@@ -279,96 +343,101 @@ k_mu_gemm(mu_table tab, mu_jobs jobs, char* ws, float lr) {
 #pragma unroll
       for (int i = 0; i < 16; ++i) acc[a][b][i] = 0.f;
 
-  if constexpr (MODE == MU_GRAM_JOIN) {      // the splits' partial tiles, in order
-    const float* s = (const float*)(base + buf.slab) + (int64_t)t * BT * BT;
-    for (int sp = 0; sp < g.splits; ++sp, s += (int64_t)tri * BT * BT)
+  typedef __attribute__((address_space(3))) void* lds_ptr;
+  typedef const __attribute__((address_space(1))) void* glb_ptr;
+  // a stage: RB row blocks x KU units x 2 KB of each operand; wave w brings in KBs w, w + 4, ...
+  const char* gl = L + (int64_t)ti * RB * kunits * 2048 + (int64_t)k0 * SU + lane * 16;
+  const char* gr = R + (int64_t)tj * RB * kunits * 2048 + (int64_t)k0 * SU + lane * 16;
+  auto issue = [&](int s, int b) {
+    char* dst = smem + b * 2 * STAGE;
+#pragma unroll
+    for (int i = 0; i < NL; ++i) {
+      const int piece = i * 4 + wave;
+      const int64_t at = (int64_t)(piece / (2 * KU)) * kunits * 2048 + (int64_t)s * SU + piece % (2 * KU) * 1024;
+      __builtin_amdgcn_global_load_lds((glb_ptr)(gl + at), (lds_ptr)(dst + piece * 1024), 16, 0, 0);
+      __builtin_amdgcn_global_load_lds((glb_ptr)(gr + at), (lds_ptr)(dst + STAGE + piece * 1024), 16, 0, 0);
+    }
+  };
+#pragma unroll
+  for (int s = 0; s < DEPTH - 1; ++s)
+    if (s < stages) issue(s, s);
+  int cur = 0;
+  for (int s = 0; s < stages; ++s) {
+    // this wave's pieces of stage s have landed (DEPTH - 2 later stages may still be on their way); behind the barrier
+    // everybody's have, and everybody is done with the stage whose place the next issue takes
+    if (DEPTH > 2 && stages - 1 - s >= DEPTH - 2) asm volatile("s_waitcnt vmcnt(%0)" ::"n"((DEPTH - 2) * 2 * NL) : "memory");
+    else asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+    asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
+    if (s + DEPTH - 1 < stages) issue(s + DEPTH - 1, cur == 0 ? DEPTH - 1 : cur - 1);
+    const char* Ls = smem + cur * 2 * STAGE + wr * TW * SU + lane * 16;
+    const char* Rs = smem + cur * 2 * STAGE + STAGE + wc * TW * SU + lane * 16;
+#pragma unroll
+    for (int k = 0; k < KU; ++k) {
+      f16x8 lh[TW], ll[TW], rh[TW], rl[TW];
+#pragma unroll
+      for (int a = 0; a < TW; ++a) {
+        lh[a] = *reinterpret_cast<const f16x8*>(Ls + a * SU + k * 2048);
+        rl[a] = *reinterpret_cast<const f16x8*>(Rs + a * SU + k * 2048 + 1024);
+        ll[a] = *reinterpret_cast<const f16x8*>(Ls + a * SU + k * 2048 + 1024);
+        rh[a] = *reinterpret_cast<const f16x8*>(Rs + a * SU + k * 2048);
+      }
+#pragma unroll
+      for (int a = 0; a < TW; ++a)
+#pragma unroll
+        for (int b = 0; b < TW; ++b) acc[a][b] = __builtin_amdgcn_mfma_f32_32x32x16_f16(lh[a], rl[b], acc[a][b], 0, 0, 0);
+#pragma unroll
+      for (int a = 0; a < TW; ++a)
+#pragma unroll
+        for (int b = 0; b < TW; ++b) acc[a][b] = __builtin_amdgcn_mfma_f32_32x32x16_f16(ll[a], rh[b], acc[a][b], 0, 0, 0);
+#pragma unroll
+      for (int a = 0; a < TW; ++a)
+#pragma unroll
+        for (int b = 0; b < TW; ++b) acc[a][b] = __builtin_amdgcn_mfma_f32_32x32x16_f16(lh[a], rh[b], acc[a][b], 0, 0, 0);
+    }
+    cur = cur + 1 == DEPTH ? 0 : cur + 1;
+  }
+
+  if constexpr (MODE == MU_SYM) {
+    if (part) {
+      float* s = (float*)(ws + (int64_t)g.slab * 256) + ((int64_t)(u - g.whole) * g.splits + split) * BT * BT;
 #pragma unroll
       for (int a = 0; a < TW; ++a)
 #pragma unroll
         for (int b = 0; b < TW; ++b)
 #pragma unroll
-          for (int q = 0; q < 4; ++q) {
-            const float4 v = *reinterpret_cast<const float4*>(s + ((wave * TW + a) * TW + b) * 1024 + q * 256 + lane * 4);
-            acc[a][b][4 * q] += v.x;
-            acc[a][b][4 * q + 1] += v.y;
-            acc[a][b][4 * q + 2] += v.z;
-            acc[a][b][4 * q + 3] += v.w;
-          }
-  } else {
-    typedef __attribute__((address_space(3))) void* lds_ptr;
-    typedef const __attribute__((address_space(1))) void* glb_ptr;
-    // a stage: RB row blocks x (2 units x 2 KB) of each operand; wave w brings in KBs w, w + 4, ...
-    auto issue = [&](int s, int b) {
-      char* dst = smem + b * 2 * STAGE;
-#pragma unroll
-      for (int i = 0; i < RB; ++i) {
-        const int kb = i * 4 + wave;         // 1 KB piece: row block kb / 4, byte (kb % 4) KB of its stage
-        const int64_t at = (int64_t)(kb >> 2) * kunits * 2048 + (int64_t)(k0 + s) * 4096 + (kb & 3) * 1024 + lane * 16;
-        __builtin_amdgcn_global_load_lds((glb_ptr)(L + (int64_t)ti * RB * kunits * 2048 + at), (lds_ptr)(dst + kb * 1024), 16, 0, 0);
-        __builtin_amdgcn_global_load_lds((glb_ptr)(R + (int64_t)tj * RB * kunits * 2048 + at), (lds_ptr)(dst + STAGE + kb * 1024), 16, 0, 0);
-      }
-    };
-    issue(0, 0);
-    for (int s = 0; s < stages; ++s) {
-      // this wave's pieces of stage s have landed; behind the barrier everybody's have, and everybody is done with s - 1
-      asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
-      if (s + 1 < stages) issue(s + 1, (s + 1) & 1);
-      const char* Ls = smem + (s & 1) * 2 * STAGE + wr * TW * 4096 + lane * 16;
-      const char* Rs = smem + (s & 1) * 2 * STAGE + STAGE + wc * TW * 4096 + lane * 16;
-#pragma unroll
-      for (int u = 0; u < 2; ++u) {
-        f16x8 lh[TW], ll[TW], rh[TW], rl[TW];
-#pragma unroll
-        for (int a = 0; a < TW; ++a) {
-          lh[a] = *reinterpret_cast<const f16x8*>(Ls + a * 4096 + u * 2048);
-          ll[a] = *reinterpret_cast<const f16x8*>(Ls + a * 4096 + u * 2048 + 1024);
-          rh[a] = *reinterpret_cast<const f16x8*>(Rs + a * 4096 + u * 2048);
-          rl[a] = *reinterpret_cast<const f16x8*>(Rs + a * 4096 + u * 2048 + 1024);
-        }
-#pragma unroll
-        for (int a = 0; a < TW; ++a)
-#pragma unroll
-          for (int b = 0; b < TW; ++b) acc[a][b] = __builtin_amdgcn_mfma_f32_32x32x16_f16(lh[a], rl[b], acc[a][b], 0, 0, 0);
-#pragma unroll
-        for (int a = 0; a < TW; ++a)
-#pragma unroll
-          for (int b = 0; b < TW; ++b) acc[a][b] = __builtin_amdgcn_mfma_f32_32x32x16_f16(ll[a], rh[b], acc[a][b], 0, 0, 0);
-#pragma unroll
-        for (int a = 0; a < TW; ++a)
-#pragma unroll
-          for (int b = 0; b < TW; ++b) acc[a][b] = __builtin_amdgcn_mfma_f32_32x32x16_f16(lh[a], rh[b], acc[a][b], 0, 0, 0);
-      }
+          for (int q = 0; q < 4; ++q)
+            *reinterpret_cast<float4*>(s + ((wave * TW + a) * TW + b) * 1024 + q * 256 + lane * 4) =
+                make_float4(acc[a][b][4 * q], acc[a][b][4 * q + 1], acc[a][b][4 * q + 2], acc[a][b][4 * q + 3]);
+      return;
     }
   }
-
-  if constexpr (MODE == MU_GRAM_SPLIT) {
-    float* s = (float*)(base + buf.slab) + ((int64_t)split * tri + t) * BT * BT;
-#pragma unroll
-    for (int a = 0; a < TW; ++a)
-#pragma unroll
-      for (int b = 0; b < TW; ++b)
-#pragma unroll
-        for (int q = 0; q < 4; ++q)
-          *reinterpret_cast<float4*>(s + ((wave * TW + a) * TW + b) * 1024 + q * 256 + lane * 4) =
-              make_float4(acc[a][b][4 * q], acc[a][b][4 * q + 1], acc[a][b][4 * q + 2], acc[a][b][4 * q + 3]);
-    return;
-  }
   if constexpr (MODE == MU_LAST) {
-    const mu_ptrs& p = jobs.p[g.first + job];
+    const mu_ptrs& p = jobs->p[g.first + job];
+    float* out = (float*)p.out;
     const int rows = g.tall ? g.n : g.m, cols = g.tall ? g.m : g.n;
-    const float scale = OPT ? lr * p.scale / (MU_SX * MU_SP) : 1.f / (MU_SX * MU_SP);
+    const float scale = OPT ? lr * p.scale * g.s0 : g.s0;
 #pragma unroll
     for (int a = 0; a < TW; ++a)
 #pragma unroll
       for (int b = 0; b < TW; ++b) {
-        const int c = tj * BT + (wc * TW + b) * 32 + l31;
+        const int c = tj * BT + (wc * TW + b) * 32 + l31, r0 = ti * BT + (wr * TW + a) * 32 + 4 * h;
+        if constexpr (OPT) {                 // sixteen loads on their way, then the stores
+          float w[16];
+          int64_t at[16];
 #pragma unroll
-        for (int i = 0; i < 16; ++i) {
-          const int r = ti * BT + (wr * TW + a) * 32 + (i & 3) + 8 * (i >> 2) + 4 * h;
-          if (r < rows && c < cols) {
-            const int64_t at = (int64_t)r * cols + c;
-            if (OPT) p.w[at] -= scale * acc[a][b][i];
-            else ((T*)p.out)[at] = from_f32<T>(scale * acc[a][b][i]);
+          for (int i = 0; i < 16; ++i) {
+            const int r = r0 + (i & 3) + 8 * (i >> 2);
+            at[i] = r < rows && c < cols ? (int64_t)r * cols + c : 0;
+            w[i] = out[at[i]];
+          }
+#pragma unroll
+          for (int i = 0; i < 16; ++i)
+            if (r0 + (i & 3) + 8 * (i >> 2) < rows && c < cols) out[at[i]] = w[i] - scale * acc[a][b][i];
+        } else {
+#pragma unroll
+          for (int i = 0; i < 16; ++i) {
+            const int r = r0 + (i & 3) + 8 * (i >> 2);
+            if (r < rows && c < cols) ((T*)p.out)[(int64_t)r * cols + c] = from_f32<T>(scale * acc[a][b][i]);
           }
         }
       }
@@ -381,95 +450,158 @@ k_mu_gemm(mu_table tab, mu_jobs jobs, char* ws, float lr) {
 #pragma unroll
     for (int b = 0; b < TW; ++b) {
       const int rb = ti * RB + wr * TW + a, cb = tj * RB + wc * TW + b;      // 32-blocks of the result
-      float v[16], w[16];
-#pragma unroll
-      for (int i = 0; i < 16; ++i) {
-        const bool diag = MODE != MU_APPLY && rb == cb && (i & 3) + 8 * (i >> 2) + 4 * h == l31;
-        if (MODE == MU_APPLY) {
-          v[i] = acc[a][b][i] * (1.f / MU_SP);
-        } else if (MODE == MU_POLY) {
-          v[i] = acc[a][b][i] * (MU_SP / (MU_SG * MU_SC)) + (diag ? MU_A * MU_SP : 0.f);
-        } else {
-          v[i] = acc[a][b][i] * (MU_SG / (MU_SX * MU_SX));
-          w[i] = v[i] * (MU_C * MU_SC / MU_SG) + (diag ? MU_B * MU_SC : 0.f);
-        }
-      }
+      float v[16];
       if constexpr (MODE == MU_APPLY) {      // rows of the result: n, columns: m
-        mu_store_cols(v, base + buf.x + ((int64_t)cb * (g.pn / 16) + rb * 2) * 2048, lane);
-        mu_store_rows(v, xt_out + ((int64_t)rb * (g.pm / 16) + cb * 2) * 2048, lane, turn);
+#pragma unroll
+        for (int i = 0; i < 16; ++i) v[i] = acc[a][b][i] * g.s0;
+        mu_store_cols(v, mu_at(ws, g, job, g.d0) + ((int64_t)cb * (g.pn / 16) + rb * 2) * 2048, lane);
+        mu_store_rows(v, mu_at(ws, g, job, g.d1) + ((int64_t)rb * (g.pm / 16) + cb * 2) * 2048, lane, turn);
       } else {
-        char* d0 = base + (MODE == MU_POLY ? buf.p : buf.a);
-        const int64_t at = ((int64_t)cb * (g.pm / 16) + rb * 2) * 2048, mirrored = ((int64_t)rb * (g.pm / 16) + cb * 2) * 2048;
-        mu_store_cols(v, d0 + at, lane);
-        if (MODE != MU_POLY) mu_store_cols(w, base + buf.c + at, lane);
-        if (ti != tj) {
-          mu_store_rows(v, d0 + mirrored, lane, turn);
-          if (MODE != MU_POLY) mu_store_rows(w, base + buf.c + mirrored, lane, turn);
-        }
+#pragma unroll
+        for (int i = 0; i < 16; ++i) v[i] = acc[a][b][i];
+        mu_store_symmetric(g, ws, job, v, rb, cb, ti != tj, lane, turn);
       }
     }
 }
 
+template <int TW, int KU, int DEPTH, int MODE>
+__global__ void __launch_bounds__(256)
+k_mu_gemm(mu_table tab, char* ws) {
+  mu_gemm_tile<f32_t, TW, KU, DEPTH, MODE, false>(tab, nullptr, ws, 0.f);
+}
+template <typename T, int TW, int KU, int DEPTH, bool OPT>
+__global__ void __launch_bounds__(256)
+k_mu_last(mu_table tab, mu_jobs jobs, char* ws, float lr) {
+  mu_gemm_tile<T, TW, KU, DEPTH, MU_LAST, OPT>(tab, &jobs, ws, lr);
+}
+
+// Joins the parts of split tiles, one 32 x 32 block of a tile each wave (blk0 counts tiles).
+template <int TW>
+__global__ void __launch_bounds__(64)
+k_mu_join(mu_table tab, char* ws) {
+  constexpr int BT = 64 * TW, SUB = 4 * TW * TW;
+  __shared__ float turn[32 * 33];
+  const int lane = threadIdx.x, tile = blockIdx.x / SUB, sub = blockIdx.x % SUB;
+  const int gi = mu_find(tab, tile);
+  const mu_task& g = tab.t[gi];
+  const int q0 = tile - tab.blk0[gi], u = g.whole + q0;
+  const int tm = g.pm / BT, per = tm * (tm + 1) / 2, job = u / per;
+  int ti, tj;
+  mu_triangle(u - job * per, tm, &ti, &tj);
+  const float* s = (const float*)(ws + (int64_t)g.slab * 256) + (int64_t)q0 * g.splits * BT * BT + sub * 1024 + lane * 4;
+  float v[16];
+#pragma unroll
+  for (int i = 0; i < 16; ++i) v[i] = 0.f;
+#pragma unroll 4
+  for (int k = 0; k < g.splits; ++k, s += BT * BT)
+#pragma unroll
+    for (int q = 0; q < 4; ++q) {
+      const float4 f = *reinterpret_cast<const float4*>(s + q * 256);
+      v[4 * q] += f.x;
+      v[4 * q + 1] += f.y;
+      v[4 * q + 2] += f.z;
+      v[4 * q + 3] += f.w;
+    }
+  const int wave = sub / (TW * TW), a = sub / TW % TW, b = sub % TW;
+  const int rb = ti * 2 * TW + (wave >> 1) * TW + a, cb = tj * 2 * TW + (wave & 1) * TW + b;
+  mu_store_symmetric(g, ws, job, v, rb, cb, ti != tj, lane, turn);
+}
+
 // ------------------------------------------------------------------------------------------------------- host ----
-struct mu_plan {
-  std::vector<int> order;               // the caller's jobs, sorted by shape
-  std::vector<mu_group> groups;
-  std::vector<int> tw;                  // of each group
-  int64_t bytes;
-};
+#define MU_SLOTS 512      // blocks of 128 x 128 tiles (64 KB of LDS) the chip holds at a time
 
 static int64_t mu_up(int64_t v, int64_t a) { return (v + a - 1) / a * a; }
+
+struct mu_group {
+  int m, n, pm, pn, count, first, tall;
+  bool longish;                        // n >= 2 m: steps in A alone, X every second or third
+  int64_t off, stride;                 // units of 256 bytes
+  int x, xt[2], a, c, p, z, q[2], norm, norm_blocks;
+};
+struct mu_plan {
+  std::vector<int> order;              // the caller's jobs, sorted by shape
+  std::vector<mu_group> groups;
+  int tw;                              // tiles of the products with X: 64 tw
+  int64_t slab, slab_units, units;
+};
+
+// Splits along k of the symmetric products of a launch: `stages` of 32 k, `tiles` in all.
+struct mu_cut { int64_t whole; int splits; };
+// Too few tiles: each in as many parts as fill the chip, four stages a part at least.  Else whole, but for what a last round
+// would leave over, if that is less than half a round (of 4096 x 4096: 16 of 528 tiles, 1.1 rounds instead of 2).
+static mu_cut mu_cut_of(int64_t tiles, int stages, int64_t all_stages, int64_t all_tiles, bool alone, int least) {
+  mu_cut c = {tiles, 1};
+  if (all_tiles < MU_SLOTS) {
+    const int64_t part = std::max<int64_t>(least, (all_stages + MU_SLOTS - 1) / MU_SLOTS);
+    c.splits = (int)std::min<int64_t>(64, std::max<int64_t>(1, (stages + part / 2) / part));
+    if (c.splits > 1) c.whole = 0;
+  } else if (alone) {
+    const int64_t rest = tiles % MU_SLOTS;
+    const int splits = rest ? (int)std::min<int64_t>(std::min<int64_t>(MU_SLOTS / rest, stages / 4), 16) : 1;
+    if (splits > 1) {
+      c.whole = tiles - rest;
+      c.splits = splits;
+    }
+  }
+  return c;
+}
 
 static void mu_make_plan(const lmh_muon_job* jobs, int count, mu_plan* pl) {
   pl->order.resize(count);
   for (int i = 0; i < count; ++i) pl->order[i] = i;
-  auto key = [&](int i) {
-    return std::make_pair(jobs[i].rows, jobs[i].cols);
-  };
+  auto key = [&](int i) { return std::make_pair(jobs[i].rows, jobs[i].cols); };
   std::stable_sort(pl->order.begin(), pl->order.end(), [&](int a, int b) { return key(a) < key(b); });
+  pl->tw = 1;
+  for (int i = 0; i < count; ++i)
+    if (std::min(jobs[i].rows, jobs[i].cols) > 64) pl->tw = 2;
+  const int bt = 64 * pl->tw;
+  int64_t off = 0;
   pl->groups.clear();
-  pl->tw.clear();
-  int64_t tiles_all = 0;
   for (int s = 0; s < count;) {
     int e = s;
     while (e < count && key(pl->order[e]) == key(pl->order[s])) ++e;
     const lmh_muon_job& j = jobs[pl->order[s]];
     mu_group g;
-    memset(&g, 0, sizeof(g));
     g.tall = j.rows > j.cols;
     g.m = g.tall ? j.cols : j.rows;
     g.n = g.tall ? j.rows : j.cols;
-    const int tw = g.m > 64 ? 2 : 1, bt = 64 * tw;
     g.pm = (int)mu_up(g.m, bt);
     g.pn = (int)mu_up(g.n, bt);
     g.count = e - s;
     g.first = s;
-    pl->groups.push_back(g);
-    pl->tw.push_back(tw);
-    const int tm = g.pm / bt;
-    tiles_all += (int64_t)g.count * tm * (tm + 1) / 2;
-    s = e;
-  }
-  int64_t off = 0;
-  for (size_t i = 0; i < pl->groups.size(); ++i) {
-    mu_group& g = pl->groups[i];
-    // the Gram products have few tiles and a long k: split it until the launch has two blocks a compute unit, 8 stages
-    // (256 k) at least to a split
-    int splits = 1;
-    while (tiles_all * splits < 512 && g.pn / 32 / (splits * 2) >= 8 && splits < 16) splits *= 2;
-    g.splits = splits;
-    const mu_buf b = mu_layout(g);
-    g.stride = mu_up(b.end, 256);
+    g.longish = g.pn >= 2 * g.pm;
+    const int mn = (int)((int64_t)g.pm * g.pn / 64), mm = (int)((int64_t)g.pm * g.pm / 64);      // 4 bytes a value, units of 256
+    int at = 0;
+    auto take = [&](int n) { const int r = at; at += n; return r; };
+    g.x = take(mn);
+    g.xt[0] = take(mn);
+    g.xt[1] = take(mn);
+    g.a = take(mm);
+    g.c = take(mm);
+    g.p = take(mm);
+    g.z = g.longish ? take(mm) : -1;
+    g.q[0] = g.longish ? take(mm) : -1;
+    g.q[1] = g.longish ? take(mm) : -1;
+    g.norm_blocks = (int)std::min<int64_t>(MU_NORM_BLOCKS, ((int64_t)g.m * g.n + MU_NORM_ELEMS - 1) / MU_NORM_ELEMS);
+    g.norm = take((int)((g.norm_blocks * sizeof(double) + 255) / 256));
+    g.stride = at;
     g.off = off;
     off += g.stride * g.count;
+    pl->groups.push_back(g);
+    s = e;
   }
-  pl->bytes = off;
+  // a launch's partial tiles: fewer than two for each place on the chip, or 64 parts of the rest of a round
+  pl->slab = off;
+  pl->slab_units = (int64_t)(2 * MU_SLOTS + 64) * bt * bt * 4 / 256;
+  pl->units = off + pl->slab_units;
 }
 
 static bool mu_jobs_ok(const lmh_muon_job* jobs, int count) {
   if (!jobs || count <= 0 || count > LMH_MUON_MAX_JOBS) return false;
   for (int i = 0; i < count; ++i)
-    if (jobs[i].rows <= 0 || jobs[i].cols <= 0 || jobs[i].rows > LMH_MUON_MAX_DIM || jobs[i].cols > LMH_MUON_MAX_DIM) return false;
+    if (jobs[i].rows <= 0 || jobs[i].cols <= 0 || jobs[i].rows > LMH_MUON_MAX_DIM || jobs[i].cols > LMH_MUON_MAX_DIM ||
+        (int64_t)jobs[i].rows * jobs[i].cols > (1 << 30))
+      return false;
   return true;
 }
 
@@ -478,90 +610,260 @@ extern "C" size_t lmh_muon_workspace_bytes(const lmh_muon_job* jobs, int count) 
   try {
     mu_plan pl;
     mu_make_plan(jobs, count, &pl);
-    return (size_t)pl.bytes + 256;
+    return pl.units > 0x7fffffff ? 0 : (size_t)pl.units * 256;
   } catch (...) {
     return 0;
   }
 }
 
+class mu_runner {
+ public:
+  mu_runner(const mu_plan& pl, char* ws, hipStream_t st) : pl_(pl), ws_(ws), st_(st) { memset(&tab_, 0, sizeof(tab_)); }
+
+  // Tasks of the next launch; `fill` sets the operands of one group's task and returns its blocks.
+  template <typename F>
+  int tasks(const std::vector<const mu_group*>& gs, size_t g0, size_t g1, F fill) {
+    int total = 0;
+    clear(&tab_);
+    for (size_t i = g0; i < g1; ++i) {
+      const mu_group& g = *gs[i];
+      mu_task& t = tab_.t[tab_.tasks];
+      base(g, &t);
+      tab_.blk0[tab_.tasks++] = total;
+      total += fill(g, &t);
+    }
+    return total;
+  }
+  void base(const mu_group& g, mu_task* t) const {
+    memset(t, 0, sizeof(*t));
+    t->off = (uint32_t)g.off;
+    t->stride = (uint32_t)g.stride;
+    t->m = g.m;
+    t->n = g.n;
+    t->pm = g.pm;
+    t->pn = g.pn;
+    t->tall = g.tall;
+    t->count = g.count;
+    t->norm = g.norm;
+    t->l = t->r = t->d0 = t->d1 = -1;
+    t->splits = 1;
+    t->whole = 0x7fffffff;
+  }
+
+  static void clear(mu_table* t) {
+    t->tasks = 0;
+    for (int i = 0; i < MU_MAX_GROUPS; ++i) t->blk0[i] = 0x7fffffff;
+  }
+
+  struct product { int l, r, d0, d1, units; float s0, g0, s1, g1; };
+  // Symmetric m x m products of the groups (`make` gives 0, 1 or 2 of a group), tiles of 64 tw.
+  template <typename F>
+  void symmetric(const std::vector<const mu_group*>& gs, int tw, F make) {
+    const int bt = 64 * tw;
+    std::vector<std::pair<const mu_group*, product>> all;
+    for (const mu_group* g : gs) {
+      product p[2];
+      const int n = make(*g, p);
+      for (int i = 0; i < n; ++i) all.push_back({g, p[i]});
+    }
+    for (size_t lo = 0; lo < all.size(); lo += MU_MAX_GROUPS) {
+      const size_t hi = std::min(all.size(), lo + MU_MAX_GROUPS);
+      int64_t tiles = 0, stages = 0;
+      for (size_t i = lo; i < hi; ++i) {
+        const int64_t tm = all[i].first->pm / bt, n = tm * (tm + 1) / 2 * all[i].first->count;
+        tiles += n;
+        stages += n * (all[i].second.units / 2);
+      }
+      int blocks = 0, joins = 0;
+      mu_table join;
+      memset(&join, 0, sizeof(join));
+      clear(&join);
+      clear(&tab_);
+      int64_t slab = pl_.slab;
+      for (size_t i = lo; i < hi; ++i) {
+        const mu_group& g = *all[i].first;
+        const product& p = all[i].second;
+        mu_task& t = tab_.t[tab_.tasks];
+        base(g, &t);
+        t.l = p.l;
+        t.r = p.r;
+        t.d0 = p.d0;
+        t.d1 = p.d1;
+        t.s0 = p.s0;
+        t.g0 = p.g0;
+        t.s1 = p.s1;
+        t.g1 = p.g1;
+        t.aux = p.units;
+        const int64_t tm = g.pm / bt, n = tm * (tm + 1) / 2 * g.count;
+        mu_cut c = mu_cut_of(n, p.units / 2, stages, tiles, hi - lo == 1, tw == 1 ? 16 : 8);
+        const int64_t need = (n - c.whole) * c.splits * bt * bt * 4 / 256;
+        if (slab + need > pl_.slab + pl_.slab_units) c = {n, 1};
+        t.whole = (int)c.whole;
+        t.splits = c.splits;
+        tab_.blk0[tab_.tasks++] = blocks;
+        blocks += (int)(c.whole + (n - c.whole) * c.splits);
+        if (c.whole < n) {
+          t.slab = (uint32_t)slab;
+          slab += need;
+          join.t[join.tasks] = t;
+          join.blk0[join.tasks++] = joins;
+          joins += (int)(n - c.whole);
+        }
+      }
+      // few blocks: one to a compute unit, with more stages on their way
+      if (tw == 1) lmh_launch((k_mu_gemm<1, 2, 4, MU_SYM>), dim3(blocks), dim3(256), 0, st_, tab_, ws_);
+      else if (blocks <= MU_SLOTS / 2) lmh_launch((k_mu_gemm<2, 2, 4, MU_SYM>), dim3(blocks), dim3(256), 0, st_, tab_, ws_);
+      else lmh_launch((k_mu_gemm<2, 2, 2, MU_SYM>), dim3(blocks), dim3(256), 0, st_, tab_, ws_);
+      if (joins) {
+        if (tw == 1) lmh_launch((k_mu_join<1>), dim3(joins * 4), dim3(64), 0, st_, join, ws_);
+        else lmh_launch((k_mu_join<2>), dim3(joins * 16), dim3(64), 0, st_, join, ws_);
+      }
+    }
+  }
+  // X <- polynomial X
+  template <typename F>
+  void apply(const std::vector<const mu_group*>& gs, F operands) {
+    const int bt = 64 * pl_.tw;
+    for (size_t lo = 0; lo < gs.size(); lo += MU_MAX_GROUPS) {
+      const int nb = tasks(gs, lo, std::min(gs.size(), lo + MU_MAX_GROUPS), [&](const mu_group& g, mu_task* t) {
+        operands(g, t);
+        t->aux = g.pm / 16;
+        return (g.pm / bt) * (g.pn / bt) * g.count;
+      });
+      if (pl_.tw == 1) lmh_launch((k_mu_gemm<1, 2, 4, MU_APPLY>), dim3(nb), dim3(256), 0, st_, tab_, ws_);
+      else lmh_launch((k_mu_gemm<2, 2, 2, MU_APPLY>), dim3(nb), dim3(256), 0, st_, tab_, ws_);
+    }
+  }
+  // Launches that take the caller's pointers: at most MU_MAX_JOBS matrices of MU_MAX_GROUPS shapes each.
+  template <typename F, typename L>
+  void with_jobs(const lmh_muon_job* jobs, const std::vector<const mu_group*>& gs, F fill, L launch) {
+    size_t i = 0;
+    int done = 0;                      // matrices of group i
+    while (i < gs.size()) {
+      mu_jobs pj;
+      memset(&pj, 0, sizeof(pj));
+      int n = 0, total = 0;
+      clear(&tab_);
+      while (i < gs.size() && tab_.tasks < MU_MAX_GROUPS && n < MU_MAX_JOBS) {
+        const mu_group& g = *gs[i];
+        const int k = std::min(g.count - done, MU_MAX_JOBS - n);
+        mu_task& t = tab_.t[tab_.tasks];
+        base(g, &t);
+        t.off = (uint32_t)(g.off + done * g.stride);
+        t.count = k;
+        t.first = n;
+        tab_.blk0[tab_.tasks++] = total;
+        total += fill(g, &t) * k;
+        for (int q = 0; q < k; ++q, ++n) {
+          const lmh_muon_job& j = jobs[pl_.order[g.first + done + q]];
+          pj.p[n] = {j.g, j.v, j.w ? (void*)j.w : j.out, j.factor, j.wd, j.scale};
+        }
+        done += k;
+        if (done == g.count) {
+          ++i;
+          done = 0;
+        }
+      }
+      launch(dim3(total), tab_, pj);
+    }
+  }
+
+ private:
+  const mu_plan& pl_;
+  char* ws_;
+  hipStream_t st_;
+  mu_table tab_;
+};
+
 template <typename T, bool OPT>
-static void mu_run(const lmh_muon_job* jobs, int count, const mu_plan& pl, int steps, float eps, float gscale, float mu, int nesterov,
-                   float lr, char* ws, hipStream_t st) {
-  // every launch takes groups and jobs as arguments: at most MU_MAX_GROUPS groups and MU_MAX_JOBS matrices at a time
-  struct range { size_t g0, g1; };
-  std::vector<mu_group> groups;
-  std::vector<int> tws;
-  for (size_t i = 0; i < pl.groups.size(); ++i) {       // groups of more matrices than one launch holds
-    mu_group g = pl.groups[i];
-    for (int done = 0; done < pl.groups[i].count; done += MU_MAX_JOBS) {
-      g.count = std::min(MU_MAX_JOBS, pl.groups[i].count - done);
-      g.off = pl.groups[i].off + (int64_t)done * g.stride;
-      g.first = pl.groups[i].first + done;
-      groups.push_back(g);
-      tws.push_back(pl.tw[i]);
-    }
+static void mu_run(const lmh_muon_job* jobs, const mu_plan& pl, int steps, float eps, float gscale, float mu, int nesterov, float lr,
+                   char* ws, hipStream_t st) {
+  mu_runner run(pl, ws, st);
+  std::vector<const mu_group*> all, gs[2];           // by kind: step by step, long
+  for (const mu_group& g : pl.groups) {
+    all.push_back(&g);
+    gs[g.longish].push_back(&g);
   }
-  std::vector<range> parts;
-  for (size_t i = 0; i < groups.size();) {
-    size_t e = i;
-    int n = 0;
-    while (e < groups.size() && e - i < MU_MAX_GROUPS && n + groups[e].count <= MU_MAX_JOBS) n += groups[e++].count;
-    parts.push_back({i, e});
-    i = e;
-  }
-  for (const range& r : parts) {
-    mu_table tab;
-    mu_jobs pj;
-    memset(&tab, 0, sizeof(tab));
-    memset(&pj, 0, sizeof(pj));
-    const int first = groups[r.g0].first;
-    int n = 0;
-    for (size_t i = r.g0; i < r.g1; ++i)
-      for (int k = 0; k < groups[i].count; ++k, ++n) {
-        const lmh_muon_job& j = jobs[pl.order[groups[i].first + k]];
-        pj.p[n] = {j.g, j.v, j.w, j.out, j.factor, j.wd, j.scale};
+  run.with_jobs(jobs, all, [](const mu_group& g, mu_task* t) {
+    t->aux = g.norm_blocks;
+    t->d0 = g.xt[1];                   // (free until the first product with X has been taken)
+    return g.norm_blocks;
+  }, [&](dim3 nb, const mu_table& tab, const mu_jobs& pj) {
+    lmh_launch((k_mu_norm<T, OPT>), nb, dim3(256), 0, st, tab, pj, ws, mu, nesterov, gscale);
+  });
+  run.with_jobs(jobs, all, [](const mu_group& g, mu_task* t) {
+    t->aux = g.norm_blocks;
+    t->l = g.xt[1];
+    t->d0 = g.x;
+    t->d1 = g.xt[0];
+    return (g.pm / 64) * (g.pn / 64);
+  }, [&](dim3 nb, const mu_table& tab, const mu_jobs& pj) {
+    lmh_launch((k_mu_planes<T, OPT>), nb, dim3(256), 0, st, tab, pj, ws, eps);
+  });
+  for (int kind = 0; kind < 2; ++kind) {
+    const std::vector<const mu_group*>& G = gs[kind];
+    if (G.empty()) continue;
+    // m x m products: 64 x 64 tiles while those of 128 x 128 would leave places free
+    int64_t tiles = 0;
+    for (const mu_group* g : G) tiles += (int64_t)g->count * (g->pm / 128) * (g->pm / 128 + 1) / 2;
+    const int tw = pl.tw == 2 && tiles >= MU_SLOTS / 2 ? 2 : 1;
+    int flip = 0;
+    for (int done = 0; done < steps;) {
+      const int left = steps - done, len = kind == 0 ? 1 : left == 4 ? 2 : std::min(left, 3);
+      // A = X X' and b I + c A
+      run.symmetric(G, pl.tw, [](const mu_group& g, mu_runner::product* p) {
+        const float s = 1.f / (MU_SX * MU_SX);
+        p[0] = {g.x, g.x, g.a, g.c, g.pn / 16, MU_SG * s, 0.f, MU_C * MU_SC * s, MU_B * MU_SC};
+        return 1;
+      });
+      int q = 0;                       // of a run of several steps: their product so far in q[q]
+      for (int k = 0; k < len; ++k) {
+        // p = (b I + c A) A + a I; the first of several is their product too
+        run.symmetric(G, tw, [&](const mu_group& g, mu_runner::product* p) {
+          const float s = 1.f / (MU_SC * MU_SG);
+          p[0] = {g.c, g.a, g.p, k == 0 && len > 1 ? g.q[0] : -1, g.pm / 16, MU_SP * s, MU_A * MU_SP, MU_SQ * s, MU_A * MU_SQ};
+          return 1;
+        });
+        if (len == 1) break;
+        // z = p A unless this is the last of them, Q <- p Q unless it is the first
+        run.symmetric(G, tw, [&](const mu_group& g, mu_runner::product* p) {
+          int n = 0;
+          if (k + 1 < len) p[n++] = {g.p, g.a, g.z, -1, g.pm / 16, MU_SG / (MU_SP * MU_SG), 0.f, 0.f, 0.f};
+          if (k > 0) p[n++] = {g.p, g.q[q], g.q[1 - q], -1, g.pm / 16, MU_SQ / (MU_SP * MU_SQ), 0.f, 0.f, 0.f};
+          return n;
+        });
+        if (k > 0) q = 1 - q;
+        if (k + 1 < len) {
+          run.symmetric(G, tw, [&](const mu_group& g, mu_runner::product* p) {      // A <- z p
+            const float s = 1.f / (MU_SG * MU_SP);
+            p[0] = {g.z, g.p, g.a, g.c, g.pm / 16, MU_SG * s, 0.f, MU_C * MU_SC * s, MU_B * MU_SC};
+            return 1;
+          });
+        }
       }
-    // blocks(g): of one matrix; tw 0: all groups
-    auto fill = [&](int tw, auto blocks) {
-      int total = 0, k = 0;
-      for (size_t i = r.g0; i < r.g1; ++i) {
-        if (tw && tws[i] != tw) continue;
-        const int per = blocks(groups[i]);
-        if (per == 0) continue;
-        tab.g[k] = groups[i];
-        tab.g[k].first -= first;
-        tab.g[k].blk0 = total;
-        tab.g[k].job_blocks = per;
-        total += per * groups[i].count;
-        ++k;
+      done += len;
+      auto operands = [&](const mu_group& g, mu_task* t) {
+        t->l = g.xt[flip];
+        t->r = len > 1 ? g.q[q] : g.p;
+        t->d0 = g.x;
+        t->d1 = g.xt[1 - flip];
+        t->s0 = len > 1 ? 1.f / MU_SQ : 1.f / MU_SP;
+      };
+      if (done < steps) {
+        run.apply(G, operands);
+        flip = 1 - flip;
+      } else {
+        run.with_jobs(jobs, G, [&](const mu_group& g, mu_task* t) {
+          operands(g, t);
+          t->s0 /= MU_SX;
+          t->aux = g.pm / 16;
+          return (g.pm / (64 * pl.tw)) * (g.pn / (64 * pl.tw));
+        }, [&](dim3 nb, const mu_table& tab, const mu_jobs& pj) {
+          if (pl.tw == 1) lmh_launch((k_mu_last<T, 1, 2, 4, OPT>), nb, dim3(256), 0, st, tab, pj, ws, lr);
+          else lmh_launch((k_mu_last<T, 2, 2, 2, OPT>), nb, dim3(256), 0, st, tab, pj, ws, lr);
+        });
       }
-      tab.groups = k;
-      return total;
-    };
-    int nb = fill(0, [](const mu_group&) { return MU_NORM_BLOCKS; });
-    lmh_launch((k_mu_norm<T, OPT>), dim3(nb), dim3(256), 0, st, tab, pj, ws, mu, nesterov, gscale);
-    nb = fill(0, [](const mu_group& g) { return (g.pm / 64) * (g.pn / 64); });
-    lmh_launch((k_mu_planes<T, OPT>), dim3(nb), dim3(256), 0, st, tab, pj, ws, MU_NORM_BLOCKS, eps);
-#define MU_GEMM(MODE_, BLOCKS_)                                                                                \
-  do {                                                                                                         \
-    for (int tw = 1; tw <= 2; ++tw) {                                                                          \
-      const int bt = 64 * tw;                                                                                  \
-      nb = fill(tw, [&](const mu_group& g) { const int tm = g.pm / bt, tri = tm * (tm + 1) / 2, tn = g.pn / bt; (void)tri; (void)tn; return (BLOCKS_); }); \
-      if (nb == 0) continue;                                                                                   \
-      if (tw == 1) lmh_launch((k_mu_gemm<T, 1, MODE_, OPT>), dim3(nb), dim3(256), 0, st, tab, pj, ws, lr);     \
-      else lmh_launch((k_mu_gemm<T, 2, MODE_, OPT>), dim3(nb), dim3(256), 0, st, tab, pj, ws, lr);             \
-    }                                                                                                          \
-  } while (0)
-    for (int it = 0; it < steps; ++it) {
-      tab.flip = it & 1;
-      MU_GEMM(MU_GRAM, (g.splits == 1 ? tri : 0));
-      MU_GEMM(MU_GRAM_SPLIT, (g.splits > 1 ? tri * g.splits : 0));
-      MU_GEMM(MU_GRAM_JOIN, (g.splits > 1 ? tri : 0));
-      MU_GEMM(MU_POLY, tri);
-      if (it + 1 < steps) MU_GEMM(MU_APPLY, tm * tn);
-      else MU_GEMM(MU_LAST, tm * tn);
     }
-#undef MU_GEMM
   }
 }
 
@@ -573,7 +875,12 @@ static int mu_check(const lmh_muon_job* jobs, int count, int steps, float eps, v
     lmh_set_error("lmh_muon: out of host memory");
     return LMH_ERR_INVALID;
   }
-  if (!ws || ws_bytes < (size_t)pl->bytes) {
+  LMH_CHECK_ARG(pl->units <= 0x7fffffff);
+  // a launch has fewer than 2^32 threads
+  int64_t most = 0;
+  for (const mu_group& g : pl->groups) most += (int64_t)g.count * (g.pm / 64) * (g.pn / 64);
+  LMH_CHECK_ARG(most < 0xffffff);
+  if (!ws || ws_bytes < (size_t)pl->units * 256) {
     lmh_set_error("lmh_muon: workspace too small");
     return LMH_ERR_WORKSPACE;
   }
@@ -589,9 +896,9 @@ extern "C" int lmh_orthogonalize(const lmh_muon_job* jobs, int count, int dtype,
   for (int i = 0; i < count; ++i) LMH_CHECK_ARG(jobs[i].g && jobs[i].out);
   hipStream_t st = (hipStream_t)stream;
   try {
-    if (dtype == LMH_F32) mu_run<f32_t, false>(jobs, count, pl, steps, eps, 1.f, 0.f, 0, 0.f, (char*)ws, st);
-    else if (dtype == LMH_F16) mu_run<f16_t, false>(jobs, count, pl, steps, eps, 1.f, 0.f, 0, 0.f, (char*)ws, st);
-    else mu_run<bf16_t, false>(jobs, count, pl, steps, eps, 1.f, 0.f, 0, 0.f, (char*)ws, st);
+    if (dtype == LMH_F32) mu_run<f32_t, false>(jobs, pl, steps, eps, 1.f, 0.f, 0, 0.f, (char*)ws, st);
+    else if (dtype == LMH_F16) mu_run<f16_t, false>(jobs, pl, steps, eps, 1.f, 0.f, 0, 0.f, (char*)ws, st);
+    else mu_run<bf16_t, false>(jobs, pl, steps, eps, 1.f, 0.f, 0, 0.f, (char*)ws, st);
   } catch (...) {
     lmh_set_error("lmh_orthogonalize: out of host memory");
     return LMH_ERR_INVALID;
@@ -607,7 +914,7 @@ extern "C" int lmh_muon_step(const lmh_muon_job* jobs, int count, int steps, flo
   if (rc != LMH_OK) return rc;
   for (int i = 0; i < count; ++i) LMH_CHECK_ARG(jobs[i].g && jobs[i].v && jobs[i].w);
   try {
-    mu_run<f32_t, true>(jobs, count, pl, steps, eps, gscale, momentum, nesterov, lr, (char*)ws, (hipStream_t)stream);
+    mu_run<f32_t, true>(jobs, pl, steps, eps, gscale, momentum, nesterov, lr, (char*)ws, (hipStream_t)stream);
   } catch (...) {
     lmh_set_error("lmh_muon_step: out of host memory");
     return LMH_ERR_INVALID;

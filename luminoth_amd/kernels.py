@@ -1476,14 +1476,19 @@ def optimizer_step(kind, w, g, slot1, slot2, seg_offset, seg_wd, seg_factor, lr,
                                  float(eps), float(gscale), _stream()), 'lmh_optimizer_step')
 
 
-MUON_MAX_DIM = 32768
+MUON_MAX_DIM = 1 << 17
+
+
+def muon_fits(rows, cols):
+    """Whether the Newton-Schulz kernels take a matrix of this size."""
+    return max(rows, cols) <= MUON_MAX_DIM and rows * cols <= 1 << 30
 
 
 def _matrix_of(t, what):
     """(..., out) weights as the matrix (inputs, out): HWIO kernels flattened like a Linear's (in, out)."""
     _refuse(t.dim() < 2 or t.numel() == 0, '%s: matrices expected, got shape %s', what, tuple(t.shape))
     rows, cols = t.numel() // t.shape[-1], t.shape[-1]
-    _refuse(max(rows, cols) > MUON_MAX_DIM, '%s: at most %d rows and columns, got %d x %d', what, MUON_MAX_DIM, rows, cols)
+    _refuse(not muon_fits(rows, cols), '%s: at most %d rows and columns and 2^30 values, got %d x %d', what, MUON_MAX_DIM, rows, cols)
     return rows, cols
 
 
@@ -1518,15 +1523,16 @@ class MuonJobs(object):
     """Weights, gradients and momentum (lists of float32 tensors of one shape each) as the descriptors of lmh_muon_step, made
     once by an optimizer whose buffers stay where they are.  weight_decay: a number or one per matrix; scale: one factor of
     the update per matrix, by default 0.2 sqrt(max(rows, cols)) - an orthogonal matrix then has the root mean square of an
-    Adam update, 0.2; factors: (n,) float32 device tensor of gradient factors (grad_clip_factors) or None."""
+    Adam update, 0.2; factors: one float32 device value per matrix that multiplies its gradient (elements of
+    grad_clip_factors' result), or None."""
 
     def __init__(self, params, grads, moms, weight_decay=0.0, scale=None, factors=None):
         params, grads, moms = list(params), list(grads), list(moms)
         n = len(params)
         _refuse(n == 0 or len(grads) != n or len(moms) != n, 'muon: as many gradients and momenta as weights expected')
-        _refuse(factors is not None and (tuple(factors.shape) != (n,) or factors.dtype != torch.float32),
-                'muon: float32 factors of shape (%d,) expected', n)
-        self.tensors = params + grads + moms + ([factors] if factors is not None else [])
+        factors = [] if factors is None else list(factors)
+        _refuse(factors and (len(factors) != n or any(f.numel() != 1 for f in factors)), 'muon: one factor per matrix expected')
+        self.tensors = params + grads + moms + factors
         self.jobs, self.count = (_lib.MuonJob * n)(), n
         for t in self.tensors:
             _refuse(t.dtype != torch.float32, 'muon: float32 expected, got %s', t.dtype)
@@ -1539,7 +1545,7 @@ class MuonJobs(object):
         _same_device(*self.tensors)
         for i, (j, w, g, v) in enumerate(zip(self.jobs, params, grads, moms)):
             j.w, j.g, j.v = _p(w).value, _p(g).value, _p(v).value
-            j.factor = factors.data_ptr() + 4 * i if factors is not None else None
+            j.factor = _p(factors[i]).value if factors else None
         # what is written must be nobody else's: a matrix given twice, or overlapping views, would be updated by two blocks at a time
         spans = sorted((t.data_ptr(), t.data_ptr() + 4 * t.numel()) for t in params + moms)
         _refuse(any(a[1] > b[0] for a, b in zip(spans, spans[1:])), 'muon: weights and momenta overlap')

@@ -3,7 +3,11 @@ luminoth/models/fasterrcnn/rcnn.py:14-411): targets + training-batch
 compaction, fused ROI crop-pooling, the base network tail (ResNet-101 block4),
 spatial mean, optional FC stack, classifier / bbox FC heads, softmax, the final
 per-class NMS proposals and the RCNN loss.  Sonnet Linear names:
-`<scope>/rcnn/{fc_i,fc_classifier,fc_bbox}/{w,b}`."""
+`<scope>/rcnn/{fc_i,fc_classifier,fc_bbox}/{w,b}`.
+
+Two keys the reference does not have: `layer_norm: True` normalises the output of every layer of the FC stack (variables
+`<scope>/rcnn/fc_i/LayerNorm/{gamma,beta}`), `top_alternatives: k` gives the k most probable classes of every proposal
+(background is class 0) with their log probabilities and the entropy in `pred['rcnn']['alternatives']` at inference."""
 import torch
 
 from luminoth_amd import autograd as A
@@ -38,6 +42,13 @@ class RCNN(object):
                                           init=get_initializer(config.rcnn_initializer, seed),
                                           weight_name='w', bias_name='b'))
             in_feat = size
+        # names of gamma, beta behind each layer of the stack
+        self._norms = [tuple('%s/fc_%d/LayerNorm/%s' % (p, i, v) for v in ('gamma', 'beta')) for i in range(len(self._layer_sizes))] \
+            if config.get('layer_norm') else [None] * len(self._layer_sizes)
+        self._top_alternatives = int(config.get('top_alternatives') or 0)
+        if not 0 <= self._top_alternatives <= min(K.LOG_PROBS_MAX_TOP, num_classes + 1):
+            raise ValueError('top_alternatives: 0 to %d expected, got %r' % (min(K.LOG_PROBS_MAX_TOP, num_classes + 1),
+                                                                             config.get('top_alternatives')))
         self._classifier_layer = ConvLayer(p + '/fc_classifier', in_feat, num_classes + 1, 1, padding='VALID',
                                            act=None, norm='bias', wd=wd,
                                            init=get_initializer(config.cls_initializer, seed),
@@ -56,12 +67,19 @@ class RCNN(object):
             # Sonnet Linear weights are (in, out): stored as the HWIO view (1,1,in,out)
             store.add(l.w_name, (l.cin, l.cout), l.init, trainable=True, wd=l.wd)
             store.add(l.b_name, (l.cout,), zeros, trainable=True)
+        ones = lambda shape, gen: torch.ones(shape)
+        for l, norm in zip(self._layers, self._norms):
+            if norm is not None:
+                store.add(norm[0], (l.cout,), ones, trainable=True)
+                store.add(norm[1], (l.cout,), zeros, trainable=True)
 
     def bind(self, store):
         for l in self.layers:
             l.bind(store, None)
             l.w = store[l.w_name].view(1, 1, l.cin, l.cout)
             l.gw = store.grads[l.w_name].view(1, 1, l.cin, l.cout)
+        # (gamma, beta, their gradients) of each norm
+        self._norm_vars = [None if n is None else (store[n[0]], store[n[1]], store.grads[n[0]], store.grads[n[1]]) for n in self._norms]
         self._anchor = torch.zeros(1, device=store.flat.device, requires_grad=True)
 
     def _dropout(self, net, is_training):
@@ -109,14 +127,20 @@ class RCNN(object):
             else:
                 net = features.reshape(features.shape[0], -1)
         net = self._dropout(net, is_training)                          # rcnn.py:196
-        for layer in self._layers:
-            net = self._dropout(self._linear(layer, net), is_training)   # rcnn.py:214-218
+        for layer, norm in zip(self._layers, self._norm_vars):
+            net = self._linear(layer, net)
+            if norm is not None:
+                net = A.StoredLayerNormFn.apply(net, self._anchor, norm)
+            net = self._dropout(net, is_training)                        # rcnn.py:214-218
         cls_score = self._linear(self._classifier_layer, net)          # (B*R, C+1)
         bbox_offsets = self._linear(self._bbox_layer, net)             # (B*R, 4C)
         cls_prob = K.softmax(cls_score.detach())
         C = self._num_classes
         pred['rcnn'] = {'cls_score': cls_score.reshape(B, R, C + 1), 'cls_prob': cls_prob.reshape(B, R, C + 1),
                         'bbox_offsets': bbox_offsets.reshape(B, R, 4 * C)}
+        if self._top_alternatives and not is_training:
+            _, entropy, logp, index, _ = K.log_probs_fwd(pred['rcnn']['cls_score'].detach(), None, self._top_alternatives)
+            pred['rcnn']['alternatives'] = {'classes': index, 'log_probs': logp, 'entropy': entropy}
         pred['proposals'] = proposals
         pred['num_proposals'] = prop_count
         if not is_training or self._debug:
@@ -178,9 +202,13 @@ class RCNN(object):
             steps.append(('drop', float(kp), seed))
             return K.dropout(x, float(kp), seed)
         net = drop(net)
-        for layer in self._layers:
+        for layer, norm in zip(self._layers, self._norm_vars):
             y = self._linear_fwd(layer, net)
             steps.append(('fc', layer, net, y))
+            if norm is not None:
+                z, mean, rstd = K.layer_norm_fwd(y, norm[0], norm[1])
+                steps.append(('norm', norm, y, mean, rstd))
+                y = z
             net = drop(y)
         cls_score = self._linear_fwd(self._classifier_layer, net)
         bbox_offsets = self._linear_fwd(self._bbox_layer, net)
@@ -204,6 +232,9 @@ class RCNN(object):
         for st in reversed(ctx['steps']):
             if st[0] == 'drop':
                 d = K.dropout(d.contiguous(), st[1], st[2])
+            elif st[0] == 'norm':
+                _, (gamma, _, dgamma, dbeta), x_in, mean, rstd = st
+                d = K.layer_norm_bwd(d, x_in, mean, rstd, gamma, dgamma, dbeta)
             else:
                 _, layer, x_in, y = st
                 d = self._linear_bwd(layer, x_in, y, d)

@@ -17,7 +17,7 @@ import torch.distributed as dist
 from luminoth_amd import kernels as K
 
 FUSED_STEP = os.environ.get('LUMINOTH_AMD_FUSED_STEP', '1') != '0'
-OPTIMIZERS = {'momentum', 'gradient_descent', 'adam', 'rmsprop'}
+OPTIMIZERS = {'momentum', 'gradient_descent', 'adam', 'rmsprop', 'muon'}
 LEARNING_RATE_DECAY_METHODS = {'piecewise_constant', 'exponential_decay'}
 
 
@@ -507,6 +507,65 @@ class RMSPropOptimizer(MomentumOptimizer):
                          factors, lr, self.decay, self.momentum, self.epsilon, gscale, slot3=self._slot3)
 
 
+class MuonOptimizer(MomentumOptimizer):
+    """Muon (no reference counterpart): the update of a weight matrix is its (Nesterov) momentum made orthogonal by Newton-Schulz
+    products, w -= lr * 0.2 sqrt(max(rows, cols)) * O(momentum) (kernels.muon_jobs_step; HWIO kernels count as (inputs, out)).
+    The factor gives O the root mean square 0.2 of an Adam update, so that ONE learning rate serves both: biases, BatchNorm and
+    LayerNorm parameters, matrices of one row or column or beyond the kernel's sizes, and variables whose name contains a
+    string of `exclude` take Adam.  As with every optimizer here the L2 term is part of the gradient (total_loss holds it) and
+    `train.clip_by_norm` acts on g + wd * w per variable."""
+    KIND = 5
+
+    def __init__(self, model, train_config, momentum=0.95, use_nesterov=True, ns_steps=5, epsilon=1e-7, beta1=0.9, beta2=0.95,
+                 adam_epsilon=1e-8, exclude=()):
+        super(MuonOptimizer, self).__init__(model, train_config, momentum=momentum, use_nesterov=use_nesterov)
+        self.ns_steps, self.epsilon = int(ns_steps), float(epsilon)
+        if not 1 <= self.ns_steps <= 64 or not self.epsilon > 0:
+            raise ValueError('muon: ns_steps in 1..64 and epsilon > 0 expected, got %r and %r' % (ns_steps, epsilon))
+        self.beta1, self.beta2, self.adam_epsilon = float(beta1), float(beta2), float(adam_epsilon)
+        exclude = [exclude] if isinstance(exclude, str) else list(exclude or ())
+        st = self.store
+        self.matrices, self.adam_runs = [], []       # names; (first segment, last segment + 1, lo, hi) of the flat buffer
+        names = st.trainable_names()
+        bounds = [st.offsets[n][1] for n in names] + [int(st.flat.numel())]
+        for i, n in enumerate(names):
+            shape = st.specs[n].shape
+            cols = shape[-1] if shape else 1
+            rows = st.offsets[n][2] // max(cols, 1)
+            if len(shape) >= 2 and min(rows, cols) > 1 and K.muon_fits(rows, cols) and not any(e in n for e in exclude):
+                self.matrices.append(n)
+            elif self.adam_runs and self.adam_runs[-1][1] == i:
+                self.adam_runs[-1] = (self.adam_runs[-1][0], i + 1, self.adam_runs[-1][2], bounds[i + 1])
+            else:
+                self.adam_runs.append((i, i + 1, bounds[i], bounds[i + 1]))
+        self._index = {n: i for i, n in enumerate(names)}
+        self._slot2 = torch.zeros_like(st.mom)
+        self._run_tables = [(st.seg_offset[a:b + 1] - lo, st.seg_wd[a:b]) for a, b, lo, _ in self.adam_runs]
+        self._jobs = None
+
+    @property
+    def _t(self):
+        return self.global_step + 1          # (as AdamOptimizer: the bias correction goes by the restored step)
+
+    def _muon_jobs(self, factors):
+        if self._jobs is None:               # the store's buffers and the factors' stay where they are
+            st = self.store
+            mom = {n: st.mom[st.offsets[n][1]:st.offsets[n][1] + st.offsets[n][2]].view(st.specs[n].shape) for n in self.matrices}
+            self._jobs = K.MuonJobs([st[n] for n in self.matrices], [st.grads[n] for n in self.matrices],
+                                    [mom[n] for n in self.matrices], [st.specs[n].wd for n in self.matrices],
+                                    factors=None if factors is None else [factors[self._index[n]] for n in self.matrices])
+        return self._jobs
+
+    def _update(self, lr, gscale, factors):
+        st = self.store
+        if self.matrices:
+            K.muon_jobs_step(self._muon_jobs(factors), lr, self.momentum, self.use_nesterov, self.ns_steps, self.epsilon, gscale)
+        lr_t = lr * (1.0 - self.beta2 ** self._t) ** 0.5 / (1.0 - self.beta1 ** self._t)
+        for (a, b, lo, hi), (seg_offset, seg_wd) in zip(self.adam_runs, self._run_tables):
+            K.optimizer_step(1, st.flat[lo:hi], st.grad[lo:hi], st.mom[lo:hi], self._slot2[lo:hi], seg_offset, seg_wd,
+                             None if factors is None else factors[a:b], lr_t, self.beta1, self.beta2, self.adam_epsilon, gscale)
+
+
 def get_optimizer(train_config, model):
     """training.py:64-81: OPTIMIZERS[type](learning_rate, **remaining optimizer config)."""
     opt = dict(train_config.optimizer)
@@ -532,6 +591,9 @@ def get_optimizer(train_config, model):
         return MomentumOptimizer(model, train_config, momentum=0.0)
     if kind == 'adam':
         return AdamOptimizer(model, train_config, **take(('beta1', 'beta2', 'epsilon')))
+    if kind == 'muon':
+        return MuonOptimizer(model, train_config, **take(('momentum', 'use_nesterov', 'ns_steps', 'epsilon', 'beta1', 'beta2',
+                                                          'adam_epsilon', 'exclude')))
     return RMSPropOptimizer(model, train_config, **take(('decay', 'momentum', 'epsilon', 'centered')))
 
 

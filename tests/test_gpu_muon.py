@@ -60,14 +60,18 @@ def test_orthogonalize(rows, cols, dtype):
 
 
 def test_many_matrices_at_once():
-    """More shapes and matrices than one launch takes; HWIO kernels count as (inputs, out); the result of each is the same alone."""
+    """More shapes and matrices than one launch takes; HWIO kernels count as (inputs, out); a matrix alone."""
     mats = [make(5 + 3 * (i % 31), 4 + 7 * (i % 29), seed=i) for i in range(101)] + [make(288, 40).view(3, 3, 32, 40)]
     got = K.orthogonalize([m.cuda() for m in mats])
     for m, o in zip(mats, got):
         assert o.shape == m.shape
         close(o.view(-1, o.shape[-1]), m.view(-1, m.shape[-1]))
+    # how a product's k is split, and so the order of its additions, goes by the whole list: each result is within bound() of the
+    # exact one, so two of them are within twice that of each other
     alone, = K.orthogonalize([mats[50].cuda()])
-    assert torch.equal(alone, got[50])
+    close(alone, mats[50])
+    assert float(torch.linalg.norm(alone.double() - got[50].double())) <= 2 * bound(mats[50])
+    assert torch.equal(alone, K.orthogonalize([mats[50].cuda()])[0])
     assert K.orthogonalize([]) == []
 
 

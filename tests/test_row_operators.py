@@ -48,7 +48,7 @@ def z(*shape, dtype=F):
     (lambda: K.orthogonalize([z(8)]), 'matrices expected'),
     (lambda: K.orthogonalize([z(8, 0)]), 'matrices expected'),
     (lambda: K.orthogonalize([z(8, 4), z(8, 4, dtype=H)]), 'one type'),
-    (lambda: K.orthogonalize([z(40000, 1)]), 'at most'),
+    (lambda: K.orthogonalize([z((1 << 17) + 1, 1)]), 'at most'),
     (lambda: K.orthogonalize([z(4, 8)], steps=0), 'steps'),
     (lambda: K.orthogonalize([z(4, 8)], eps=0.0), 'eps'),
     (lambda: K.muon_step([z(4, 8)], [z(4, 8)], [z(4, 8)], lr=0.1), 'ROCm device'),
@@ -56,7 +56,7 @@ def z(*shape, dtype=F):
     (lambda: K.muon_step([], [], [], lr=0.1), 'as many'),
     (lambda: K.muon_step([z(4, 8)], [z(8, 4)], [z(4, 8)], lr=0.1), 'one shape'),
     (lambda: K.muon_step([z(4, 8, dtype=H)], [z(4, 8)], [z(4, 8)], lr=0.1), 'float32 expected'),
-    (lambda: K.muon_step([z(4, 8)], [z(4, 8)], [z(4, 8)], lr=0.1, factors=z(2)), 'factors'),
+    (lambda: K.muon_step([z(4, 8)], [z(4, 8)], [z(4, 8)], lr=0.1, factors=z(2)), 'one factor'),
 ])
 def test_refusals(call, text):
     with pytest.raises(Err, match=text):
@@ -96,6 +96,44 @@ def test_c_entries_refuse_before_they_launch():
         assert orth(**bad) == -1, bad                      # (the last: no input and no output)
     assert orth(ws=None) == -3 and orth(size=need // 2) == -3
     assert lib.lmh_muon_step(job, 1, 5, 1e-7, 1.0, 0.9, 1, 0.1, p, need, None) == -1
-    for rows, cols in ((0, 8), (4, -1), (32769, 1)):
+    for rows, cols in ((0, 8), (4, -1), ((1 << 17) + 1, 1), (1 << 16, 1 << 15)):
         job[0].rows, job[0].cols = rows, cols
         assert lib.lmh_muon_workspace_bytes(job, 1) == 0 and orth() == -1
+
+
+def small_store():
+    from luminoth_amd.params import ParamStore
+    st = ParamStore()
+    zeros = lambda shape, gen: torch.zeros(shape)                                  # noqa: E731
+    for name, shape, wd in (('a/conv/weights', (3, 3, 4, 8), 0.1), ('a/conv/beta', (8,), 0.0), ('a/conv/gamma', (8,), 0.0),
+                            ('b/fc/w', (10, 6), 0.2), ('b/fc/b', (6,), 0.0), ('b/col/w', (9, 1), 0.0), ('b/out/w', (6, 3), 0.0)):
+        st.add(name, shape, zeros, wd=wd)
+    return st.build('cpu')
+
+
+def test_muon_takes_the_matrices_and_adam_the_rest():
+    from luminoth_amd.utils import training as T
+    from luminoth_amd.utils.config import get_config
+
+    class Model(object):
+        store = small_store()
+
+    def make(**opt):
+        cfg = get_config({'model': {'type': 'fasterrcnn'}, 'train': {'optimizer': dict(opt, _replace=True, type='muon')}})
+        return T.get_optimizer(cfg.train, Model)
+    opt = make(exclude=['out'])
+    assert (opt.momentum, opt.use_nesterov, opt.ns_steps) == (0.95, True, 5)
+    assert opt.matrices == ['a/conv/weights', 'b/fc/w']
+    off = Model.store.offsets
+    assert [(a, b) for a, b, _, _ in opt.adam_runs] == [(1, 3), (4, 7)]
+    assert [lo for _, _, lo, _ in opt.adam_runs] == [off['a/conv/beta'][1], off['b/fc/b'][1]]
+    for (a, b, lo, hi), (seg, wd) in zip(opt.adam_runs, opt._run_tables):
+        assert int(seg[0]) == 0 and int(seg[-1]) == hi - lo and wd.numel() == b - a
+    assert opt.adam_runs[-1][3] == Model.store.flat.numel()
+    assert make(momentum=0.8, use_nesterov=False, ns_steps=3).ns_steps == 3 and 'b/out/w' in make().matrices
+    with pytest.raises(TypeError, match='decay'):
+        make(decay=0.9)
+    with pytest.raises(ValueError, match='ns_steps'):
+        make(ns_steps=0)
+    with pytest.raises(Err, match='ROCm device'):
+        opt.step()
