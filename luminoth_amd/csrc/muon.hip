@@ -43,7 +43,7 @@
 #define MU_MAX_GROUPS 24  // of one launch (kernel arguments: under 4 KB together)
 #define MU_MAX_JOBS 44
 #define MU_NORM_BLOCKS 256
-#define MU_NORM_ELEMS 8192    // at least this many per block of k_mu_norm
+#define MU_NORM_ELEMS 2048    // at least this many per block of k_mu_norm
 
 typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
 typedef float f32x16 __attribute__((ext_vector_type(16)));
@@ -212,50 +212,56 @@ k_mu_planes(mu_table tab, mu_jobs jobs, char* ws, float eps) {
 }
 
 // ---- products ------------------------------------------------------------------------------------------------
-// The 32 x 32 accumulator (lane: column lane & 31, register i: row (i & 3) + 8 (i >> 2) + 4 (lane >> 5)) as planes whose rows
-// are its COLUMNS and whose k are its rows: two 16-k units at `out` (+ 2048).
-__device__ __forceinline__ void mu_store_cols(const float* v, char* out, int lane) {
+// The 32 x 32 accumulator (lane: column lane & 31, register i: row (i & 3) + 8 (i >> 2) + 4 (lane >> 5)) as planes:
+//  cols: rows = its COLUMNS, k = its rows, two 16-k units at `cols` (+ 2048): pairs of registers are pairs along k, and the lane
+//        halves trade so that a lane has eight successive ones;
+//  rows: the other way round, if wanted: hi and lo of a value as one word through `turn`, 32 x MU_PITCH words of this wave's LDS.
+#define MU_PITCH 40      // writes of the two lane halves (four rows apart) hit the two halves of the banks; 16-byte rows
+typedef _Float16 f16x2 __attribute__((ext_vector_type(2)));
+typedef float f32x2 __attribute__((ext_vector_type(2)));
+__device__ __forceinline__ void mu_store(const float* v, char* cols, char* rows, int lane, uint32_t* turn) {
+  uint32_t hi[8], lo[8];                     // of registers 2 j, 2 j + 1
 #pragma unroll
-  for (int u = 0; u < 2; ++u) {
-    uint32_t hi[4], lo[4];                   // [q = 2u: pairs 0, 1][q = 2u + 1: pairs 0, 1]
-#pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      uint16_t p0, q0, p1, q1;
-      mu_split(v[8 * u + 2 * j], &p0, &q0);
-      mu_split(v[8 * u + 2 * j + 1], &p1, &q1);
-      hi[j] = p0 | ((uint32_t)p1 << 16);
-      lo[j] = q0 | ((uint32_t)q1 << 16);
-    }
-    // rows 8 q + 4 (lane >> 5) + 0..3: the lane halves trade so that a lane has eight successive ones
-    auto a = __builtin_amdgcn_permlane32_swap(hi[0], hi[2], false, false);
-    auto b = __builtin_amdgcn_permlane32_swap(hi[1], hi[3], false, false);
-    auto c = __builtin_amdgcn_permlane32_swap(lo[0], lo[2], false, false);
-    auto d = __builtin_amdgcn_permlane32_swap(lo[1], lo[3], false, false);
-    *reinterpret_cast<raw16*>(out + u * 2048 + lane * 16) = raw16{a[0], b[0], a[1], b[1]};
-    *reinterpret_cast<raw16*>(out + u * 2048 + 1024 + lane * 16) = raw16{c[0], d[0], c[1], d[1]};
+  for (int j = 0; j < 8; ++j) {
+    const f32x2 x = {v[2 * j], v[2 * j + 1]};
+    const f16x2 h = __builtin_convertvector(x, f16x2);
+    const f16x2 l = __builtin_convertvector(x - __builtin_convertvector(h, f32x2), f16x2);
+    hi[j] = __builtin_bit_cast(uint32_t, h);
+    lo[j] = __builtin_bit_cast(uint32_t, l);
   }
-}
-// ... the other way round (rows = its rows, k = its columns): through `t`, 32 x 33 floats of this wave's LDS.
-__device__ __forceinline__ void mu_store_rows(const float* v, char* out, int lane, float* t) {
   const int l31 = lane & 31, h = lane >> 5;
+  if (rows) {
 #pragma unroll
-  for (int i = 0; i < 16; ++i) t[((i & 3) + 8 * (i >> 2) + 4 * h) * 33 + l31] = v[i];
-  __builtin_amdgcn_wave_barrier();
+    for (int j = 0; j < 8; ++j) {
+      const int r = (2 * j & 3) + 8 * (j >> 1) + 4 * h;
+      turn[r * MU_PITCH + l31] = __builtin_amdgcn_perm(lo[j], hi[j], 0x05040100);
+      turn[(r + 1) * MU_PITCH + l31] = __builtin_amdgcn_perm(lo[j], hi[j], 0x07060302);
+    }
+  }
 #pragma unroll
   for (int u = 0; u < 2; ++u) {
-    uint32_t hi[4], lo[4];
-#pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      uint16_t p0, q0, p1, q1;
-      mu_split(t[l31 * 33 + u * 16 + h * 8 + 2 * j], &p0, &q0);
-      mu_split(t[l31 * 33 + u * 16 + h * 8 + 2 * j + 1], &p1, &q1);
-      hi[j] = p0 | ((uint32_t)p1 << 16);
-      lo[j] = q0 | ((uint32_t)q1 << 16);
-    }
-    *reinterpret_cast<raw16*>(out + u * 2048 + lane * 16) = raw16{hi[0], hi[1], hi[2], hi[3]};
-    *reinterpret_cast<raw16*>(out + u * 2048 + 1024 + lane * 16) = raw16{lo[0], lo[1], lo[2], lo[3]};
+    auto a = __builtin_amdgcn_permlane32_swap(hi[4 * u], hi[4 * u + 2], false, false);
+    auto b = __builtin_amdgcn_permlane32_swap(hi[4 * u + 1], hi[4 * u + 3], false, false);
+    auto c = __builtin_amdgcn_permlane32_swap(lo[4 * u], lo[4 * u + 2], false, false);
+    auto d = __builtin_amdgcn_permlane32_swap(lo[4 * u + 1], lo[4 * u + 3], false, false);
+    *reinterpret_cast<raw16*>(cols + u * 2048 + lane * 16) = raw16{a[0], b[0], a[1], b[1]};
+    *reinterpret_cast<raw16*>(cols + u * 2048 + 1024 + lane * 16) = raw16{c[0], d[0], c[1], d[1]};
   }
-  __builtin_amdgcn_wave_barrier();
+  if (rows) {
+    __builtin_amdgcn_wave_barrier();         // (one wave's LDS accesses are in order)
+#pragma unroll
+    for (int u = 0; u < 2; ++u) {
+      const raw16* p = reinterpret_cast<const raw16*>(turn + l31 * MU_PITCH + u * 16 + h * 8);
+      const raw16 x = p[0], y = p[1];
+      *reinterpret_cast<raw16*>(rows + u * 2048 + lane * 16) =
+          raw16{__builtin_amdgcn_perm(x[1], x[0], 0x05040100), __builtin_amdgcn_perm(x[3], x[2], 0x05040100),
+                __builtin_amdgcn_perm(y[1], y[0], 0x05040100), __builtin_amdgcn_perm(y[3], y[2], 0x05040100)};
+      *reinterpret_cast<raw16*>(rows + u * 2048 + 1024 + lane * 16) =
+          raw16{__builtin_amdgcn_perm(x[1], x[0], 0x07060302), __builtin_amdgcn_perm(x[3], x[2], 0x07060302),
+                __builtin_amdgcn_perm(y[1], y[0], 0x07060302), __builtin_amdgcn_perm(y[3], y[2], 0x07060302)};
+    }
+    __builtin_amdgcn_wave_barrier();
+  }
 }
 
 // Tile t (row by row) of the upper triangle of tm x tm tiles.
@@ -269,7 +275,7 @@ __device__ __forceinline__ void mu_triangle(int t, int tm, int* ti, int* tj) {
 // The accumulator of 32-blocks (rb, cb) of a symmetric result, scaled into its one or two buffers, and mirrored unless the
 // whole tile lies on the diagonal.
 __device__ __forceinline__ void mu_store_symmetric(const mu_task& g, char* ws, int job, const float* acc, int rb, int cb, bool mirror,
-                                                   int lane, float* turn) {
+                                                   int lane, uint32_t* turn) {
   const int l31 = lane & 31, h = lane >> 5, units = g.pm / 16;
 #pragma unroll
   for (int k = 0; k < 2; ++k) {
@@ -280,8 +286,7 @@ __device__ __forceinline__ void mu_store_symmetric(const mu_task& g, char* ws, i
 #pragma unroll
     for (int i = 0; i < 16; ++i) v[i] = acc[i] * s + (rb == cb && (i & 3) + 8 * (i >> 2) + 4 * h == l31 ? on : 0.f);
     char* out = mu_at(ws, g, job, d);
-    mu_store_cols(v, out + ((int64_t)cb * units + rb * 2) * 2048, lane);
-    if (mirror) mu_store_rows(v, out + ((int64_t)rb * units + cb * 2) * 2048, lane, turn);
+    mu_store(v, out + ((int64_t)cb * units + rb * 2) * 2048, mirror ? out + ((int64_t)rb * units + cb * 2) * 2048 : nullptr, lane, turn);
   }
 }
 
@@ -304,17 +309,22 @@ __device__ __forceinline__ void mu_gemm_tile(const mu_table& tab, const mu_jobs*
   const mu_task& g = tab.t[gi];
   int u = blk - tab.blk0[gi], split = 0, ti, tj, job;
   const int tm = g.pm / BT, tn = g.pn / BT, per = MODE == MU_SYM ? tm * (tm + 1) / 2 : tm * tn;
+  int t;
   if (MODE == MU_SYM && g.whole == 0) {      // all tiles split: a matrix's tiles of one part of k are neighbours
-    const int in = u % (per * g.splits);
-    job = u / (per * g.splits);
-    split = in / per;
-    u = job * per + in % per;
-  } else if (MODE == MU_SYM && u >= g.whole) {
-    split = (u - g.whole) % g.splits;
-    u = g.whole + (u - g.whole) / g.splits;
+    const unsigned both = (unsigned)per * g.splits, in = (unsigned)u % both;
+    job = (unsigned)u / both;
+    split = in / (unsigned)per;
+    t = in - split * per;
+    u = job * per + t;
+  } else {
+    if (MODE == MU_SYM && u >= g.whole) {
+      const unsigned rest = u - g.whole;
+      u = g.whole + rest / (unsigned)g.splits;
+      split = rest % (unsigned)g.splits;
+    }
+    job = (unsigned)u / (unsigned)per;
+    t = u - job * per;
   }
-  job = u / per;
-  const int t = u - job * per;
   const bool turned = MODE == MU_LAST && !g.tall;
   if (MODE == MU_SYM) {
     mu_triangle(t, tm, &ti, &tj);
@@ -331,9 +341,9 @@ __device__ __forceinline__ void mu_gemm_tile(const mu_table& tab, const mu_jobs*
   int k0 = 0, stages = kunits / KU;
   const bool part = MODE == MU_SYM && u >= g.whole;
   if (part) {                                // splits share the stages evenly
-    const int all = stages;
-    k0 = (int)((int64_t)all * split / g.splits);
-    stages = (int)((int64_t)all * (split + 1) / g.splits) - k0;
+    const unsigned all = stages, parts = g.splits;       // (at most 2^13 stages in 64 parts)
+    k0 = (int)(all * split / parts);
+    stages = (int)(all * (split + 1) / parts) - k0;
   }
   f32x16 acc[TW][TW];
 #pragma unroll
@@ -444,7 +454,7 @@ __device__ __forceinline__ void mu_gemm_tile(const mu_table& tab, const mu_jobs*
     return;
   }
   __syncthreads();                           // the stages' LDS is free
-  float* turn = (float*)smem + wave * 32 * 33;
+  uint32_t* turn = (uint32_t*)smem + wave * 32 * MU_PITCH;
 #pragma unroll
   for (int a = 0; a < TW; ++a)
 #pragma unroll
@@ -454,8 +464,8 @@ __device__ __forceinline__ void mu_gemm_tile(const mu_table& tab, const mu_jobs*
       if constexpr (MODE == MU_APPLY) {      // rows of the result: n, columns: m
 #pragma unroll
         for (int i = 0; i < 16; ++i) v[i] = acc[a][b][i] * g.s0;
-        mu_store_cols(v, mu_at(ws, g, job, g.d0) + ((int64_t)cb * (g.pn / 16) + rb * 2) * 2048, lane);
-        mu_store_rows(v, mu_at(ws, g, job, g.d1) + ((int64_t)rb * (g.pm / 16) + cb * 2) * 2048, lane, turn);
+        mu_store(v, mu_at(ws, g, job, g.d0) + ((int64_t)cb * (g.pn / 16) + rb * 2) * 2048,
+                 mu_at(ws, g, job, g.d1) + ((int64_t)rb * (g.pm / 16) + cb * 2) * 2048, lane, turn);
       } else {
 #pragma unroll
         for (int i = 0; i < 16; ++i) v[i] = acc[a][b][i];
@@ -480,7 +490,7 @@ template <int TW>
 __global__ void __launch_bounds__(64)
 k_mu_join(mu_table tab, char* ws) {
   constexpr int BT = 64 * TW, SUB = 4 * TW * TW;
-  __shared__ float turn[32 * 33];
+  __shared__ __attribute__((aligned(16))) uint32_t turn[32 * MU_PITCH];
   const int lane = threadIdx.x, tile = blockIdx.x / SUB, sub = blockIdx.x % SUB;
   const int gi = mu_find(tab, tile);
   const mu_task& g = tab.t[gi];
@@ -514,7 +524,7 @@ static int64_t mu_up(int64_t v, int64_t a) { return (v + a - 1) / a * a; }
 
 struct mu_group {
   int m, n, pm, pn, count, first, tall;
-  bool longish;                        // n >= 2 m: steps in A alone, X every second or third
+  bool longish;                        // steps in A alone, X every second or third
   int64_t off, stride;                 // units of 256 bytes
   int x, xt[2], a, c, p, z, q[2], norm, norm_blocks;
 };
@@ -554,6 +564,11 @@ static void mu_make_plan(const lmh_muon_job* jobs, int count, mu_plan* pl) {
   pl->tw = 1;
   for (int i = 0; i < count; ++i)
     if (std::min(jobs[i].rows, jobs[i].cols) > 64) pl->tw = 2;
+  // one long matrix, and the others but for large ones go its way: the number of multiplications is the same for m = n, and two
+  // kinds would take their launches one after the other
+  bool all_long = false;
+  for (int i = 0; i < count; ++i)
+    if (std::max(jobs[i].rows, jobs[i].cols) >= 2 * std::min(jobs[i].rows, jobs[i].cols)) all_long = true;
   const int bt = 64 * pl->tw;
   int64_t off = 0;
   pl->groups.clear();
@@ -569,7 +584,7 @@ static void mu_make_plan(const lmh_muon_job* jobs, int count, mu_plan* pl) {
     g.pn = (int)mu_up(g.n, bt);
     g.count = e - s;
     g.first = s;
-    g.longish = g.pn >= 2 * g.pm;
+    g.longish = all_long && g.pm <= 2048 ? true : g.n >= 2 * g.m;
     const int mn = (int)((int64_t)g.pm * g.pn / 64), mm = (int)((int64_t)g.pm * g.pm / 64);      // 4 bytes a value, units of 256
     int at = 0;
     auto take = [&](int n) { const int r = at; at += n; return r; };
@@ -722,15 +737,15 @@ class mu_runner {
   }
   // X <- polynomial X
   template <typename F>
-  void apply(const std::vector<const mu_group*>& gs, F operands) {
-    const int bt = 64 * pl_.tw;
+  void apply(const std::vector<const mu_group*>& gs, int tw, F operands) {
+    const int bt = 64 * tw;
     for (size_t lo = 0; lo < gs.size(); lo += MU_MAX_GROUPS) {
       const int nb = tasks(gs, lo, std::min(gs.size(), lo + MU_MAX_GROUPS), [&](const mu_group& g, mu_task* t) {
         operands(g, t);
         t->aux = g.pm / 16;
         return (g.pm / bt) * (g.pn / bt) * g.count;
       });
-      if (pl_.tw == 1) lmh_launch((k_mu_gemm<1, 2, 4, MU_APPLY>), dim3(nb), dim3(256), 0, st_, tab_, ws_);
+      if (tw == 1) lmh_launch((k_mu_gemm<1, 2, 4, MU_APPLY>), dim3(nb), dim3(256), 0, st_, tab_, ws_);
       else lmh_launch((k_mu_gemm<2, 2, 2, MU_APPLY>), dim3(nb), dim3(256), 0, st_, tab_, ws_);
     }
   }
@@ -804,14 +819,20 @@ static void mu_run(const lmh_muon_job* jobs, const mu_plan& pl, int steps, float
     const std::vector<const mu_group*>& G = gs[kind];
     if (G.empty()) continue;
     // m x m products: 64 x 64 tiles while those of 128 x 128 would leave places free
-    int64_t tiles = 0;
-    for (const mu_group* g : G) tiles += (int64_t)g->count * (g->pm / 128) * (g->pm / 128 + 1) / 2;
-    const int tw = pl.tw == 2 && tiles >= MU_SLOTS / 2 ? 2 : 1;
+    int64_t tiles = 0, xtiles = 0, xstages = 0;
+    for (const mu_group* g : G) {
+      const int64_t t = (int64_t)g->count * (g->pm / 128) * (g->pm / 128 + 1) / 2;
+      tiles += t;
+      xtiles += (int64_t)g->count * (g->pm / 128) * (g->pn / 128);
+      xstages += t * (g->pn / 32);
+    }
+    const int tw = pl.tw == 2 && tiles >= 256 ? 2 : 1;
+    const int tw_apply = pl.tw == 2 && xtiles >= 128 ? 2 : 1, tw_gram = pl.tw == 2 && xstages >= 4096 ? 2 : 1;
     int flip = 0;
     for (int done = 0; done < steps;) {
       const int left = steps - done, len = kind == 0 ? 1 : left == 4 ? 2 : std::min(left, 3);
       // A = X X' and b I + c A
-      run.symmetric(G, pl.tw, [](const mu_group& g, mu_runner::product* p) {
+      run.symmetric(G, tw_gram, [](const mu_group& g, mu_runner::product* p) {
         const float s = 1.f / (MU_SX * MU_SX);
         p[0] = {g.x, g.x, g.a, g.c, g.pn / 16, MU_SG * s, 0.f, MU_C * MU_SC * s, MU_B * MU_SC};
         return 1;
@@ -850,16 +871,16 @@ static void mu_run(const lmh_muon_job* jobs, const mu_plan& pl, int steps, float
         t->s0 = len > 1 ? 1.f / MU_SQ : 1.f / MU_SP;
       };
       if (done < steps) {
-        run.apply(G, operands);
+        run.apply(G, tw_apply, operands);
         flip = 1 - flip;
       } else {
         run.with_jobs(jobs, G, [&](const mu_group& g, mu_task* t) {
           operands(g, t);
           t->s0 /= MU_SX;
           t->aux = g.pm / 16;
-          return (g.pm / (64 * pl.tw)) * (g.pn / (64 * pl.tw));
+          return (g.pm / (64 * tw_apply)) * (g.pn / (64 * tw_apply));
         }, [&](dim3 nb, const mu_table& tab, const mu_jobs& pj) {
-          if (pl.tw == 1) lmh_launch((k_mu_last<T, 1, 2, 4, OPT>), nb, dim3(256), 0, st, tab, pj, ws, lr);
+          if (tw_apply == 1) lmh_launch((k_mu_last<T, 1, 2, 4, OPT>), nb, dim3(256), 0, st, tab, pj, ws, lr);
           else lmh_launch((k_mu_last<T, 2, 2, 2, OPT>), nb, dim3(256), 0, st, tab, pj, ws, lr);
         });
       }
