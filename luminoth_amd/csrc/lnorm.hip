@@ -22,13 +22,10 @@ k_ln_fwd(const T* __restrict__ x, int64_t ldx, const P* __restrict__ gamma, cons
   const int lane = threadIdx.x & (TPR - 1), grp = threadIdx.x / TPR;
   float ga[NC * VEC], be[NC * VEC];
 #pragma unroll
-  for (int c = 0; c < NC; ++c)
-#pragma unroll
-    for (int e = 0; e < VEC; ++e) {
-      const int col = (c * TPR + lane) * VEC + e;
-      ga[c * VEC + e] = gamma && col < D ? to_f32(gamma[col]) : 1.f;
-      be[c * VEC + e] = beta && col < D ? to_f32(beta[col]) : 0.f;
-    }
+  for (int c = 0; c < NC; ++c) {
+    load_params<VEC>(ga + c * VEC, gamma, (c * TPR + lane) * VEC, D, 1.f);
+    load_params<VEC>(be + c * VEC, beta, (c * TPR + lane) * VEC, D, 0.f);
+  }
   const int64_t step = (int64_t)gridDim.x * GPB;
   int64_t base = (int64_t)blockIdx.x * GPB;
   raw16 cur[NC], nxt[NC];
@@ -108,11 +105,11 @@ k_ln_fwd_long(const T* __restrict__ x, int64_t ldx, const P* __restrict__ gamma,
     for (int64_t col = (int64_t)threadIdx.x * VEC; col < D; col += 1024 * VEC) {
       const raw16 r = load_cols(xr, (int)col, D);
       float o[VEC];
+      float ga[VEC], be[VEC];
+      load_params<VEC>(ga, gamma, (int)col, D, 1.f);
+      load_params<VEC>(be, beta, (int)col, D, 0.f);
 #pragma unroll
-      for (int e = 0; e < VEC; ++e) {
-        const bool in = col + e < D;
-        o[e] = fmaf((elem<T>(r, e) - mu) * rs, gamma && in ? to_f32(gamma[col + e]) : 1.f, beta && in ? to_f32(beta[col + e]) : 0.f);
-      }
+      for (int e = 0; e < VEC; ++e) o[e] = fmaf((elem<T>(r, e) - mu) * rs, ga[e], be[e]);
       store_cols(y + row * (int64_t)D, (int)col, D, o);
     }
     if (threadIdx.x == 0) {
@@ -134,13 +131,11 @@ k_ln_bwd(const T* __restrict__ dy, int64_t lddy, const T* __restrict__ x, int64_
   const int lane = threadIdx.x & (TPR - 1), grp = threadIdx.x / TPR;
   float ga[E], dg[E], db[E];
 #pragma unroll
-  for (int c = 0; c < NC; ++c)
+  for (int c = 0; c < NC; ++c) {
+    load_params<VEC>(ga + c * VEC, gamma, (c * TPR + lane) * VEC, D, 1.f);
 #pragma unroll
-    for (int e = 0; e < VEC; ++e) {
-      const int col = (c * TPR + lane) * VEC + e;
-      ga[c * VEC + e] = gamma && col < D ? to_f32(gamma[col]) : 1.f;
-      dg[c * VEC + e] = db[c * VEC + e] = 0.f;
-    }
+    for (int e = 0; e < VEC; ++e) dg[c * VEC + e] = db[c * VEC + e] = 0.f;
+  }
   const int64_t step = (int64_t)gridDim.x * GPB;
   int64_t base = (int64_t)blockIdx.x * GPB;
   raw16 cx[NC], cd[NC], ca[NC], nx[NC], nd[NC], na[NC];
@@ -271,9 +266,11 @@ k_ln_bwd_long(const T* __restrict__ dy, int64_t lddy, const T* __restrict__ x, i
     float a = 0.f, b = 0.f;
     for (int64_t col = (int64_t)threadIdx.x * VEC; col < D; col += 1024 * VEC) {
       const raw16 rx = load_cols(x + row * ldx, (int)col, D), rd = load_cols(dy + row * lddy, (int)col, D);
+      float ga[VEC];
+      load_params<VEC>(ga, gamma, (int)col, D, 1.f);
 #pragma unroll
       for (int e = 0; e < VEC; ++e) {
-        const float t = elem<T>(rd, e) * (gamma && col + e < D ? to_f32(gamma[col + e]) : 1.f);
+        const float t = elem<T>(rd, e) * ga[e];
         a += t;
         b = fmaf(t, (elem<T>(rx, e) - mu) * rs, b);
       }
@@ -284,10 +281,11 @@ k_ln_bwd_long(const T* __restrict__ dy, int64_t lddy, const T* __restrict__ x, i
       const raw16 rx = load_cols(x + row * ldx, (int)col, D), rd = load_cols(dy + row * lddy, (int)col, D);
       raw16 ra = {0, 0, 0, 0};
       if (addend) ra = load_cols(addend + row * ldadd, (int)col, D);
-      float o[VEC];
+      float ga[VEC], o[VEC];
+      load_params<VEC>(ga, gamma, (int)col, D, 1.f);
 #pragma unroll
       for (int e = 0; e < VEC; ++e) {
-        const float t = elem<T>(rd, e) * (gamma && col + e < D ? to_f32(gamma[col + e]) : 1.f);
+        const float t = elem<T>(rd, e) * ga[e];
         o[e] = rs * (t - a - (elem<T>(rx, e) - mu) * rs * b) + elem<T>(ra, e);
       }
       store_cols(dx + row * (int64_t)D, (int)col, D, o);
@@ -350,11 +348,13 @@ k_ln_params(const float* __restrict__ part, int nb, int D, int W, int tpr, int v
 }
 
 // ------------------------------------------------------------------------------------------------------- host ----
+#define LN_FWD_BLOCKS 1536        // six of 256 threads a compute unit: what its registers hold (1024: 1-14 % slower, 2048: 6-26 %)
 struct ln_shape { int tpr, nc; };
-// 16 columns a thread at most: 16, 64, 256 or 1024 threads a row
-static ln_shape ln_pick(int D, int vec) {
+// 16 columns a thread at most: 16, 64, 256 or 1024 threads a row; the forward pass of 16-bit rows of 4097 to 8192 columns has 512
+// (three blocks a compute unit instead of one: 6000 x 8192 bf16 50 -> 35 us; fp32 60 -> 64, the backward pass 75 -> 78)
+static ln_shape ln_pick(int D, int vec, bool fwd = false) {
   ln_shape s;
-  s.tpr = D <= 256 ? 16 : D <= 1024 ? 64 : D <= 4096 ? 256 : 1024;
+  s.tpr = D <= 256 ? 16 : D <= 1024 ? 64 : D <= 4096 ? 256 : fwd && vec == 8 && D <= 8192 ? 512 : 1024;
   const int per = (D + s.tpr * vec - 1) / (s.tpr * vec);
   s.nc = vec == 8 ? (per <= 1 ? 1 : 2) : (per <= 1 ? 1 : per <= 2 ? 2 : 4);
   return s;
@@ -366,8 +366,9 @@ static int ln_bwd_blocks(int64_t rows, int D, int vec) {
   if (D > LN_MAX_REG_COLS) return (int)(rows < LN_LONG_SLICES ? rows : LN_LONG_SLICES);
   const ln_shape s = ln_pick(D, vec);
   const int bt = ln_bwd_threads(s.tpr), gpb = bt / s.tpr;
-  // a group walks over four rows at least: what a block leaves (its sums, a partial row) costs as much as some rows
-  const int64_t need = (rows + 4 * gpb - 1) / (4 * gpb), cap = s.tpr == 1024 ? 256 : 512;
+  // what the registers hold at a time: 256 blocks with 16 columns a thread (a second one would wait: 5003 x 1001 f16 15.5 us, 18.5 with
+  // 512), 512 with 8 (60000 x 500 f16 69 us, 103 with 256), 768 with 4
+  const int64_t need = (rows + gpb - 1) / gpb, cap = s.tpr == 1024 || s.nc * vec == 16 ? 256 : s.nc * vec == 8 ? 512 : 768;
   return (int)(need < cap ? need : cap);
 }
 static int ln_part_cols(int D, int vec) {         // columns of a partial row
@@ -403,13 +404,20 @@ static void ln_fwd_launch(const void* x, int64_t ldx, const void* gamma, const v
                (const P*)beta, (T*)y, mean, rstd, rows, D, inv_d, eps);
     return;
   }
-  const ln_shape s = ln_pick(D, row_type<T>::VEC);
+  const ln_shape s = ln_pick(D, row_type<T>::VEC, true);
   const int bt = s.tpr > 256 ? s.tpr : 256, gpb = bt / s.tpr;
-  const int64_t need = (rows + gpb - 1) / gpb, cap = bt == 1024 ? 512 : 2048;
+  const int64_t need = (rows + gpb - 1) / gpb, cap = LN_FWD_BLOCKS * 256 / (bt == 1024 ? 1536 : bt);
   const dim3 grid((unsigned)(need < cap ? need : cap));
 #define LN_FWD(T_, P_, TPR_, NC_)                                                                                          \
   lmh_launch((k_ln_fwd<T_, P_, TPR_, NC_>), grid, dim3(bt), 0, st, (const T_*)x, ldx, (const P_*)gamma, (const P_*)beta, (T_*)y, mean, \
              rstd, rows, D, inv_d, eps)
+  if constexpr (row_type<T>::VEC == 8) {
+    if (s.tpr == 512) {
+      if (s.nc == 1) LN_FWD(T, P, 512, 1);
+      else LN_FWD(T, P, 512, 2);
+      return;
+    }
+  }
   LN_PICK(LN_FWD, T, P);
 #undef LN_FWD
 }

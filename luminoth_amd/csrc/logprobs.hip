@@ -6,17 +6,19 @@
 //   the k largest x_j, equal ones in the order of their index, as (j, (x_j - m) - log S)
 //   dx_j = sum over the given ones of g (d_j,idx - p_j)  -  g_H p_j (log p_j + H),   p_j = exp(x_j - lse)
 //
-// Forward: a block (256 threads) holds a SEGMENT of a row in registers as it lies in memory (16-byte vectors, at most 8 a
-// thread: 16384 classes in 16 bits), so the logits are read once for all of it.  A short row is one wave's.  The maximum
-// of the segment is known before the first exponential, so there is ONE exponential a class.  Alternatives: the k-th
-// largest of a wave's 64 lane maxima is a lower bound of the k-th largest value (bit by bit with ballots: 32 compares);
-// the vectors that reach the best wave's bound go into a list of LDS, of those the values that do - some dozens - into a
-// second one, and an entry's place is the number of larger ones.  Value and index make one 64-bit key (larger value first, then lower index): all keys differ, so
-// the order in which lanes append does not matter.  Segments of one row are joined by a second launch.
+// Forward: a block (256 threads) takes one row, or a part of it, SEGMENT by segment: 16-byte vectors as they lie in memory, at most
+// 4 a thread (8192 classes in 16 bits), read once for all of it.  A short row is one wave's.  Every thread keeps a maximum and
+// sums of its own over its segments (rescaled when the maximum grows: one more exponential for 32) and they are joined at the
+// end: no barrier inside the loop.
+// Alternatives: the k-th largest of a wave's 64 lane maxima so far is a lower bound of the k-th largest value (bit by bit with
+// ballots: 16 compares); vectors that reach the bound go into a list of LDS whole - some dozens, fewer and fewer from segment to
+// segment -, of those the values that reach the last bound into a second one, and an entry's place there is the number of
+// larger ones.  Value and index make one 64-bit key (larger value first, then lower index): all keys differ, so the order in
+// which lanes append does not matter.  Parts of one row are joined by a second launch.
 #include "rowops.h"
 
 #define LP_MAX_TOP LMH_LOG_PROBS_MAX_TOP
-#define LP_SEG_VECS 8
+#define LP_SEG_VECS 4             // 64 registers: eight blocks a compute unit (8: 88 registers, 2-4 % slower)
 #define LP_JOIN_LDS 4096
 
 typedef unsigned long long u64;
@@ -88,129 +90,151 @@ __device__ __forceinline__ bool lp_target(const T* x, const I* targets, int64_t 
   return true;
 }
 
-template <typename T> __device__ __forceinline__ raw16 load_classes(const T* row, int col, int end) {
-  constexpr int VEC = row_type<T>::VEC;
-  if (col + VEC <= end) return load16(row + col);
-  const uint32_t none = __is_same(T, f32_t) ? 0xff800000u : __is_same(T, f16_t) ? 0xfc00fc00u : 0xff80ff80u;
-  raw16 r = {none, none, none, none};
-  if (col < end) {
-#pragma unroll
-    for (int e = 0; e < VEC; ++e)
-      if (col + e < end) {
-        if constexpr (VEC == 4) {
-          r[e] = __float_as_uint(row[col + e].v);
-        } else {
-          const uint32_t b = __builtin_bit_cast(uint16_t, row[col + e]), sh = 16 * (e & 1);
-          r[e >> 1] = (r[e >> 1] & ~(0xffffu << sh)) | (b << sh);
-        }
-      }
-  }
-  return r;
+template <typename T> __device__ __forceinline__ raw16 load_classes(const T* row, int col, int end) {       // -inf behind the end
+  return load_cols(row, col, end, __is_same(T, f32_t) ? 0xff800000u : __is_same(T, f16_t) ? 0xfc00fc00u : 0xff80ff80u);
 }
 
-// TPR threads a row or segment (64: one wave, no block-wide step; 256: the block), NV vectors a thread.
-// Partial results of a segment: stats[(row * segs + seg) * 3] and, sorted, best[(row * segs + seg) * k].
+// TPR threads a row or a part of one (64: one wave, no block-wide step; 256: the block), NV vectors a thread and segment, `run`
+// segments a part.  Results of a part: stats[(row * parts + part) * 3] and, sorted, best[(row * parts + part) * k].
 template <typename T, typename I, int TPR, int NV>
 __global__ void __launch_bounds__(256)
-k_log_probs(const T* __restrict__ x, int64_t ldx, const I* __restrict__ targets, int64_t rows, int V, int k, int segs, lp_out out,
+k_log_probs(const T* __restrict__ x, int64_t ldx, const I* __restrict__ targets, int64_t rows, int V, int k, int run, int parts, lp_out out,
             float* __restrict__ stats, u64* __restrict__ best) {
-  constexpr int VEC = row_type<T>::VEC, SEG = TPR * NV * VEC, GPB = 256 / TPR, WPG = TPR / 64;
-  constexpr int LIST = TPR == 64 ? 128 : 512, VLIST = TPR == 64 ? 64 : 256;
+  constexpr int VEC = row_type<T>::VEC, SEG = TPR * NV * VEC, GPB = 256 / TPR;
+  constexpr int LIST = TPR == 64 ? 128 : 512, VLIST = TPR == 64 ? 128 : 512;
+  constexpr uint32_t NONE = 0x007fffffu;                        // the key of -inf
   __shared__ float red[3][4];
-  __shared__ uint32_t red_key[4];
+  __shared__ uint32_t bounds[4];
   __shared__ u64 list[GPB][LIST];
   __shared__ u64 winner[4];
   __shared__ raw16 vlist[GPB][VLIST];
   __shared__ int vcol[GPB][VLIST], vcount[GPB], count[GPB];
-  const int lane = threadIdx.x & (TPR - 1), grp = threadIdx.x / TPR;
-  const int64_t unit = (int64_t)blockIdx.x * GPB + grp;         // (row, segment)
-  const int64_t row = unit / segs;
-  const int seg = (int)(unit % segs);
+  const int lane = threadIdx.x & (TPR - 1), grp = threadIdx.x / TPR, wave = threadIdx.x >> 6;
+  const int64_t unit = (int64_t)blockIdx.x * GPB + grp;         // (row, part)
+  const int64_t row = parts == 1 ? unit : unit / parts;
+  const int first = parts == 1 ? 0 : (int)(unit % parts) * run * SEG;
   const bool live = row < rows;                                 // (whole waves: TPR >= 64)
-  const int first = seg * SEG;
   const T* xr = x + (live ? row : 0) * ldx;
-  const int end = live ? V : 0;
-  // (behind the end: -inf, which no maximum and no sum sees)
-  raw16 r[NV];
-#pragma unroll
-  for (int v = 0; v < NV; ++v) r[v] = load_classes(xr, first + (v * TPR + lane) * VEC, end);
+  const int64_t stop = (int64_t)first + (int64_t)run * SEG;
+  const int end = !live ? 0 : stop < V ? (int)stop : V;         // of this part
   if (lane == 0) count[grp] = vcount[grp] = 0;
+  if ((threadIdx.x & 63) == 0) bounds[wave] = 0;
+  __syncthreads();
 
-  // ---- maximum, of every vector and of all (fmaxf passes over not-a-number: those rows show in S)
-  float vmax[NV], mine = -INFINITY;
+  float m = -INFINITY, S = 0.f, W = 0.f;                        // this thread's
+  uint32_t top = 0, own = 0;                                    // this lane's largest key, this wave's bound
+  for (int base = first; base < end; base += SEG) {
+    // (behind the end: -inf, which no maximum and no sum sees)
+    raw16 r[NV];
 #pragma unroll
-  for (int v = 0; v < NV; ++v) {
-    vmax[v] = elem<T>(r[v], 0);
+    for (int v = 0; v < NV; ++v) r[v] = load_classes(xr, base + (v * TPR + lane) * VEC, end);
+    // maximum, of every vector and of all (fmaxf passes over not-a-number: those rows show in S)
+    float vmax[NV], mine = -INFINITY;
 #pragma unroll
-    for (int e = 1; e < VEC; ++e) vmax[v] = fmaxf(vmax[v], elem<T>(r[v], e));
-    mine = fmaxf(mine, vmax[v]);
+    for (int v = 0; v < NV; ++v) {
+      vmax[v] = elem<T>(r[v], 0);
+#pragma unroll
+      for (int e = 1; e < VEC; ++e) vmax[v] = fmaxf(vmax[v], elem<T>(r[v], e));
+      mine = fmaxf(mine, vmax[v]);
+    }
+    // (what was unpacked for the maxima is unpacked again below: kept, it would take a register a class)
+#pragma unroll
+    for (int v = 0; v < NV; ++v) asm volatile("" : "+v"(r[v]));
+    if (mine > m) {                                             // sums of (x - m): exp(d) of them, and d more in each
+      const float d = m - mine, f = S > 0.f ? __expf(d) : S;    // (S = 0: nothing there; not-a-number stays)
+      W = S > 0.f ? f * fmaf(fmaxf(d, -200.f), S, W) : W;
+      S *= f;
+      m = mine;
+    }
+    const float m0 = m == -INFINITY ? 0.f : m;
+    // entries of the list: what k values of this wave's earlier segments reach is not needed (those come first), nor what is
+    // below k values of this segment and those, or of another wave
+    uint32_t low = 0xffffffffu;
+    if (k > 0) {
+      const uint32_t key = lp_key(mine);
+      top = key > top ? key : top;
+      if (__any(key > own && key > NONE)) {
+        const uint32_t now = lp_kth_of_wave(top, k);
+        low = own + 1 > NONE + 1 ? own + 1 : NONE + 1;
+        low = now > low ? now : low;
+        own = now;
+        if constexpr (TPR > 64) {                               // (others' bounds may be old: old ones hold too)
+          volatile uint32_t* b = bounds;
+          if ((threadIdx.x & 63) == 0) b[wave] = now;
+#pragma unroll
+          for (int w = 0; w < 4; ++w) {
+            const uint32_t o = b[w];
+            low = o > low ? o : low;
+          }
+        }
+      }
+    }
+    // (keys and values are in the same order: one compare of values a vector)
+    const float low_value = low == 0xffffffffu ? INFINITY : lp_unkey(low);
+#pragma unroll
+    for (int v = 0; v < NV; ++v) {
+#pragma unroll
+      for (int e = 0; e < VEC; ++e) {
+        const float z = elem<T>(r[v], e) - m0, p = __expf(z);
+        S += p;
+        W = fmaf(fmaxf(z, -200.f), p, W);          // (p = 0 below -104: -inf must not meet it)
+      }
+      if (vmax[v] >= low_value && low != 0xffffffffu) {
+        const int at = atomicAdd(&vcount[grp], 1);
+        if (at < VLIST) {
+          vlist[grp][at] = r[v];
+          vcol[grp][at] = base + (v * TPR + lane) * VEC;
+        }
+      }
+    }
   }
-  float m = reduce64(mine, op_max());
-  uint32_t bound = 0;
-  if (k > 0) bound = lp_kth_of_wave(lp_key(mine), k);
+
+  // ---- the threads' sums joined
+  float M = reduce64(m, op_max());
   if constexpr (TPR > 64) {
     if ((threadIdx.x & 63) == 0) {
-      red[0][threadIdx.x >> 6] = m;
-      red_key[threadIdx.x >> 6] = bound;
+      red[0][wave] = M;
+      bounds[wave] = own;
     }
     __syncthreads();
 #pragma unroll
-    for (int w = 0; w < 4; ++w) {
-      m = fmaxf(m, red[0][w]);
-      bound = red_key[w] > bound ? red_key[w] : bound;
-    }
+    for (int w = 0; w < 4; ++w) M = fmaxf(M, red[0][w]);
   }
-  const float m0 = m == -INFINITY ? 0.f : m;
-
-  // ---- sums, and the entries of the list
-  float S = 0.f, W = 0.f;
-#pragma unroll
-  for (int v = 0; v < NV; ++v) {
-#pragma unroll
-    for (int e = 0; e < VEC; ++e) {
-      const float z = elem<T>(r[v], e) - m0, p = __expf(z);
-      S += p;
-      W = fmaf(fmaxf(z, -200.f), p, W);          // (p = 0 below -104: -inf must not meet it)
-    }
-    if (k > 0 && lp_key(vmax[v]) >= bound) {       // the vector goes to the list whole
-      const int at = atomicAdd(&vcount[grp], 1);
-      if (at < VLIST) {
-        vlist[grp][at] = r[v];
-        vcol[grp][at] = first + (v * TPR + lane) * VEC;
-      }
-    }
+  const float m0 = M == -INFINITY ? 0.f : M;
+  if (S > 0.f) {
+    const float d = m - m0, f = __expf(d);
+    W = f * fmaf(fmaxf(d, -200.f), S, W);
+    S *= f;
   }
   S = reduce64(S, op_add());
   W = reduce64(W, op_add());
   if constexpr (TPR > 64) {
     if ((threadIdx.x & 63) == 0) {
-      red[1][threadIdx.x >> 6] = S;
-      red[2][threadIdx.x >> 6] = W;
+      red[1][wave] = S;
+      red[2][wave] = W;
     }
-  }
-  __syncthreads();
-  if constexpr (TPR > 64) {
+    __syncthreads();
     S = (red[1][0] + red[1][1]) + (red[1][2] + red[1][3]);
     W = (red[2][0] + red[2][1]) + (red[2][2] + red[2][3]);
   }
   float log_s = 0.f;
-  if (segs == 1) {
+  if (parts == 1) {
     log_s = S == 0.f ? 0.f : logf(S);
     if (live && lane == 0) {
       float xt;
       const bool has = lp_target<T, I>(xr, targets, row, V, &xt);
-      lp_finish_row(out, row, m, S, W, has, xt);
+      lp_finish_row(out, row, M, S, W, has, xt);
     }
   } else if (live && lane == 0) {
     float* st = stats + unit * 3;
-    st[0] = m;
+    st[0] = M;
     st[1] = S;
     st[2] = W;
   }
   if (k == 0 || !live) return;          // (block-uniform but for waves of TPR = 64, which meet no barrier below)
 
   auto emit = [&](int rank, u64 pair) {
-    if (segs == 1) {
+    if (parts == 1) {
       out.index[row * k + rank] = (int64_t)(uint32_t)~(uint32_t)pair;
       const uint32_t key = (uint32_t)(pair >> 32);
       out.top[row * k + rank] = key == 0xffffffffu ? NAN : (lp_unkey(key) - m0) - log_s;
@@ -218,6 +242,12 @@ k_log_probs(const T* __restrict__ x, int64_t ldx, const I* __restrict__ targets,
       best[unit * k + rank] = pair;
     }
   };
+  uint32_t bound = own;
+  if constexpr (TPR > 64) {
+#pragma unroll
+    for (int w = 0; w < 4; ++w) bound = bounds[w] > bound ? bounds[w] : bound;
+  }
+  bound = bound > NONE ? bound : NONE + 1;
   const int nv = vcount[grp];
   int n = LIST + 1;
   if (nv <= VLIST) {
@@ -239,28 +269,37 @@ k_log_probs(const T* __restrict__ x, int64_t ldx, const I* __restrict__ targets,
       for (int j = 0; j < n; ++j) rank += list[grp][j] > p;
       if (rank < k) emit(rank, p);
     }
-    if (segs > 1)                       // a last segment shorter than k
-      for (int i = n + lane; i < k; i += TPR) emit(i, 0);
+    // fewer than k classes above -inf: those of -inf in the order of their index, then (a short part) none
+    if (n < k && lane < 64) {
+      int at = n;
+      for (int base = first; base < end && at < k; base += 64) {
+        const int col = base + lane;
+        const bool none = col < end && lp_key(to_f32(xr[col])) == NONE;
+        const u64 mask = __ballot(none);
+        const int rank = at + __popcll(mask & ((1ull << lane) - 1));
+        if (none && rank < k) emit(rank, lp_pair(NONE, (uint32_t)col));
+        at += __popcll(mask);
+      }
+      if (at + lane < k) emit(at + lane, 0);
+    }
     return;
   }
   // many equal values, most large ones in few lanes, or not-a-number among them: k times the largest key below the last one
   u64 last = ~0ull;
   for (int rank = 0; rank < k; ++rank) {
     u64 mx = 0;
-#pragma unroll
-    for (int v = 0; v < NV; ++v)
+    for (int col = first + lane * VEC; col < end; col += TPR * VEC) {
+      const raw16 r = load_classes(xr, col, end);
 #pragma unroll
       for (int e = 0; e < VEC; ++e) {
-        const int col = first + (v * TPR + lane) * VEC + e;
-        if (col < end) {
-          const u64 p = lp_pair(lp_key(elem<T>(r[v], e)), (uint32_t)col);
-          if (p < last && p > mx) mx = p;
-        }
+        const u64 p = lp_pair(lp_key(elem<T>(r, e)), (uint32_t)(col + e));
+        if (col + e < end && p < last && p > mx) mx = p;
       }
+    }
     mx = wave_max_u64(mx);
     if constexpr (TPR > 64) {
       __syncthreads();                  // (the last round's winners are read)
-      if ((threadIdx.x & 63) == 0) winner[threadIdx.x >> 6] = mx;
+      if ((threadIdx.x & 63) == 0) winner[wave] = mx;
       __syncthreads();
 #pragma unroll
       for (int w = 0; w < 4; ++w) mx = winner[w] > mx ? winner[w] : mx;
@@ -270,7 +309,7 @@ k_log_probs(const T* __restrict__ x, int64_t ldx, const I* __restrict__ targets,
   }
 }
 
-// One block a row: the segments' lists go to LDS (every list is sorted), then the first wave joins the sums and takes k times
+// One block a row: the parts' lists go to LDS (every list is sorted), then the first wave joins the sums and takes k times
 // the largest of the lists' heads.
 template <typename T, typename I>
 __global__ void __launch_bounds__(256)
@@ -386,48 +425,68 @@ k_log_probs_bwd(const T* __restrict__ x, int64_t ldx, const I* __restrict__ targ
 }
 
 // ------------------------------------------------------------------------------------------------------- host ----
-struct lp_plan { int tpr, nv, segs; };
-static lp_plan lp_pick(int64_t rows, int V, int vec) {
+struct lp_plan { int tpr, nv, run, parts; };
+// A short row is one wave's.  A longer one is cut into segments, shorter ones while there are fewer than two blocks for a compute
+// unit; of full segments a block takes several behind each other (the list of alternatives then lets fewer and fewer vectors in,
+// and there is less to join: 2048 rows of 100003 classes in f16 with 8 alternatives took 162 us segment by segment, 91 us with
+// whole rows = 4.5 TB/s).
+#define LP_BLOCKS 2048     // blocks the chip holds at a time, eight a compute unit
+#define LP_RUN_TOP 32      // beyond, a wave's bound (of 64 lanes) is loose and lists of several segments would overflow
+static lp_plan lp_pick(int64_t rows, int V, int vec, int top) {
   lp_plan p;
+  p.run = p.parts = 1;
   if (V <= 64 * vec * 2) {
     p.tpr = 64;
     p.nv = V <= 64 * vec ? 1 : 2;
-    p.segs = 1;
     return p;
   }
   p.tpr = 256;
   p.nv = LP_SEG_VECS;
-  while (p.nv > 1 && (256 * vec * (p.nv / 2) >= V || rows * ((V + (int64_t)256 * vec * p.nv - 1) / (256 * vec * p.nv)) < 512)) p.nv /= 2;
-  p.segs = (V + (int64_t)256 * vec * p.nv - 1) / (256 * vec * p.nv);
+  auto segments = [&](int nv) { return ((int64_t)V + 256 * vec * nv - 1) / (256 * vec * nv); };
+  while (p.nv > 1 && (256 * vec * (p.nv / 2) >= V || rows * segments(p.nv) < 512)) p.nv /= 2;
+  const int64_t segs = segments(p.nv);
+  p.parts = (int)segs;
+  if (p.nv == LP_SEG_VECS && top <= LP_RUN_TOP) {
+    // as many parts as take the least time: rounds of blocks times segments of one, and 0.4 of a segment for what a block costs
+    float least = 1e30f;
+    for (int64_t parts = 1; parts <= segs && (parts == 1 || rows * (parts - 1) < 4 * LP_BLOCKS); ++parts) {
+      const float t = (float)((rows * parts + LP_BLOCKS - 1) / LP_BLOCKS) * ((float)((segs + parts - 1) / parts) + 0.4f);
+      if (t < least) {
+        least = t;
+        p.parts = (int)parts;
+      }
+    }
+  }
+  p.run = (int)((segs + p.parts - 1) / p.parts);         // even parts
   return p;
 }
 
 extern "C" size_t lmh_log_probs_workspace_bytes(int64_t rows, int V, int dtype, int top) {
   if (rows <= 0 || V <= 0 || V > LMH_ROW_MAX_COLS || top < 0 || top > LP_MAX_TOP) return 0;
-  const lp_plan p = lp_pick(rows, V, dtype == LMH_F32 ? 4 : 8);
-  if (p.segs == 1) return 0;
-  return lmh_align_up((size_t)rows * p.segs * 3 * sizeof(float), 256) + lmh_align_up((size_t)rows * p.segs * top * sizeof(u64), 256) + 256;
+  const lp_plan p = lp_pick(rows, V, dtype == LMH_F32 ? 4 : 8, top);
+  if (p.parts == 1) return 0;
+  return lmh_align_up((size_t)rows * p.parts * 3 * sizeof(float), 256) + lmh_align_up((size_t)rows * p.parts * top * sizeof(u64), 256) + 256;
 }
 
 template <typename T, typename I>
 static void lp_fwd_launch(const void* x, int64_t ldx, const void* targets, int64_t rows, int V, int k, const lp_out& o, void* ws, hipStream_t st) {
-  const lp_plan p = lp_pick(rows, V, row_type<T>::VEC);
+  const lp_plan p = lp_pick(rows, V, row_type<T>::VEC, k);
   float* stats = (float*)ws;
-  u64* best = ws ? (u64*)((char*)ws + lmh_align_up((size_t)rows * p.segs * 3 * sizeof(float), 256)) : nullptr;
-  const int64_t units = rows * p.segs;
+  u64* best = ws ? (u64*)((char*)ws + lmh_align_up((size_t)rows * p.parts * 3 * sizeof(float), 256)) : nullptr;
+  const int64_t units = rows * p.parts;
   const unsigned blocks = (unsigned)(p.tpr == 64 ? (units + 3) / 4 : units);
 #define LP_FWD(TPR_, NV_)                                                                                                   \
-  lmh_launch((k_log_probs<T, I, TPR_, NV_>), dim3(blocks), dim3(256), 0, st, (const T*)x, ldx, (const I*)targets, rows, V, k, p.segs, o, \
-             stats, best)
+  lmh_launch((k_log_probs<T, I, TPR_, NV_>), dim3(blocks), dim3(256), 0, st, (const T*)x, ldx, (const I*)targets, rows, V, k, p.run, p.parts, \
+             o, stats, best)
   if (p.tpr == 64) { if (p.nv == 1) LP_FWD(64, 1); else LP_FWD(64, 2); }
   else if (p.nv == 1) LP_FWD(256, 1);
   else if (p.nv == 2) LP_FWD(256, 2);
   else if (p.nv == 4) LP_FWD(256, 4);
   else LP_FWD(256, 8);
 #undef LP_FWD
-  if (p.segs > 1)       // few entries: one wave a row
-    lmh_launch((k_log_probs_join<T, I>), dim3((unsigned)rows), dim3(p.segs * k > 512 ? 256 : 64),
-               (unsigned)(p.segs <= 64 && p.segs * k <= LP_JOIN_LDS ? p.segs * k * sizeof(u64) : 0), st, (const T*)x, ldx, (const I*)targets, rows, V, k, p.segs, o,
+  if (p.parts > 1)       // few entries: one wave a row
+    lmh_launch((k_log_probs_join<T, I>), dim3((unsigned)rows), dim3(p.parts * k > 512 ? 256 : 64),
+               (unsigned)(p.parts <= 64 && p.parts * k <= LP_JOIN_LDS ? p.parts * k * sizeof(u64) : 0), st, (const T*)x, ldx, (const I*)targets, rows, V, k, p.parts, o,
                (const float*)stats, (const u64*)best);
 }
 
@@ -465,8 +524,8 @@ static bool lp_args_ok(int dtype, int64_t rows, int V, int64_t ldx, int top) {
   // a launch has fewer than 2^32 threads
   const int vec = dtype == LMH_F32 ? 4 : 8;
   if (rows > 0x3ffffff) return false;
-  const lp_plan p = lp_pick(rows, V, vec);
-  return rows * p.segs / (256 / p.tpr) < 0xffffff && rows * lp_bwd_chunks(rows, V, vec) < 0xffffff;
+  const lp_plan p = lp_pick(rows, V, vec, top);
+  return rows * p.parts / (256 / p.tpr) < 0xffffff && rows * lp_bwd_chunks(rows, V, vec) < 0xffffff;
 }
 
 extern "C" int lmh_log_probs_fwd(const void* x, int64_t ldx, int dtype, const void* targets, int index64, int64_t rows, int V, int top,

@@ -61,32 +61,95 @@ template <typename T> __device__ __forceinline__ raw16 pack16(const float* f) {
   }
   return r;
 }
-// One element into position e (a compile-time constant after unrolling) of a vector that is read element by element.
-template <typename T> __device__ __forceinline__ void put_elem(raw16& r, int e, T v) {
-  if constexpr (sizeof(T) == 4) r[e] = __float_as_uint(v.v);
-  else r[e >> 1] |= (uint32_t)__builtin_bit_cast(uint16_t, v) << (16 * (e & 1));
-}
-// Columns [col, col + VEC) of a row of D; zeros behind its end.
-template <typename T> __device__ __forceinline__ raw16 load_cols(const T* row, int col, int D) {
-  constexpr int VEC = row_type<T>::VEC;
-  raw16 r = {0, 0, 0, 0};
-  if (col + VEC <= D) {
-    r = load16(row + col);
-  } else if (col < D) {
-#pragma unroll
-    for (int e = 0; e < VEC; ++e)
-      if (col + e < D) put_elem<T>(r, e, row[col + e]);
+// The last vector of a row, `rem` < VEC values (the same for every lane: a row's length modulo VEC): 8, 4 and 2 bytes at a time, as
+// its bits say, so at most three accesses instead of seven.
+typedef uint32_t raw8_a4 __attribute__((ext_vector_type(2), aligned(4)));
+typedef uint32_t raw8_a2 __attribute__((ext_vector_type(2), aligned(2)));
+typedef uint32_t raw4_a2 __attribute__((aligned(2)));
+template <typename T> __device__ __forceinline__ raw16 load_tail(const T* p, int rem, uint32_t fill) {
+  raw16 r = {fill, fill, fill, fill};
+  if constexpr (sizeof(T) == 4) {
+    if (rem & 2) {
+      const raw8_a4 v = *reinterpret_cast<const raw8_a4*>(p);
+      r[0] = v[0];
+      r[1] = v[1];
+      if (rem & 1) r[2] = *reinterpret_cast<const uint32_t*>(p + 2);
+    } else {
+      r[0] = *reinterpret_cast<const uint32_t*>(p);
+    }
+  } else {
+    auto one = [&](int i) { return (fill & 0xffff0000u) | *reinterpret_cast<const uint16_t*>(p + i); };
+    if (rem & 4) {
+      const raw8_a2 v = *reinterpret_cast<const raw8_a2*>(p);
+      r[0] = v[0];
+      r[1] = v[1];
+      if (rem & 2) {
+        r[2] = *reinterpret_cast<const raw4_a2*>(p + 4);
+        if (rem & 1) r[3] = one(6);
+      } else if (rem & 1) {
+        r[2] = one(4);
+      }
+    } else if (rem & 2) {
+      r[0] = *reinterpret_cast<const raw4_a2*>(p);
+      if (rem & 1) r[1] = one(2);
+    } else {
+      r[0] = one(0);
+    }
   }
+  return r;
+}
+template <typename T> __device__ __forceinline__ void store_tail(T* p, int rem, raw16 r) {
+  if constexpr (sizeof(T) == 4) {
+    if (rem & 2) {
+      *reinterpret_cast<raw8_a4*>(p) = raw8_a4{r[0], r[1]};
+      if (rem & 1) *reinterpret_cast<uint32_t*>(p + 2) = r[2];
+    } else {
+      *reinterpret_cast<uint32_t*>(p) = r[0];
+    }
+  } else {
+    auto one = [&](int i, uint32_t v) { *reinterpret_cast<uint16_t*>(p + i) = (uint16_t)v; };
+    if (rem & 4) {
+      *reinterpret_cast<raw8_a2*>(p) = raw8_a2{r[0], r[1]};
+      if (rem & 2) {
+        *reinterpret_cast<raw4_a2*>(p + 4) = r[2];
+        if (rem & 1) one(6, r[3]);
+      } else if (rem & 1) {
+        one(4, r[2]);
+      }
+    } else if (rem & 2) {
+      *reinterpret_cast<raw4_a2*>(p) = r[0];
+      if (rem & 1) one(2, r[1]);
+    } else {
+      one(0, r[0]);
+    }
+  }
+}
+// Columns [col, col + VEC) of a row of D, col a multiple of VEC; `fill` (two 16-bit values or one of 32) behind its end.
+template <typename T> __device__ __forceinline__ raw16 load_cols(const T* row, int col, int D, uint32_t fill = 0) {
+  constexpr int VEC = row_type<T>::VEC;
+  raw16 r = {fill, fill, fill, fill};
+  if (col + VEC <= D) r = load16(row + col);
+  else if (col < D) r = load_tail(row + col, D & (VEC - 1), fill);
   return r;
 }
 template <typename T> __device__ __forceinline__ void store_cols(T* row, int col, int D, const float* f) {
   constexpr int VEC = row_type<T>::VEC;
-  if (col + VEC <= D) {
-    store16(row + col, pack16<T>(f));
-  } else if (col < D) {
+  if (col + VEC <= D) store16(row + col, pack16<T>(f));
+  else if (col < D) store_tail(row + col, D & (VEC - 1), pack16<T>(f));
+}
+
+// N parameters from column `col` on, `fill` where there are none.
+template <int N, typename P> __device__ __forceinline__ void load_params(float* out, const P* p, int col, int D, float fill) {
+  constexpr int VEC = row_type<P>::VEC < N ? row_type<P>::VEC : N;
 #pragma unroll
-    for (int e = 0; e < VEC; ++e)
-      if (col + e < D) row[col + e] = from_f32<T>(f[e]);
+  for (int i = 0; i < N; i += VEC) {
+    raw16 r = {0, 0, 0, 0};
+    if (p && VEC == row_type<P>::VEC) r = load_cols(p, col + i, D);
+#pragma unroll
+    for (int e = 0; e < VEC; ++e) {
+      out[i + e] = fill;
+      if (p && col + i + e < D) out[i + e] = VEC == row_type<P>::VEC ? elem<P>(r, e) : to_f32(p[col + i + e]);
+    }
   }
 }
 

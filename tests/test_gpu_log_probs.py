@@ -3,7 +3,8 @@ formulas in float64.
 
 Tolerances, u = 2^-24, z = x - max: x - max rounds to |z| u; an exponential is off by 2 |z| u (its argument's product) and 4 u of its
 own; a sum of up to 16384 classes rounds 64 times in a thread, some 10 times across, and once per segment when joined, so
-log S is off by at most (100 + 4 E|z|) u, E = mean under p.  The entropy's second sum has the same errors times |z|."""
+log S is off by at most (100 + 4 E|z|) u, E = mean under p.  (Several segments in a thread round as often as that many parts
+joined; a thread's maximum grows at most that often, by a factor with the errors of one exponential.)  The entropy's second sum has the same errors times |z|."""
 import math
 
 import pytest
@@ -115,6 +116,39 @@ def test_masks(C, dtype):
     logp, entropy, top, index, lse = (v.cpu() for v in K.log_probs_fwd(x.cuda(), t.cuda(), 20))
     assert logp[0] == 0 and entropy[0] == 0 and logp[1] == -math.inf and entropy[1] == 0 and lse[1] == -math.inf
     assert torch.equal(index[1], torch.arange(20)) and (top[1] == -math.inf).all() and logp[5] == -math.inf
+
+
+@pytest.mark.parametrize('rows,C,dtype', [(2100, 16389, torch.float32), (1400, 33001, torch.bfloat16), (4200, 16390, torch.float16)])
+@pytest.mark.parametrize('k', [1, 20, 40])
+def test_many_rows(rows, C, dtype, k):
+    """Enough rows that a block takes several segments of one: ordinary rows, rows in order, of one value, of few values, masked
+    ones.  The reference runs on the GPU in float64, on every 7th row and those."""
+    g = torch.Generator(device='cuda').manual_seed(C)
+    x = (torch.randn((rows, C), generator=g, device='cuda') * 3).to(dtype)
+    t = torch.randint(0, C, (rows,), generator=g, device='cuda')
+    x[0] = torch.linspace(-9, 9, C, device='cuda')
+    x[7] = torch.linspace(9, -9, C, device='cuda')
+    x[14] = 1.5
+    x[21] = torch.randint(-3, 3, (C,), generator=g, device='cuda').to(dtype)
+    x[28] = -math.inf
+    x[35, torch.randperm(C, generator=g, device='cuda')[: C - 9]] = -math.inf
+    x[42, : C - 5] = -math.inf
+    x[49, 11:] = -math.inf
+    x[56, ::2] = -math.inf
+    x[63] = 0.0
+    x[63, ::3] = -0.0
+    x[70, C // 2] = math.nan
+    t[77] = -1
+    got = K.log_probs_fwd(x, t, k)
+    at = torch.arange(0, rows, 7)
+    at = at[at != 70]
+    xs = x[at.cuda()].cpu()
+    check_fwd(xs, t[at.cuda()].cpu(), k, [v[at.cuda()].cpu() for v in got])
+    assert torch.isnan(got[0][70]) and torch.isnan(got[2][70]).all() and int(got[3][70, 0]) == C // 2
+    other = K.log_probs_fwd(x, t, 0)                       # without alternatives: the same sums
+    for a, b in zip(got, other):
+        if b is not None:
+            assert torch.equal(a.nan_to_num(7), b.nan_to_num(7)) or k > 32
 
 
 def test_not_a_number_and_no_class():
