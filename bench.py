@@ -424,7 +424,9 @@ def main():
         # Every process started by a launcher (torch.distributed.run sets WORLD_SIZE, also for ONE rank) gets the same
         # mapping, so the N = 1 point of a scaling run and its N > 1 points differ in the exchange only; the plain
         # `python bench.py` headline keeps HIP's default (A/B of the two at N = 1: DESIGN.md 8).
-        os.environ.setdefault('GPU_MAX_HW_QUEUES', '8')
+        # (a machine may export HIP's own default, 4: fewer queues than the step has streams)
+        if int(os.environ.get('GPU_MAX_HW_QUEUES') or 0) < 8:
+            os.environ['GPU_MAX_HW_QUEUES'] = '8'
     rank = int(os.environ.get('RANK', '0'))
     local_rank = int(os.environ.get('LOCAL_RANK', '0'))
     if not torch.cuda.is_available():
