@@ -357,10 +357,11 @@ def allreduce_probe(flat_numel, device, reps=5, bucket_mb=12):
                                 'correct': bool(abs(float(t[0]) - world) < 1e-3)})
         del t
     (ts, bs), (tl, bl) = sorted(times.values(), key=lambda v: v[1])
-    bucket, alpha, beta = bucket_bytes_from_probe(ts, bs, tl, bl)
+    # a quarter of the gradient at most, whatever a collective costs: larger buckets leave nothing to exchange under the backward
+    bucket, alpha, beta = bucket_bytes_from_probe(ts, bs, tl, bl, hi=min(64 << 20, max(4 << 20, int(flat_numel) >> 20 << 20)))
     out.update({'alpha_us': alpha * 1e6, 'beta_GB/s': beta / 1e9, 'bucket_bytes_from_probe': bucket,
                 'model': 't(bytes) = alpha + bytes / beta from the two messages; bucket = smallest size with alpha <= 25 % of '
-                         'its transfer time, 1 MB steps, clamped to [4, 64] MB'})
+                         'its transfer time, 1 MB steps, clamped to [4, 64] MB and to a quarter of the gradient'})
     return out
 
 
