@@ -264,12 +264,26 @@ __device__ __forceinline__ void mu_store(const float* v, char* cols, char* rows,
   }
 }
 
-// Tile t (row by row) of the upper triangle of tm x tm tiles.
+// Tile t of the upper triangle of tm x tm tiles: in strips of eight rows, a strip column by column, so that neighbours share
+// operands.
 __device__ __forceinline__ void mu_triangle(int t, int tm, int* ti, int* tj) {
-  int i = 0;
-  while (t >= tm - i) t -= tm - i++;
-  *ti = i;
-  *tj = i + t;
+  int top = 0, high = min(8, tm), all;
+  while (t >= (all = high * (high + 1) / 2 + high * (tm - top - high))) {
+    t -= all;
+    top += high;
+    high = min(8, tm - top);
+  }
+  const int corner = high * (high + 1) / 2;  // the strip's first columns are cut off by the diagonal
+  if (t < corner) {
+    int c = 0;
+    while (t > c) t -= ++c;
+    *ti = top + t;
+    *tj = top + c;
+  } else {
+    t -= corner;
+    *ti = top + t % high;
+    *tj = top + high + t / high;
+  }
 }
 
 // The accumulator of 32-blocks (rb, cb) of a symmetric result, scaled into its one or two buffers, and mirrored unless the
