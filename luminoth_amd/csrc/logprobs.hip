@@ -15,6 +15,9 @@
 // segment -, of those the values that reach the last bound into a second one, and an entry's place there is the number of
 // larger ones.  Value and index make one 64-bit key (larger value first, then lower index): all keys differ, so the order in
 // which lanes append does not matter.  Parts of one row are joined by a second launch.
+#include <algorithm>
+#include <cmath>
+
 #include "rowops.h"
 
 #define LP_MAX_TOP LMH_LOG_PROBS_MAX_TOP
@@ -94,19 +97,19 @@ template <typename T> __device__ __forceinline__ raw16 load_classes(const T* row
   return load_cols(row, col, end, __is_same(T, f32_t) ? 0xff800000u : __is_same(T, f16_t) ? 0xfc00fc00u : 0xff80ff80u);
 }
 
-// TPR threads a row or a part of one (64: one wave, no block-wide step; 256: the block), NV vectors a thread and segment, `run`
+// TPR threads a row or a part of one (64: one wave, no block-wide step; 256 or 1024: the block), NV vectors a thread and segment, `run`
 // segments a part.  Results of a part: stats[(row * parts + part) * 3] and, sorted, best[(row * parts + part) * k].
 template <typename T, typename I, int TPR, int NV>
-__global__ void __launch_bounds__(256)
+__global__ void __launch_bounds__(TPR > 256 ? TPR : 256)
 k_log_probs(const T* __restrict__ x, int64_t ldx, const I* __restrict__ targets, int64_t rows, int V, int k, int run, int parts, lp_out out,
             float* __restrict__ stats, u64* __restrict__ best) {
-  constexpr int VEC = row_type<T>::VEC, SEG = TPR * NV * VEC, GPB = 256 / TPR;
-  constexpr int LIST = TPR == 64 ? 128 : 512, VLIST = TPR == 64 ? 128 : 512;
+  constexpr int VEC = row_type<T>::VEC, SEG = TPR * NV * VEC, GPB = TPR > 256 ? 1 : 256 / TPR, NW = TPR > 256 ? TPR / 64 : 4;
+  constexpr int LIST = TPR == 64 ? 128 : 512, VLIST = TPR == 64 ? 128 : TPR == 256 ? 512 : 1024;
   constexpr uint32_t NONE = 0x007fffffu;                        // the key of -inf
-  __shared__ float red[3][4];
-  __shared__ uint32_t bounds[4];
+  __shared__ float red[3][NW];
+  __shared__ uint32_t bounds[NW];
   __shared__ u64 list[GPB][LIST];
-  __shared__ u64 winner[4];
+  __shared__ u64 winner[NW];
   __shared__ raw16 vlist[GPB][VLIST];
   __shared__ int vcol[GPB][VLIST], vcount[GPB], count[GPB];
   const int lane = threadIdx.x & (TPR - 1), grp = threadIdx.x / TPR, wave = threadIdx.x >> 6;
@@ -162,7 +165,7 @@ k_log_probs(const T* __restrict__ x, int64_t ldx, const I* __restrict__ targets,
           volatile uint32_t* b = bounds;
           if ((threadIdx.x & 63) == 0) b[wave] = now;
 #pragma unroll
-          for (int w = 0; w < 4; ++w) {
+          for (int w = 0; w < NW; ++w) {
             const uint32_t o = b[w];
             low = o > low ? o : low;
           }
@@ -198,7 +201,7 @@ k_log_probs(const T* __restrict__ x, int64_t ldx, const I* __restrict__ targets,
     }
     __syncthreads();
 #pragma unroll
-    for (int w = 0; w < 4; ++w) M = fmaxf(M, red[0][w]);
+    for (int w = 0; w < NW; ++w) M = fmaxf(M, red[0][w]);
   }
   const float m0 = M == -INFINITY ? 0.f : M;
   if (S > 0.f) {
@@ -214,8 +217,12 @@ k_log_probs(const T* __restrict__ x, int64_t ldx, const I* __restrict__ targets,
       red[2][wave] = W;
     }
     __syncthreads();
-    S = (red[1][0] + red[1][1]) + (red[1][2] + red[1][3]);
-    W = (red[2][0] + red[2][1]) + (red[2][2] + red[2][3]);
+    S = W = 0.f;
+#pragma unroll
+    for (int w = 0; w < NW; ++w) {
+      S += red[1][w];
+      W += red[2][w];
+    }
   }
   float log_s = 0.f;
   if (parts == 1) {
@@ -245,7 +252,7 @@ k_log_probs(const T* __restrict__ x, int64_t ldx, const I* __restrict__ targets,
   uint32_t bound = own;
   if constexpr (TPR > 64) {
 #pragma unroll
-    for (int w = 0; w < 4; ++w) bound = bounds[w] > bound ? bounds[w] : bound;
+    for (int w = 0; w < NW; ++w) bound = bounds[w] > bound ? bounds[w] : bound;
   }
   bound = bound > NONE ? bound : NONE + 1;
   const int nv = vcount[grp];
@@ -257,6 +264,20 @@ k_log_probs(const T* __restrict__ x, int64_t ldx, const I* __restrict__ targets,
       if (key >= bound && col < end) {
         const int at = atomicAdd(&count[grp], 1);
         if (at < LIST) list[grp][at] = lp_pair(key, (uint32_t)col);
+      }
+    }
+    if constexpr (TPR > 64) __syncthreads();
+    n = count[grp];
+  } else if (S == S) {                  // more vectors than the list holds: once more through the part, with the last bound
+    for (int col = first + lane * VEC; col < end; col += TPR * VEC) {
+      const raw16 r = load_classes(xr, col, end);
+#pragma unroll
+      for (int e = 0; e < VEC; ++e) {
+        const uint32_t key = lp_key(elem<T>(r, e));
+        if (key >= bound && col + e < end) {
+          const int at = atomicAdd(&count[grp], 1);
+          if (at < LIST) list[grp][at] = lp_pair(key, (uint32_t)(col + e));
+        }
       }
     }
     if constexpr (TPR > 64) __syncthreads();
@@ -284,7 +305,7 @@ k_log_probs(const T* __restrict__ x, int64_t ldx, const I* __restrict__ targets,
     }
     return;
   }
-  // many equal values, most large ones in few lanes, or not-a-number among them: k times the largest key below the last one
+  // many equal values or not-a-number among them: k times the largest key below the last one
   u64 last = ~0ull;
   for (int rank = 0; rank < k; ++rank) {
     u64 mx = 0;
@@ -302,7 +323,7 @@ k_log_probs(const T* __restrict__ x, int64_t ldx, const I* __restrict__ targets,
       if ((threadIdx.x & 63) == 0) winner[wave] = mx;
       __syncthreads();
 #pragma unroll
-      for (int w = 0; w < 4; ++w) mx = winner[w] > mx ? winner[w] : mx;
+      for (int w = 0; w < NW; ++w) mx = winner[w] > mx ? winner[w] : mx;
     }
     if (lane == 0) emit(rank, mx);
     last = mx;
@@ -431,7 +452,9 @@ struct lp_plan { int tpr, nv, run, parts; };
 // and there is less to join: 2048 rows of 100003 classes in f16 with 8 alternatives took 162 us segment by segment, 91 us with
 // whole rows = 4.5 TB/s).
 #define LP_BLOCKS 2048     // blocks the chip holds at a time, eight a compute unit
-#define LP_RUN_TOP 32      // beyond, a wave's bound (of 64 lanes) is loose and lists of several segments would overflow
+// Up to 256 rows of at most this many bytes go to one large block each: 1 x 60000 bf16 takes 11 us, as in parts with the launch that
+// joins them (5 + 5 us), but one launch of the host's; 40 x 130000 19 us against 7 + 5.
+#define LP_ALONE 131072
 static lp_plan lp_pick(int64_t rows, int V, int vec, int top) {
   lp_plan p;
   p.run = p.parts = 1;
@@ -440,16 +463,25 @@ static lp_plan lp_pick(int64_t rows, int V, int vec, int top) {
     p.nv = V <= 64 * vec ? 1 : 2;
     return p;
   }
+  if (rows <= 256 && (int64_t)V * (16 / vec) <= LP_ALONE) {
+    p.tpr = 1024;
+    p.nv = LP_SEG_VECS;
+    while (p.nv > 1 && 1024 * vec * (p.nv / 2) >= V) p.nv /= 2;
+    p.run = (V + 1024 * vec * p.nv - 1) / (1024 * vec * p.nv);
+    return p;
+  }
   p.tpr = 256;
   p.nv = LP_SEG_VECS;
   auto segments = [&](int nv) { return ((int64_t)V + 256 * vec * nv - 1) / (256 * vec * nv); };
-  while (p.nv > 1 && (256 * vec * (p.nv / 2) >= V || rows * segments(p.nv) < 512)) p.nv /= 2;
+  while (p.nv > 1 && (256 * vec * (p.nv / 2) >= V || (rows * segments(p.nv) < 512 && segments(p.nv / 2) <= 64))) p.nv /= 2;
   const int64_t segs = segments(p.nv);
   p.parts = (int)segs;
-  if (p.nv == LP_SEG_VECS && top <= LP_RUN_TOP) {
+  // n segments of random values put at most about 4.8 top (log n + 0.6) vectors into the list of 512: as many as make 400
+  const int most = top ? (int)std::min(1e6, std::max(1.0, std::exp(std::min(20.0, 400 / (4.8 * top) - 0.6)))) : 1000000;
+  if (p.nv == LP_SEG_VECS) {
     // as many parts as take the least time: rounds of blocks times segments of one, and 0.4 of a segment for what a block costs
     float least = 1e30f;
-    for (int64_t parts = 1; parts <= segs && (parts == 1 || rows * (parts - 1) < 4 * LP_BLOCKS); ++parts) {
+    for (int64_t parts = (segs + most - 1) / most, lo = parts; parts <= segs && (parts == lo || rows * (parts - 1) < 4 * LP_BLOCKS); ++parts) {
       const float t = (float)((rows * parts + LP_BLOCKS - 1) / LP_BLOCKS) * ((float)((segs + parts - 1) / parts) + 0.4f);
       if (t < least) {
         least = t;
@@ -457,6 +489,7 @@ static lp_plan lp_pick(int64_t rows, int V, int vec, int top) {
       }
     }
   }
+  if (top > 0 && p.parts > 64) p.parts = 64;      // a lane of the joining wave has one list
   p.run = (int)((segs + p.parts - 1) / p.parts);         // even parts
   return p;
 }
@@ -474,15 +507,15 @@ static void lp_fwd_launch(const void* x, int64_t ldx, const void* targets, int64
   float* stats = (float*)ws;
   u64* best = ws ? (u64*)((char*)ws + lmh_align_up((size_t)rows * p.parts * 3 * sizeof(float), 256)) : nullptr;
   const int64_t units = rows * p.parts;
-  const unsigned blocks = (unsigned)(p.tpr == 64 ? (units + 3) / 4 : units);
+  const unsigned blocks = (unsigned)(p.tpr == 64 ? (units + 3) / 4 : units);      // (256 or 1024 threads a part)
 #define LP_FWD(TPR_, NV_)                                                                                                   \
-  lmh_launch((k_log_probs<T, I, TPR_, NV_>), dim3(blocks), dim3(256), 0, st, (const T*)x, ldx, (const I*)targets, rows, V, k, p.run, p.parts, \
+  lmh_launch((k_log_probs<T, I, TPR_, NV_>), dim3(blocks), dim3(TPR_ > 256 ? TPR_ : 256), 0, st, (const T*)x, ldx, (const I*)targets, rows, V, k, p.run, p.parts, \
              o, stats, best)
   if (p.tpr == 64) { if (p.nv == 1) LP_FWD(64, 1); else LP_FWD(64, 2); }
+  else if (p.tpr == 1024) { if (p.nv == 1) LP_FWD(1024, 1); else if (p.nv == 2) LP_FWD(1024, 2); else LP_FWD(1024, 4); }
   else if (p.nv == 1) LP_FWD(256, 1);
   else if (p.nv == 2) LP_FWD(256, 2);
-  else if (p.nv == 4) LP_FWD(256, 4);
-  else LP_FWD(256, 8);
+  else LP_FWD(256, 4);
 #undef LP_FWD
   if (p.parts > 1)       // few entries: one wave a row
     lmh_launch((k_log_probs_join<T, I>), dim3((unsigned)rows), dim3(p.parts * k > 512 ? 256 : 64),
@@ -525,7 +558,7 @@ static bool lp_args_ok(int dtype, int64_t rows, int V, int64_t ldx, int top) {
   const int vec = dtype == LMH_F32 ? 4 : 8;
   if (rows > 0x3ffffff) return false;
   const lp_plan p = lp_pick(rows, V, vec, top);
-  return rows * p.parts / (256 / p.tpr) < 0xffffff && rows * lp_bwd_chunks(rows, V, vec) < 0xffffff;
+  return rows * p.parts / (p.tpr == 64 ? 4 : 1) < 0xffffff && rows * lp_bwd_chunks(rows, V, vec) < 0xffffff;
 }
 
 extern "C" int lmh_log_probs_fwd(const void* x, int64_t ldx, int dtype, const void* targets, int index64, int64_t rows, int V, int top,

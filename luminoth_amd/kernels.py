@@ -6,7 +6,6 @@ that merely own the memory.  Nothing in this file computes with torch ops, and
 nothing falls back to the CPU: tensors must live on a ROCm device.
 """
 import ctypes
-import functools
 import threading
 import os
 
@@ -1295,18 +1294,6 @@ def _new_like(t):
 _get_device = getattr(torch._C, '_cuda_getDevice', torch.cuda.current_device)      # (~10x cheaper than current_device())
 
 
-def _on_device_of(fn):
-    """The call runs with the device of its first tensor as the current one (its current stream is the launch stream)."""
-    @functools.wraps(fn)
-    def call(first, *args, **kwargs):
-        t = first if isinstance(first, torch.Tensor) else first[0] if len(first) else None
-        if t is None or not t.is_cuda or t.get_device() == _get_device():
-            return fn(first, *args, **kwargs)
-        with torch.cuda.device(t.device):
-            return fn(first, *args, **kwargs)
-    return call
-
-
 def _row_stream(dev):
     if _stream_override is not None:
         return _stream_override
@@ -1328,7 +1315,6 @@ def _ln_params(x, cols, *params):
     return ROW_DTYPES[torch.float32 if dtype is None else dtype]
 
 
-@_on_device_of
 def layer_norm_fwd(x, gamma=None, beta=None, eps=1e-5):
     """y = (x - mean) * rstd * gamma + beta over the last dimension of x (..., D) in float32, float16 or bfloat16 -> (y like x
     but contiguous, mean, rstd: float32 of shape (...)).  Rows may lie in a wider buffer."""
@@ -1336,6 +1322,9 @@ def layer_norm_fwd(x, gamma=None, beta=None, eps=1e-5):
     rows, cols, ld = _rows_of(x, 'layer_norm')
     pdtype = _ln_params(x, cols, gamma, beta)
     dev = _same_device(x, gamma, beta)
+    if dev != _get_device():
+        with torch.cuda.device(dev):
+            return layer_norm_fwd(x, gamma, beta, eps)
     y = _new_like(x)
     mean = _new(x.shape[:-1], torch.float32, x.device)
     rstd = _new_like(mean)
@@ -1344,7 +1333,6 @@ def layer_norm_fwd(x, gamma=None, beta=None, eps=1e-5):
     return y, mean, rstd
 
 
-@_on_device_of
 def layer_norm_bwd(dy, x, mean, rstd, gamma=None, dgamma=None, dbeta=None, addend=None, need_dx=True):
     """-> dx (contiguous; + addend, the gradient of x from its other consumers); dgamma / dbeta (D,), float32 or x's type, are
     written when given (sums over all rows in a fixed order)."""
@@ -1362,6 +1350,9 @@ def layer_norm_bwd(dy, x, mean, rstd, gamma=None, dgamma=None, dbeta=None, adden
     _refuse(rstd.shape != lead or rstd.dtype is not torch.float32, 'layer_norm: rstd of the forward expected')
     pdtype = _ln_params(x, cols, gamma, dgamma, dbeta)
     dev = _same_device(x, dy, mean, rstd, gamma, dgamma, dbeta, addend)
+    if dev != _get_device():
+        with torch.cuda.device(dev):
+            return layer_norm_bwd(dy, x, mean, rstd, gamma, dgamma, dbeta, addend, need_dx)
     dx = _new_like(x) if need_dx else None
     ws, nbytes = None, 0
     if dgamma is not None or dbeta is not None:
@@ -1390,7 +1381,6 @@ def _lp_args(logits, targets, top_k):
     return dtype, rows, cols, ld, index64
 
 
-@_on_device_of
 def log_probs_fwd(logits, targets=None, top_k=0):
     """logits (..., C) in float32, float16 or bfloat16, targets (...) int32 / int64 or None -> (logp, entropy, top_logp, top_index,
     lse): log p of the targets (None without them), entropy -sum p log p and log sum exp of every row (float32), and the top_k
@@ -1401,6 +1391,9 @@ def log_probs_fwd(logits, targets=None, top_k=0):
     k = int(top_k)
     dtype, rows, cols, ld, index64 = _lp_args(logits, targets, k)
     dev = _same_device(logits, targets)
+    if dev != _get_device():
+        with torch.cuda.device(dev):
+            return log_probs_fwd(logits, targets, k)
     device, lead = logits.device, logits.shape[:-1]
     entropy = _new(lead, torch.float32, device)
     lse = _new_like(entropy)
@@ -1414,7 +1407,6 @@ def log_probs_fwd(logits, targets=None, top_k=0):
     return logp, entropy, top, index, lse
 
 
-@_on_device_of
 def log_probs_bwd(logits, targets, lse, entropy, g_logp=None, g_entropy=None, top_index=None, g_top=None):
     """-> gradient of the logits (their type, contiguous) from the gradients of log_probs_fwd's logp, entropy and top_logp (each
     may be None)."""
@@ -1433,6 +1425,9 @@ def log_probs_bwd(logits, targets, lse, entropy, g_logp=None, g_entropy=None, to
         _refuse(top_index.shape != lead + (k,) or top_index.dtype is not torch.int64 or g_top.shape != top_index.shape or
                 g_top.dtype is not torch.float32, 'log_probs: int64 alternatives and their float32 gradients of one shape expected')
     dev = _same_device(logits, targets, lse, entropy, g_logp, g_entropy, top_index, g_top)
+    if dev != _get_device():
+        with torch.cuda.device(dev):
+            return log_probs_bwd(logits, targets, lse, entropy, g_logp, g_entropy, top_index, g_top)
     dx = _new_like(logits)
     what = 'log_probs'
     check(lib.lmh_log_probs_bwd(_pr(logits), ld, dtype, _flat(targets, what), index64, _flat(lse, what), _flat(entropy, what),
@@ -1492,7 +1487,6 @@ def _matrix_of(t, what):
     return rows, cols
 
 
-@_on_device_of
 def orthogonalize(mats, steps=5, eps=1e-7):
     """O(U) of every matrix of the list (one type: float32, float16 or bfloat16; (..., out) weights count as (inputs, out)): `steps`
     Newton-Schulz steps that take the singular values to about 1 -> list of new tensors.  One set of launches for all of
@@ -1508,7 +1502,10 @@ def orthogonalize(mats, steps=5, eps=1e-7):
     for j, u in zip(jobs, mats):
         _refuse(u.dtype != mats[0].dtype, 'orthogonalize: matrices of one type expected, got %s and %s', mats[0].dtype, u.dtype)
         j.rows, j.cols = _matrix_of(u, 'orthogonalize')
-    _same_device(*mats)
+    dev = _same_device(*mats)
+    if dev != _get_device():
+        with torch.cuda.device(dev):
+            return orthogonalize(mats, steps, eps)
     for j, u in zip(jobs, mats):
         o = _new(u.shape, u.dtype, u.device)
         out.append(o)
@@ -1542,7 +1539,7 @@ class MuonJobs(object):
             j.rows, j.cols = _matrix_of(w, 'muon')
             j.wd = float(weight_decay[i]) if isinstance(weight_decay, (list, tuple)) else float(weight_decay)
             j.scale = float(scale[i]) if scale is not None else 0.2 * max(j.rows, j.cols) ** 0.5
-        _same_device(*self.tensors)
+        self.device = _same_device(*self.tensors)
         for i, (j, w, g, v) in enumerate(zip(self.jobs, params, grads, moms)):
             j.w, j.g, j.v = _p(w).value, _p(g).value, _p(v).value
             j.factor = _p(factors[i]).value if factors else None
@@ -1551,18 +1548,14 @@ class MuonJobs(object):
         _refuse(any(a[1] > b[0] for a, b in zip(spans, spans[1:])), 'muon: weights and momenta overlap')
         self.ws_bytes = _lib.load().lmh_muon_workspace_bytes(self.jobs, n)
 
-    def __len__(self):
-        return self.count
 
-    def __getitem__(self, i):
-        return self.tensors[i]
-
-
-@_on_device_of
 def muon_jobs_step(jobs, lr, momentum=0.95, nesterov=True, steps=5, eps=1e-7, gscale=1.0):
     """One step of lmh_muon_step over the matrices of a MuonJobs, in place: g' = (gscale g + wd w) factor, v = momentum v + g',
     w -= lr scale O(nesterov ? g' + momentum v : v)."""
     _refuse(not 1 <= int(steps) <= 64 or not float(eps) > 0, 'muon: 1 to 64 steps and eps > 0 expected')
+    if jobs.device != _get_device():
+        with torch.cuda.device(jobs.device):
+            return muon_jobs_step(jobs, lr, momentum, nesterov, steps, eps, gscale)
     lib = _lib.load()
     plan_keep(*jobs.tensors)
     ws = _new((jobs.ws_bytes,), torch.uint8, jobs.tensors[0].device)

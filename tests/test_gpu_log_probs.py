@@ -151,6 +151,19 @@ def test_many_rows(rows, C, dtype, k):
             assert torch.equal(a.nan_to_num(7), b.nan_to_num(7)) or k > 32
 
 
+@pytest.mark.parametrize('rows,C,dtype,k', [(2, 1000003, torch.float32, 40), (2, 300007, torch.bfloat16, 64), (3000, 20000, torch.float16, 64)])
+def test_long_lists_of_alternatives(rows, C, dtype, k):
+    """More vectors than the list of a part holds, and more parts than 64."""
+    g = torch.Generator(device='cuda').manual_seed(k)
+    x = (torch.randn((rows, C), generator=g, device='cuda') * 2).to(dtype)
+    x[0] = torch.linspace(-20, 20, C, device='cuda')
+    x[1, 5:] = x[1, 5]
+    t = torch.arange(rows, device='cuda')
+    got = K.log_probs_fwd(x, t, k)
+    n = min(rows, 200)
+    check_fwd(x[:n].cpu(), t[:n].cpu(), k, [v[:n].cpu() for v in got])
+
+
 def test_not_a_number_and_no_class():
     x, t = make(5, 3000, torch.float32)
     x[1, 17] = math.nan
