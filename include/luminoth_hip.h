@@ -232,7 +232,7 @@ int lmh_layer_norm_bwd(const void* dy, int64_t lddy, const void* x, int64_t ldx,
  * not-a-number comes first).  A target < 0 is not asked for: logp 0, no gradient; one >= cols gives not-a-number.  Classes of
  * -inf have p = 0; in a row of -inf alone every log probability and lse are -inf, entropy and gradient 0.
  * Backward: dx = g_logp (1[target] - p) + sum_i g_top[i] (1[top_index[i]] - p) - g_entropy p (log p + entropy); g_logp, g_entropy
- * may be NULL, top = 0: no alternatives. */
+ * may be NULL, top = 0: no alternatives.  Fewer than 2^24 - 1 rows, and parts of long rows, a call. */
 #define LMH_LOG_PROBS_MAX_TOP 64
 size_t lmh_log_probs_workspace_bytes(int64_t rows, int cols, int dtype, int top);
 int lmh_log_probs_fwd(const void* x, int64_t ldx, int dtype, const void* targets, int index64, int64_t rows, int cols, int top,
@@ -246,7 +246,8 @@ int lmh_log_probs_bwd(const void* x, int64_t ldx, int dtype, const void* targets
  * eps), in products of fp32 accuracy.
  * lmh_orthogonalize: out = O(g); g and out of `dtype`.
  * lmh_muon_step (fp32): g' = (g gscale + wd w) * factor, v = momentum v + g', U = nesterov ? g' + momentum v : v,
- * w -= lr scale O(U); `factor`: one float on the device (a clip factor of lmh_grad_clip_factors) or NULL. */
+ * w -= lr scale O(U); `factor`: one float on the device (a clip factor of lmh_grad_clip_factors) or NULL.  Every w and v is
+ * a matrix of its own, apart from each other, from g and from the factors. */
 #define LMH_MUON_MAX_JOBS 65536
 #define LMH_MUON_MAX_DIM (1 << 17)      /* rows and columns; rows * cols <= 2^30 */
 #define LMH_MUON_MAX_STEPS 64

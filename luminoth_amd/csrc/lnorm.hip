@@ -328,22 +328,25 @@ template <typename P>
 __global__ void __launch_bounds__(1024)
 k_ln_params(const float* __restrict__ part, int nb, int D, int W, int tpr, int vec, P* __restrict__ dgamma, P* __restrict__ dbeta) {
   __shared__ float red[16][65];
-  const int64_t i = (int64_t)blockIdx.x * 64 + (threadIdx.x & 63);      // place in [dgamma | dbeta]
   const int s = threadIdx.x >> 6;
-  float a = 0.f;
-  if (i < 2 * (int64_t)W) {
+  for (int64_t first = (int64_t)blockIdx.x * 64; first < 2 * (int64_t)W; first += (int64_t)gridDim.x * 64) {
+    const int64_t i = first + (threadIdx.x & 63);                       // place in [dgamma | dbeta]
+    float a = 0.f;
+    if (i < 2 * (int64_t)W) {
 #pragma unroll 8
-    for (int r = s; r < nb; r += 16) a += part[(size_t)r * 2 * W + i];
-  }
-  red[s][threadIdx.x & 63] = a;
-  __syncthreads();
-  if (s == 0 && i < 2 * (int64_t)W) {
+      for (int r = s; r < nb; r += 16) a += part[(size_t)r * 2 * W + i];
+    }
+    red[s][threadIdx.x & 63] = a;
+    __syncthreads();
+    if (s == 0 && i < 2 * (int64_t)W) {
 #pragma unroll
-    for (int r = 1; r < 16; ++r) a += red[r][threadIdx.x];
-    P* out = i < W ? dgamma : dbeta;
-    int p = (int)(i < W ? i : i - W);
-    if (tpr) p = (p / tpr / vec * tpr + p % tpr) * vec + p / tpr % vec;
-    if (out && p < D) out[p] = from_f32<P>(a);
+      for (int r = 1; r < 16; ++r) a += red[r][threadIdx.x];
+      P* out = i < W ? dgamma : dbeta;
+      int p = (int)(i < W ? i : i - W);
+      if (tpr) p = (p / tpr / vec * tpr + p % tpr) * vec + p / tpr % vec;
+      if (out && p < D) out[p] = from_f32<P>(a);
+    }
+    __syncthreads();
   }
 }
 
@@ -380,18 +383,23 @@ static int ln_part_cols(int D, int vec) {         // columns of a partial row
 static bool ln_dtype_ok(int d) { return d == LMH_F32 || d == LMH_F16 || d == LMH_BF16; }
 static int ln_vec(int d) { return d == LMH_F32 ? 4 : 8; }
 
-#define LN_PICK_NC(CALL, T, P, TPR)                                             \
+// CALL(T, P, threads, vectors) for a shape: one or two vectors of 16-bit values, two or four of fp32 (one too for 16 threads).
+// LEAST: of a row of 1024 threads in 16 bits
+#define LN_PICK_NC(CALL, T, P, TPR, LEAST16)                                    \
   do {                                                                          \
-    if (row_type<T>::VEC == 8) { if (s.nc == 1) CALL(T, P, TPR, 1); else CALL(T, P, TPR, 2); } \
-    else { if (s.nc == 1) CALL(T, P, TPR, 1); else if (s.nc == 2) CALL(T, P, TPR, 2); else CALL(T, P, TPR, (row_type<T>::VEC == 8 ? 2 : 4)); } \
+    if constexpr (row_type<T>::VEC == 8) {                                      \
+      if (s.nc <= LEAST16) CALL(T, P, TPR, LEAST16); else CALL(T, P, TPR, 2);   \
+    } else {                                                                    \
+      if (TPR == 16 && s.nc == 1) CALL(T, P, 16, 1); else if (s.nc == 2) CALL(T, P, TPR, 2); else CALL(T, P, TPR, 4); \
+    }                                                                           \
   } while (0)
-#define LN_PICK(CALL, T, P)                                                     \
+#define LN_PICK(CALL, T, P, LEAST)                                              \
   do {                                                                          \
     switch (s.tpr) {                                                            \
-      case 16: LN_PICK_NC(CALL, T, P, 16); break;                               \
-      case 64: LN_PICK_NC(CALL, T, P, 64); break;                               \
-      case 256: LN_PICK_NC(CALL, T, P, 256); break;                             \
-      default: LN_PICK_NC(CALL, T, P, 1024);                                    \
+      case 16: LN_PICK_NC(CALL, T, P, 16, 1); break;                            \
+      case 64: LN_PICK_NC(CALL, T, P, 64, 1); break;                            \
+      case 256: LN_PICK_NC(CALL, T, P, 256, 1); break;                          \
+      default: LN_PICK_NC(CALL, T, P, 1024, LEAST);                             \
     }                                                                           \
   } while (0)
 
@@ -413,12 +421,11 @@ static void ln_fwd_launch(const void* x, int64_t ldx, const void* gamma, const v
              rstd, rows, D, inv_d, eps)
   if constexpr (row_type<T>::VEC == 8) {
     if (s.tpr == 512) {
-      if (s.nc == 1) LN_FWD(T, P, 512, 1);
-      else LN_FWD(T, P, 512, 2);
+      LN_FWD(T, P, 512, 2);
       return;
     }
   }
-  LN_PICK(LN_FWD, T, P);
+  LN_PICK(LN_FWD, T, P, 2);
 #undef LN_FWD
 }
 
@@ -445,12 +452,13 @@ static void ln_bwd_launch(const void* dy, int64_t lddy, const void* x, int64_t l
   lmh_launch((k_ln_bwd<T_, P_, TPR_, NC_, (TPR_ == 1024 ? 1024 : 512), (TPR_ < 1024)>), dim3((unsigned)nb), dim3(ln_bwd_threads(TPR_)),     \
              (unsigned)(TPR_ == 1024 ? 0 : 512 / TPR_ / 2 * 2 * sizeof(float) * NC_ * row_type<T_>::VEC * TPR_), st, (const T_*)dy, lddy, (const T_*)x, ldx, (const T_*)addend, ldadd, \
              mean, rstd, (const P_*)gamma, (T_*)dx, p, rows, D, inv_d)
-    LN_PICK(LN_BWD, T, P);
+    LN_PICK(LN_BWD, T, P, 1);
 #undef LN_BWD
   }
   if (params) {
     const int W = ln_part_cols(D, row_type<T>::VEC), tpr = D > LN_MAX_REG_COLS ? 0 : ln_pick(D, row_type<T>::VEC).tpr;
-    lmh_launch((k_ln_params<P>), dim3((unsigned)((2 * (int64_t)W + 63) / 64)), dim3(1024), 0, st, (const float*)part, nb, D, W, tpr,
+    const int64_t strips = (2 * (int64_t)W + 63) / 64;
+    lmh_launch((k_ln_params<P>), dim3((unsigned)(strips < 65536 ? strips : 65536)), dim3(1024), 0, st, (const float*)part, nb, D, W, tpr,
                row_type<T>::VEC, (P*)dgamma, (P*)dbeta);
   }
 }

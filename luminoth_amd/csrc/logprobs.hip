@@ -402,16 +402,19 @@ k_log_probs_join(const T* __restrict__ x, int64_t ldx, const I* __restrict__ tar
 }
 
 // Gradient: a thread's vectors of one row, then the given classes' own entries, written whole (p, entropy and every
-// gradient given for that class, in the order target, alternative 0, 1, ...) by one thread each, behind a barrier.
-template <typename T, typename I>
+// gradient given for that class, in the order target, alternative 0, 1, ...) by one thread each, behind a barrier.  A short row is
+// one wave's, a longer one is cut into `chunks` of one block each.
+template <typename T, typename I, int TPR>
 __global__ void __launch_bounds__(256)
 k_log_probs_bwd(const T* __restrict__ x, int64_t ldx, const I* __restrict__ targets, const float* __restrict__ lse,
                 const float* __restrict__ entropy, const float* __restrict__ g_logp, const float* __restrict__ g_entropy,
                 const int64_t* __restrict__ index, const float* __restrict__ g_top, int64_t rows, int V, int k, int chunk, int chunks,
                 T* __restrict__ dx) {
   constexpr int VEC = row_type<T>::VEC;
-  const int64_t row = blockIdx.x / chunks;
-  const int first = (int)(blockIdx.x % chunks) * chunk;
+  const int lane = threadIdx.x & (TPR - 1);
+  const int64_t row = TPR == 64 ? (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6) : blockIdx.x / chunks;
+  if (TPR == 64 && row >= rows) return;                         // (no barrier below)
+  const int first = TPR == 64 ? 0 : (int)(blockIdx.x % chunks) * chunk;
   const int end = V - first < chunk ? V : first + chunk;
   const T* xr = x + row * ldx;
   T* dr = dx + row * (int64_t)V;
@@ -427,7 +430,7 @@ k_log_probs_bwd(const T* __restrict__ x, int64_t ldx, const I* __restrict__ targ
     const float lp = f - l, p = __expf(lp);
     return p > 0.f || p != p ? -p * fmaf(gh, lp + h, G) : 0.f;
   };
-  for (int col = first + (int)threadIdx.x * VEC; col < end; col += 256 * VEC) {
+  for (int col = first + lane * VEC; col < end; col += TPR * VEC) {
     const raw16 r = load_cols(xr, col, end);
     float o[VEC];
 #pragma unroll
@@ -435,8 +438,10 @@ k_log_probs_bwd(const T* __restrict__ x, int64_t ldx, const I* __restrict__ targ
     store_cols(dr, col, end, o);
   }
   if (empty) return;
-  __syncthreads();
-  for (int i = (int)threadIdx.x - 1; i < k; i += 256) {
+  // the vectors' stores come first: those of the block, or of this wave
+  if constexpr (TPR == 64) asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+  else __syncthreads();
+  for (int i = lane - 1; i < k; i += TPR) {
     const int64_t at = i < 0 ? t : index[row * k + i];
     if (at < first || at >= end) continue;
     float g = at == t ? gt : 0.f;
@@ -540,8 +545,12 @@ static void lp_bwd_launch(const void* x, int64_t ldx, const void* targets, const
                           hipStream_t st) {
   const int chunk = lp_bwd_chunk(rows, V, row_type<T>::VEC);
   const int chunks = (int)lp_bwd_chunks(rows, V, row_type<T>::VEC);
-  lmh_launch((k_log_probs_bwd<T, I>), dim3((unsigned)(rows * chunks)), dim3(256), 0, st, (const T*)x, ldx, (const I*)targets, lse, entropy,
-             g_logp, g_entropy, index, g_top, rows, V, k, chunk, chunks, (T*)dx);
+#define LP_BWD(TPR_, BLOCKS_)                                                                                               \
+  lmh_launch((k_log_probs_bwd<T, I, TPR_>), dim3((unsigned)(BLOCKS_)), dim3(256), 0, st, (const T*)x, ldx, (const I*)targets, lse, entropy, \
+             g_logp, g_entropy, index, g_top, rows, V, k, chunk, chunks, (T*)dx)
+  if (V <= 64 * row_type<T>::VEC * 2) LP_BWD(64, (rows + 3) / 4);
+  else LP_BWD(256, rows * chunks);
+#undef LP_BWD
 }
 
 #define LP_TYPES(FN, ...)                                                                                                   \
@@ -556,7 +565,7 @@ static bool lp_args_ok(int dtype, int64_t rows, int V, int64_t ldx, int top) {
   if (rows < 0 || V <= 0 || V > LMH_ROW_MAX_COLS || ldx < V || top < 0 || top > LP_MAX_TOP || top > V) return false;
   // a launch has fewer than 2^32 threads
   const int vec = dtype == LMH_F32 ? 4 : 8;
-  if (rows > 0x3ffffff) return false;
+  if (rows >= 0xffffff) return false;
   const lp_plan p = lp_pick(rows, V, vec, top);
   return rows * p.parts / (p.tpr == 64 ? 4 : 1) < 0xffffff && rows * lp_bwd_chunks(rows, V, vec) < 0xffffff;
 }

@@ -182,9 +182,9 @@ k_mu_planes(mu_table tab, mu_jobs jobs, char* ws, float eps) {
   __syncthreads();
   double norm = sqrt(total);
   if (norm < (double)eps) norm = (double)eps;            // (not a number stays one)
-  const float inv = (float)((double)MU_SX / norm);
+  const double inv = (double)MU_SX / norm;               // (may lie outside fp32's range, X does not)
 #pragma unroll
-  for (int i = 0; i < 16; ++i) tile[i * 4 + (threadIdx.x >> 6)][threadIdx.x & 63] = x[i] * inv;
+  for (int i = 0; i < 16; ++i) tile[i * 4 + (threadIdx.x >> 6)][threadIdx.x & 63] = (float)((double)x[i] * inv);
   __syncthreads();
   // stored rows as rows (k = stored columns): X for a wide matrix, X' for a tall one; and the other way round
   char* by_row = mu_at(ws, g, job, g.tall ? g.d1 : g.d0);

@@ -1386,7 +1386,7 @@ def log_probs_fwd(logits, targets=None, top_k=0):
     lse): log p of the targets (None without them), entropy -sum p log p and log sum exp of every row (float32), and the top_k
     (<= 64) most probable classes with their log p, (..., top_k) float32 / int64, equal ones in the order of their index (None
     with top_k = 0).  A target -1 is not asked for (0), one that is no class gives nan.  Classes of -inf have p = 0; a row of -inf
-    alone has log p = lse = -inf and entropy 0.  include/luminoth_hip.h lmh_log_probs_fwd."""
+    alone has log p = lse = -inf and entropy 0.  Fewer than 2^24 - 1 rows a call.  include/luminoth_hip.h lmh_log_probs_fwd."""
     lib = _lib.load()
     k = int(top_k)
     dtype, rows, cols, ld, index64 = _lp_args(logits, targets, k)
@@ -1539,13 +1539,17 @@ class MuonJobs(object):
             j.rows, j.cols = _matrix_of(w, 'muon')
             j.wd = float(weight_decay[i]) if isinstance(weight_decay, (list, tuple)) else float(weight_decay)
             j.scale = float(scale[i]) if scale is not None else 0.2 * max(j.rows, j.cols) ** 0.5
+        # what is written must be nobody else's: a matrix given twice, or overlapping views, would be updated by two blocks at a time
+        spans = sorted((t.data_ptr(), t.data_ptr() + 4 * t.numel(), 1) for t in params + moms)
+        _refuse(any(a[1] > b[0] for a, b in zip(spans, spans[1:])), 'muon: weights and momenta overlap')
+        spans, end, read_end = sorted(spans + [(t.data_ptr(), t.data_ptr() + 4 * t.numel(), 0) for t in grads + factors]), 0, 0
+        for lo, hi, written in spans:
+            _refuse(lo < end or (written and lo < read_end), 'muon: gradients or factors overlap weights or momenta')
+            end, read_end = (hi, read_end) if written else (end, max(read_end, hi))
         self.device = _same_device(*self.tensors)
         for i, (j, w, g, v) in enumerate(zip(self.jobs, params, grads, moms)):
             j.w, j.g, j.v = _p(w).value, _p(g).value, _p(v).value
             j.factor = _p(factors[i]).value if factors else None
-        # what is written must be nobody else's: a matrix given twice, or overlapping views, would be updated by two blocks at a time
-        spans = sorted((t.data_ptr(), t.data_ptr() + 4 * t.numel()) for t in params + moms)
-        _refuse(any(a[1] > b[0] for a, b in zip(spans, spans[1:])), 'muon: weights and momenta overlap')
         self.ws_bytes = _lib.load().lmh_muon_workspace_bytes(self.jobs, n)
 
 

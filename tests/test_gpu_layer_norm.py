@@ -231,3 +231,61 @@ def test_streams_and_graph():
         dx2 = K.layer_norm_bwd(dy, x, m2, r2, gamma, dg2, db2)
         for a, b in ((y, y2), (dx, dx2), (dg, dg2), (db, db2)):
             assert torch.equal(a, b)
+
+
+def test_rows_far_apart_and_results_beyond_32_bits():
+    """Rows 2^30 values apart (offsets pass 2^31), and more than 2^31 values in all: a row does not depend on the others."""
+    ld = 2 ** 30 + 64
+    far = torch.empty(3 * ld, device='cuda', dtype=torch.bfloat16)
+    x, dy = (far.as_strided((3, 1000), (ld, 1), at) for at in (0, 2000))
+    x.copy_(make(3, 1000, torch.bfloat16))
+    dy.copy_(make(3, 1000, torch.bfloat16, seed=1))
+    for a, b in zip(K.layer_norm_fwd(x), K.layer_norm_fwd(x.contiguous())):
+        assert torch.equal(a, b)
+    _, mean, rstd = K.layer_norm_fwd(x)
+    assert torch.equal(K.layer_norm_bwd(dy, x, mean, rstd, addend=dy), K.layer_norm_bwd(dy.contiguous(), x.contiguous(), mean, rstd, addend=dy))
+    del far, x, dy
+    x = torch.empty((2 ** 19 + 3, 4096), device='cuda', dtype=torch.bfloat16).normal_()
+    y, mean, rstd = K.layer_norm_fwd(x)
+    for a, b in zip((y, mean, rstd), K.layer_norm_fwd(x[-5:])):
+        assert torch.equal(a[-5:], b)
+    dx = K.layer_norm_bwd(y, x, mean, rstd)
+    assert torch.equal(dx[-5:], K.layer_norm_bwd(y[-5:], x[-5:], mean[-5:], rstd[-5:]))
+
+
+def test_parameters_of_very_long_rows():
+    """More columns than one launch has threads for: two rows, so a column's sum is one addition of fp32 products (three roundings
+    each, of x - mean, times rstd, times dy)."""
+    D = 2 ** 27 + 5
+    x, dy = torch.empty((2, D), device='cuda').normal_(), torch.empty((2, D), device='cuda').normal_()
+    mean, rstd = torch.tensor([0.25, -0.5], device='cuda'), torch.tensor([1.5, 0.75], device='cuda')
+    dg, db = torch.empty(D, device='cuda'), torch.empty(D, device='cuda')
+    assert K.layer_norm_bwd(dy, x, mean, rstd, None, dg, db, need_dx=False) is None
+    for lo in range(0, D, 2 ** 25):
+        X, Y = x[:, lo:lo + 2 ** 25].double(), dy[:, lo:lo + 2 ** 25].double()
+        each = Y * (X - mean.double()[:, None]) * rstd.double()[:, None]
+        assert ((dg[lo:lo + 2 ** 25].double() - each.sum(0)).abs() <= 5 * U * each.abs().sum(0) + 1e-37).all()
+        assert ((db[lo:lo + 2 ** 25].double() - Y.sum(0)).abs() <= U * Y.sum(0).abs() + 1e-37).all()
+
+
+def test_two_graphs_in_turn():
+    """Two captured backward passes with partial sums of their own, replayed one behind the other with eager calls between."""
+    sets, graphs, outs = [], [], []
+    for seed, D in ((0, 700), (1, 5000)):
+        x, dy = make(90, D, torch.float32, seed=seed).cuda(), make(90, D, torch.float32, seed=seed + 5).cuda()
+        y, mean, rstd = K.layer_norm_fwd(x)
+        sets.append((dy, x, mean, rstd, None, torch.empty(D, device='cuda'), torch.empty(D, device='cuda')))
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            outs.append(K.layer_norm_bwd(*sets[-1]))
+        graphs.append(graph)
+    for _ in range(3):
+        for s in sets:
+            s[0].mul_(-0.5)
+        graphs[0].replay()
+        graphs[1].replay()
+        torch.cuda.synchronize()
+        for s, dx in zip(sets, outs):
+            dg, db = torch.empty_like(s[5]), torch.empty_like(s[6])
+            assert torch.equal(dx, K.layer_norm_bwd(*s[:5], dg, db))
+            assert torch.equal(s[5], dg) and torch.equal(s[6], db)

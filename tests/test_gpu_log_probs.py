@@ -314,3 +314,62 @@ def test_streams_and_graph():
         e = K.log_probs_fwd(x, t, 6)
         for a, b in zip((logp, entropy, top, index, lse, dx), e + (K.log_probs_bwd(x, t, e[4], e[1], ones, ones),)):
             assert torch.equal(a, b)
+
+
+@pytest.mark.parametrize('C', [20, 3000])
+def test_targets_of_32_bits_and_repeated_alternatives(C):
+    x, t = make(7, C, torch.bfloat16)
+    t[2] = -1
+    dev, t64, t32 = x.cuda(), t.cuda(), t.int().cuda()
+    for a, b in zip(K.log_probs_fwd(dev, t64, 3), K.log_probs_fwd(dev, t32, 3)):
+        assert torch.equal(a, b)
+    _, entropy, _, _, lse = K.log_probs_fwd(dev, None, 0)
+    index = torch.tensor([[C - 1, 0, C - 1, 5]] * 7)
+    gl, gt = torch.linspace(-1, 1, 7), torch.linspace(-3, 2, 28).view(7, 4)
+    dx = [K.log_probs_bwd(dev, v, lse, entropy, gl.cuda(), None, index.cuda(), gt.cuda()) for v in (t64, t32)]
+    assert torch.equal(dx[0], dx[1])
+    want, tol = bwd_reference(x, t, gl, None, index, gt)
+    near(dx[0], want, tol + 2.0 ** -8 * (want.abs() + tol) + 1e-37, 'repeated')
+
+
+def test_rows_far_apart_and_results_beyond_32_bits():
+    ld, t = 2 ** 30 + 64, torch.tensor([5, 2999, 0]).cuda()
+    far = torch.empty(3 * ld, device='cuda', dtype=torch.bfloat16)
+    x = far.as_strided((3, 3000), (ld, 1))
+    x.copy_(make(3, 3000, torch.bfloat16)[0])
+    got, want = K.log_probs_fwd(x, t, 4), K.log_probs_fwd(x.contiguous(), t, 4)
+    for a, b in zip(got, want):
+        assert torch.equal(a, b)
+    ones = torch.ones(3, device='cuda')
+    assert torch.equal(K.log_probs_bwd(x, t, got[4], got[1], ones, ones), K.log_probs_bwd(x.contiguous(), t, got[4], got[1], ones, ones))
+    del far, x
+    rows, C = 2 ** 16 + 3, 33000
+    x = torch.empty((rows, C), device='cuda', dtype=torch.bfloat16).normal_()
+    t = torch.randint(0, C, (rows,), generator=torch.Generator().manual_seed(0))
+    logp, entropy, top, index, lse = K.log_probs_fwd(x, t.cuda(), 2)
+    check_fwd(x[-3:].cpu(), t[-3:], 2, [v[-3:] for v in (logp, entropy, top, index, lse)])
+    ones = torch.ones(rows, device='cuda')
+    dx = K.log_probs_bwd(x, t.cuda(), lse, entropy, ones, ones)
+    want, tol = bwd_reference(x[-3:].cpu(), t[-3:], torch.ones(3), torch.ones(3), None, None)
+    near(dx[-3:], want, tol + 2.0 ** -8 * (want.abs() + tol) + 1e-37, 'last rows')
+
+
+def test_two_graphs_in_turn():
+    """Two captured calls whose rows are joined from parts, replayed one behind the other with eager calls between."""
+    inputs, graphs, outs = [], [], []
+    for seed, C in ((0, 300007), (1, 70001)):
+        x, t = make(3, C, torch.float32, seed=seed)
+        inputs.append((x.cuda(), t.cuda(), 5))
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            outs.append(K.log_probs_fwd(*inputs[-1]))
+        graphs.append(graph)
+    for _ in range(3):
+        for x, _, _ in inputs:
+            x.mul_(-0.75)
+        graphs[0].replay()
+        graphs[1].replay()
+        torch.cuda.synchronize()
+        for args, got in zip(inputs, outs):
+            for a, b in zip(got, K.log_probs_fwd(*args)):
+                assert torch.equal(a, b)

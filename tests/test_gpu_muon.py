@@ -163,3 +163,42 @@ def test_same_bits_streams_and_graph():
         for inputs, got in ((mats, outs[0]), (other, outs[1])):
             for a, b in zip(got, K.orthogonalize(inputs)):
                 assert torch.equal(a, b)
+
+
+@pytest.mark.parametrize('rows,cols', [(4100, 4200), (4000, 9000)])
+def test_large_matrices(rows, cols):
+    """More tiles than one round of blocks takes: the last ones are split along k and joined; the reference on the device too."""
+    u = make(rows, cols).cuda()
+    out, = K.orthogonalize([u])
+    want = ns(u)
+    assert float(torch.linalg.norm(out.double() - want)) <= bound(u) + 2.0 ** -24 * float(torch.linalg.norm(want))
+
+
+def test_norms_at_the_ends_of_the_range():
+    """8192 / |U|_F, the factor of the planes, beyond fp32's range at both ends (and below its normal numbers)."""
+    tiny = make(40, 90, scale=1e-36)
+    close(K.orthogonalize([tiny.cuda()], eps=1e-38)[0], tiny, eps=1e-38)
+    huge = make(2600, 2700).clamp(-3.0, 3.0) * 1e38
+    out, = K.orthogonalize([huge.cuda()])
+    want = ns(huge.cuda())
+    assert float(torch.linalg.norm(out.double() - want)) <= bound(huge) + 2.0 ** -24 * float(torch.linalg.norm(want))
+
+
+def test_many_steps_stay_in_the_band():
+    """The quintic takes [0.68, 1.21] into itself (its extremes there: 1.2025 at 0.5545 from below, 0.682 at 1.0501), and every
+    singular value that fp32 can tell from zero gets there in 64 steps; rounding adds 2^-20 at most a step, which the slopes
+    in the band (below 3.5 in magnitude) do not let grow past 2^-17 while a value moves to and fro inside it."""
+    u = make(64, 96)
+    s = torch.linalg.svdvals(K.orthogonalize([u.cuda()], steps=64)[0].cpu().double())
+    assert s.min() >= 0.67 and s.max() <= 1.22
+
+
+def test_one_gradient_for_two_weights():
+    w = [make(48, 32, seed=i).cuda() for i in range(2)]
+    v = [torch.zeros_like(t) for t in w]
+    g = make(48, 32, seed=7).cuda()
+    w2, v2 = [t.clone() for t in w], [t.clone() for t in v]
+    K.muon_step(w, [g, g], v, lr=0.1)
+    K.muon_step(w2, [g.clone(), g.clone()], v2, lr=0.1)
+    for a, b in zip(w + v, w2 + v2):
+        assert torch.equal(a, b)

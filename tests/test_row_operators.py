@@ -63,6 +63,21 @@ def test_refusals(call, text):
         call()
 
 
+def test_muon_refuses_shared_memory():
+    w, g, v = z(4, 8), z(4, 8), z(4, 8)
+    flat = z(80)
+    for params, grads, moms, factors, text in (([w, w], [g, g], [v, z(4, 8)], None, 'weights and momenta overlap'),
+                                               ([w], [g], [w], None, 'weights and momenta overlap'),
+                                               ([flat[:32].view(4, 8)], [g], [flat[24:56].view(4, 8)], None, 'weights and momenta overlap'),
+                                               ([w], [v], [v], None, 'gradients or factors overlap'),
+                                               ([w], [w], [v], None, 'gradients or factors overlap'),
+                                               ([flat[40:72].view(4, 8)], [flat[16:48].view(4, 8)], [v], None, 'gradients or factors overlap'),
+                                               ([w], [g], [v], [v.view(-1)[:1]], 'gradients or factors overlap'),
+                                               ([w, z(4, 8)], [g, g], [v, z(4, 8)], [flat[:1], flat[:1]], 'ROCm device')):
+        with pytest.raises(Err, match=text):
+            K.muon_step(params, grads, moms, lr=0.1, factors=factors)
+
+
 def test_c_entries_refuse_before_they_launch():
     lib = _lib.load()
     buf = (ctypes.c_float * 64)()
@@ -80,7 +95,7 @@ def test_c_entries_refuse_before_they_launch():
                                            k.get('cols', 8), k.get('top', 0), k.get('lp', None), p, p, k.get('tl', p), k.get('ti', p),
                                            k.get('ws', p), k.get('n', 1 << 20), None)
     for bad in (dict(x=None), dict(ld=7), dict(dt=-1), dict(t=p), dict(lp=p), dict(top=9), dict(cols=100, ld=100, top=65), dict(top=-1),
-                dict(top=2, tl=None), dict(top=2, ti=None), dict(rows=-3), dict(rows=2 ** 40)):
+                dict(top=2, tl=None), dict(top=2, ti=None), dict(rows=-3), dict(rows=2 ** 40), dict(rows=2 ** 24 - 1)):
         assert lp(**bad) == -1, bad
     assert lp(cols=40000, ld=40000, n=0) == -3 and lp(cols=40000, ld=40000, ws=None) == -3 and lp(rows=0) == 0
     lb = lambda **k: lib.lmh_log_probs_bwd(p, 8, 0, k.get('t', None), 1, k.get('lse', p), k.get('h', p), k.get('gl', None),      # noqa: E731
