@@ -27,6 +27,7 @@
 // Products with too few tiles for the chip (a long k), and the tiles that a last round of blocks would leave over, are split
 // along k; their parts are joined, in order, by a launch of their own.
 #include <algorithm>
+#include <tuple>
 #include <vector>
 
 #include "rowops.h"
@@ -42,6 +43,11 @@
 #define MU_SQ 1024.f      // products of up to three of them
 #define MU_MAX_GROUPS 24  // of one launch (kernel arguments: under 4 KB together)
 #define MU_MAX_JOBS 44
+// up to this many tiles of 64 x 64: tiles of 32 x 32 with four waves on each (one matrix, all steps: 1024 x 320, 15 tiles, 165 -> 121 us;
+// 512 x 1024, 36 tiles, 188 -> 138; 1024 x 2048, 136 tiles, 356 -> 291; no gain from there on: 1408 x 1500, 253 tiles, 448 and 443;
+// the 42 matrices of a ResNet-50 detector, 328 tiles, 13.3 us a launch both)
+#define MU_SMALL 160
+#define MU_SMALL_X 256        // ... of the products with X
 #define MU_NORM_BLOCKS 256
 #define MU_NORM_ELEMS 2048    // at least this many per block of k_mu_norm
 
@@ -289,12 +295,12 @@ __device__ __forceinline__ void mu_triangle(int t, int tm, int* ti, int* tj) {
 // The accumulator of 32-blocks (rb, cb) of a symmetric result, scaled into its one or two buffers, and mirrored unless the
 // whole tile lies on the diagonal.
 __device__ __forceinline__ void mu_store_symmetric(const mu_task& g, char* ws, int job, const float* acc, int rb, int cb, bool mirror,
-                                                   int lane, uint32_t* turn) {
+                                                   int lane, uint32_t* turn, int only = -1) {
   const int l31 = lane & 31, h = lane >> 5, units = g.pm / 16;
 #pragma unroll
   for (int k = 0; k < 2; ++k) {
     const int d = k ? g.d1 : g.d0;
-    if (d < 0) continue;
+    if (d < 0 || (only >= 0 && k != only)) continue;
     const float s = k ? g.s1 : g.s0, on = k ? g.g1 : g.g0;
     float v[16];
 #pragma unroll
@@ -499,11 +505,155 @@ k_mu_last(mu_table tab, mu_jobs jobs, char* ws, float lr) {
   mu_gemm_tile<T, TW, KU, DEPTH, MU_LAST, OPT>(tab, &jobs, ws, lr);
 }
 
-// Joins the parts of split tiles, one 32 x 32 block of a tile each wave (blk0 counts tiles).
-template <int TW>
+// Few tiles: one of 32 x 32 by four waves, a quarter of k each.  What bounds such a launch is how fast a compute unit gets its operands
+// from beyond its die's L2 (some 40 GB/s: another die wrote them; a stage of 32 k of a 64 x 64 tile took 0.42 us, whether two or
+// seven more were on their way), so more units with less each: operands come straight to registers (eight units of 16 k on
+// their way in a wave), without LDS and barriers, and the quarters are added in LDS, in order.
+template <typename T, int MODE, bool OPT>
+__device__ __forceinline__ void mu_small_tile(const mu_table& tab, const mu_jobs* jobs, char* ws, float lr) {
+  constexpr int CHUNK = 4;
+  __shared__ __attribute__((aligned(16))) float quarter[4][1024];
+  __shared__ __attribute__((aligned(16))) uint32_t turns[2][32 * MU_PITCH];
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, l31 = lane & 31, h = lane >> 5;
+  int blk = blockIdx.x;
+  constexpr int RUN = 32;                    // neighbours on a die, as above (8: 4-5 % slower)
+  if (blk < (int)(gridDim.x / (8 * RUN) * (8 * RUN))) blk = blk / (8 * RUN) * (8 * RUN) + (blk & 7) * RUN + (blk >> 3) % RUN;
+  const int gi = mu_find(tab, blk);
+  const mu_task& g = tab.t[gi];
+  int u = blk - tab.blk0[gi], split = 0, ti, tj;
+  const int tm = g.pm / 32, tn = g.pn / 32, per = MODE == MU_SYM ? tm * (tm + 1) / 2 : tm * tn;
+  const bool part = MODE == MU_SYM && g.whole == 0;
+  int job, t;
+  if (part) {
+    const unsigned both = (unsigned)per * g.splits, in = (unsigned)u % both;
+    job = (unsigned)u / both;
+    split = in / (unsigned)per;
+    t = in - split * per;
+    u = job * per + t;
+  } else {
+    job = (unsigned)u / (unsigned)per;
+    t = u - job * per;
+  }
+  const bool turned = MODE == MU_LAST && !g.tall;
+  if (MODE == MU_SYM) {
+    mu_triangle(t, tm, &ti, &tj);
+  } else {
+    const int row = t / tm, col = t % tm;
+    ti = turned ? col : row;
+    tj = turned ? row : col;
+  }
+  const int kunits = g.aux;
+  int k0 = 0, k1 = kunits;
+  if (part) {
+    k0 = (int)((unsigned)kunits * split / (unsigned)g.splits);
+    k1 = (int)((unsigned)kunits * (split + 1) / (unsigned)g.splits);
+  }
+  const int u0 = k0 + (k1 - k0) * wave / 4, u1 = k0 + (k1 - k0) * (wave + 1) / 4;
+  const char* L = mu_at(ws, g, job, turned ? g.r : g.l) + (int64_t)ti * kunits * 2048 + lane * 16;
+  const char* R = mu_at(ws, g, job, turned ? g.l : g.r) + (int64_t)tj * kunits * 2048 + lane * 16;
+  f32x16 acc;
+#pragma unroll
+  for (int i = 0; i < 16; ++i) acc[i] = 0.f;
+  f16x8 f[2][CHUNK][4];
+  auto fetch = [&](int at, f16x8 (&d)[CHUNK][4]) {
+#pragma unroll
+    for (int c = 0; c < CHUNK; ++c) {
+      const int64_t off = (int64_t)max(min(at + c, u1 - 1), u0) * 2048;          // (behind the end: the last unit, not used)
+      d[c][0] = *reinterpret_cast<const f16x8*>(L + off);
+      d[c][1] = *reinterpret_cast<const f16x8*>(L + off + 1024);
+      d[c][2] = *reinterpret_cast<const f16x8*>(R + off);
+      d[c][3] = *reinterpret_cast<const f16x8*>(R + off + 1024);
+    }
+  };
+  auto work = [&](int at, const f16x8 (&d)[CHUNK][4]) {
+#pragma unroll
+    for (int c = 0; c < CHUNK; ++c)
+      if (at + c < u1) {
+        acc = __builtin_amdgcn_mfma_f32_32x32x16_f16(d[c][0], d[c][3], acc, 0, 0, 0);
+        acc = __builtin_amdgcn_mfma_f32_32x32x16_f16(d[c][1], d[c][2], acc, 0, 0, 0);
+        acc = __builtin_amdgcn_mfma_f32_32x32x16_f16(d[c][0], d[c][2], acc, 0, 0, 0);
+      }
+  };
+  if (u0 < u1) {
+    fetch(u0, f[0]);
+    for (int at = u0; at < u1; at += 2 * CHUNK) {
+      if (at + CHUNK < u1) fetch(at + CHUNK, f[1]);
+      work(at, f[0]);
+      if (at + 2 * CHUNK < u1) fetch(at + 2 * CHUNK, f[0]);
+      if (at + CHUNK < u1) work(at + CHUNK, f[1]);
+    }
+  }
+#pragma unroll
+  for (int i = 0; i < 4; ++i)
+    *reinterpret_cast<float4*>(&quarter[wave][i * 256 + lane * 4]) = make_float4(acc[4 * i], acc[4 * i + 1], acc[4 * i + 2], acc[4 * i + 3]);
+  __syncthreads();
+  if (MODE != MU_LAST && wave >= 2) return;
+  float v[16];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    float4 a = *reinterpret_cast<const float4*>(&quarter[0][i * 256 + lane * 4]);
+#pragma unroll
+    for (int w = 1; w < 4; ++w) {
+      const float4 b = *reinterpret_cast<const float4*>(&quarter[w][i * 256 + lane * 4]);
+      a.x += b.x;
+      a.y += b.y;
+      a.z += b.z;
+      a.w += b.w;
+    }
+    v[4 * i] = a.x;
+    v[4 * i + 1] = a.y;
+    v[4 * i + 2] = a.z;
+    v[4 * i + 3] = a.w;
+  }
+  uint32_t* turn = turns[wave & 1];
+  if constexpr (MODE == MU_SYM) {
+    if (part) {
+      if (wave) return;
+      float* s = (float*)(ws + (int64_t)g.slab * 256) + ((int64_t)u * g.splits + split) * 1024;
+#pragma unroll
+      for (int q = 0; q < 4; ++q) *reinterpret_cast<float4*>(s + q * 256 + lane * 4) = make_float4(v[4 * q], v[4 * q + 1], v[4 * q + 2], v[4 * q + 3]);
+      return;
+    }
+    mu_store_symmetric(g, ws, job, v, ti, tj, ti != tj, lane, turn, wave);
+  } else if constexpr (MODE == MU_APPLY) {
+    if (wave) return;
+#pragma unroll
+    for (int i = 0; i < 16; ++i) v[i] *= g.s0;
+    mu_store(v, mu_at(ws, g, job, g.d0) + ((int64_t)tj * (g.pn / 16) + ti * 2) * 2048, mu_at(ws, g, job, g.d1) + ((int64_t)ti * (g.pm / 16) + tj * 2) * 2048,
+             lane, turn);
+  } else {
+    const mu_ptrs& p = jobs->p[g.first + job];
+    float* out = (float*)p.out;
+    const int rows = g.tall ? g.n : g.m, cols = g.tall ? g.m : g.n;
+    const float scale = OPT ? lr * p.scale * g.s0 : g.s0;
+    const int c = tj * 32 + l31, r0 = ti * 32 + 4 * h;
+#pragma unroll
+    for (int i = 0; i < 16; ++i) {
+      if ((i >> 2) != wave) continue;                  // four rows of every eight a wave
+      const int r = r0 + (i & 3) + 8 * (i >> 2);
+      if (r < rows && c < cols) {
+        if constexpr (OPT) out[(int64_t)r * cols + c] -= scale * v[i];
+        else ((T*)p.out)[(int64_t)r * cols + c] = from_f32<T>(scale * v[i]);
+      }
+    }
+  }
+}
+template <int MODE>
+__global__ void __launch_bounds__(256)
+k_mu_small(mu_table tab, char* ws) {
+  mu_small_tile<f32_t, MODE, false>(tab, nullptr, ws, 0.f);
+}
+template <typename T, bool OPT>
+__global__ void __launch_bounds__(256)
+k_mu_small_last(mu_table tab, mu_jobs jobs, char* ws, float lr) {
+  mu_small_tile<T, MU_LAST, OPT>(tab, &jobs, ws, lr);
+}
+
+// Joins the parts of split tiles (SIDE 32-blocks wide), one 32 x 32 block of a tile each wave (blk0 counts tiles).
+template <int SIDE>
 __global__ void __launch_bounds__(64)
 k_mu_join(mu_table tab, char* ws) {
-  constexpr int BT = 64 * TW, SUB = 4 * TW * TW;
+  constexpr int BT = 32 * SIDE, SUB = SIDE * SIDE, TW = SIDE == 4 ? 2 : 1;
   __shared__ __attribute__((aligned(16))) uint32_t turn[32 * MU_PITCH];
   const int lane = threadIdx.x, tile = blockIdx.x / SUB, sub = blockIdx.x % SUB;
   const int gi = mu_find(tab, tile);
@@ -527,7 +677,7 @@ k_mu_join(mu_table tab, char* ws) {
       v[4 * q + 3] += f.w;
     }
   const int wave = sub / (TW * TW), a = sub / TW % TW, b = sub % TW;
-  const int rb = ti * 2 * TW + (wave >> 1) * TW + a, cb = tj * 2 * TW + (wave & 1) * TW + b;
+  const int rb = ti * SIDE + (wave >> 1) * TW + a, cb = tj * SIDE + (wave & 1) * TW + b;
   mu_store_symmetric(g, ws, job, v, rb, cb, ti != tj, lane, turn);
 }
 
@@ -570,14 +720,42 @@ static mu_cut mu_cut_of(int64_t tiles, int stages, int64_t all_stages, int64_t a
   return c;
 }
 
+// Tiles (of 128 x 128 and 64 x 64) of the m x m products and of those with X, and what sides (of 32) they have.
+struct mu_counts {
+  int64_t tiles = 0, xtiles = 0, xstages = 0, tiles64 = 0, xtiles64 = 0;
+  void add(int64_t pm, int64_t pn, int64_t count) {
+    const int64_t t = count * (pm / 128) * (pm / 128 + 1) / 2;
+    tiles += t;
+    xtiles += count * (pm / 128) * (pn / 128);
+    xstages += t * (pn / 32);
+    tiles64 += count * (pm / 64) * (pm / 64 + 1) / 2;
+    xtiles64 += count * (pm / 64) * (pn / 64);
+  }
+  // 64 x 64 while tiles of 128 x 128 would leave places free
+  int square() const { return tiles64 <= MU_SMALL ? 1 : tiles < 256 ? 2 : 4; }
+  int apply() const { return xtiles64 <= MU_SMALL_X ? 1 : xtiles < 128 ? 2 : 4; }
+  int gram() const { return tiles64 <= MU_SMALL ? 1 : xstages < 4096 ? 2 : 4; }
+  bool large() const { return square() == 4 || apply() == 4 || gram() == 4; }
+};
+
 static void mu_make_plan(const lmh_muon_job* jobs, int count, mu_plan* pl) {
   pl->order.resize(count);
   for (int i = 0; i < count; ++i) pl->order[i] = i;
-  auto key = [&](int i) { return std::make_pair(jobs[i].rows, jobs[i].cols); };
-  std::stable_sort(pl->order.begin(), pl->order.end(), [&](int a, int b) { return key(a) < key(b); });
+  // by shape, those of the longest products first: a launch's last blocks are short ones
+  auto key = [&](int i) {
+    const int r = jobs[i].rows, c = jobs[i].cols;
+    return std::make_tuple(std::min(r, c), std::max(r, c), r);
+  };
+  std::stable_sort(pl->order.begin(), pl->order.end(), [&](int a, int b) { return key(a) > key(b); });
+  // rows and columns are padded to 128 where a tile of 128 x 128 may be taken (mu_counts), to 64 where none is
+  mu_counts all;
   pl->tw = 1;
-  for (int i = 0; i < count; ++i)
-    if (std::min(jobs[i].rows, jobs[i].cols) > 64) pl->tw = 2;
+  for (int i = 0; i < count; ++i) {
+    const int m = std::min(jobs[i].rows, jobs[i].cols), n = std::max(jobs[i].rows, jobs[i].cols);
+    if (m > 64) pl->tw = 2;
+    all.add(mu_up(m, 128), mu_up(n, 128), 1);
+  }
+  if (!all.large()) pl->tw = 1;
   // one long matrix, and the others but for large ones go its way: the number of multiplications is the same for m = n, and two
   // kinds would take their launches one after the other
   bool all_long = false;
@@ -687,8 +865,8 @@ class mu_runner {
   struct product { int l, r, d0, d1, units; float s0, g0, s1, g1; };
   // Symmetric m x m products of the groups (`make` gives 0, 1 or 2 of a group), tiles of 64 tw.
   template <typename F>
-  void symmetric(const std::vector<const mu_group*>& gs, int tw, F make) {
-    const int bt = 64 * tw;
+  void symmetric(const std::vector<const mu_group*>& gs, int side, F make) {
+    const int bt = 32 * side;
     std::vector<std::pair<const mu_group*, product>> all;
     for (const mu_group* g : gs) {
       product p[2];
@@ -724,7 +902,7 @@ class mu_runner {
         t.g1 = p.g1;
         t.aux = p.units;
         const int64_t tm = g.pm / bt, n = tm * (tm + 1) / 2 * g.count;
-        mu_cut c = mu_cut_of(n, p.units / 2, stages, tiles, hi - lo == 1, tw == 1 ? 16 : 8);
+        mu_cut c = mu_cut_of(n, p.units / 2, stages, tiles, side > 1 && hi - lo == 1, side == 1 ? 32 : side == 2 ? 16 : 8);
         const int64_t need = (n - c.whole) * c.splits * bt * bt * 4 / 256;
         if (slab + need > pl_.slab + pl_.slab_units) c = {n, 1};
         t.whole = (int)c.whole;
@@ -740,26 +918,29 @@ class mu_runner {
         }
       }
       // few blocks: one to a compute unit, with more stages on their way
-      if (tw == 1) lmh_launch((k_mu_gemm<1, 2, 4, MU_SYM>), dim3(blocks), dim3(256), 0, st_, tab_, ws_);
+      if (side == 1) lmh_launch((k_mu_small<MU_SYM>), dim3(blocks), dim3(256), 0, st_, tab_, ws_);
+      else if (side == 2) lmh_launch((k_mu_gemm<1, 2, 4, MU_SYM>), dim3(blocks), dim3(256), 0, st_, tab_, ws_);
       else if (blocks <= MU_SLOTS / 2) lmh_launch((k_mu_gemm<2, 2, 4, MU_SYM>), dim3(blocks), dim3(256), 0, st_, tab_, ws_);
       else lmh_launch((k_mu_gemm<2, 2, 2, MU_SYM>), dim3(blocks), dim3(256), 0, st_, tab_, ws_);
       if (joins) {
-        if (tw == 1) lmh_launch((k_mu_join<1>), dim3(joins * 4), dim3(64), 0, st_, join, ws_);
-        else lmh_launch((k_mu_join<2>), dim3(joins * 16), dim3(64), 0, st_, join, ws_);
+        if (side == 1) lmh_launch((k_mu_join<1>), dim3(joins), dim3(64), 0, st_, join, ws_);
+        else if (side == 2) lmh_launch((k_mu_join<2>), dim3(joins * 4), dim3(64), 0, st_, join, ws_);
+        else lmh_launch((k_mu_join<4>), dim3(joins * 16), dim3(64), 0, st_, join, ws_);
       }
     }
   }
   // X <- polynomial X
   template <typename F>
-  void apply(const std::vector<const mu_group*>& gs, int tw, F operands) {
-    const int bt = 64 * tw;
+  void apply(const std::vector<const mu_group*>& gs, int side, F operands) {
+    const int bt = 32 * side;
     for (size_t lo = 0; lo < gs.size(); lo += MU_MAX_GROUPS) {
       const int nb = tasks(gs, lo, std::min(gs.size(), lo + MU_MAX_GROUPS), [&](const mu_group& g, mu_task* t) {
         operands(g, t);
         t->aux = g.pm / 16;
         return (g.pm / bt) * (g.pn / bt) * g.count;
       });
-      if (tw == 1) lmh_launch((k_mu_gemm<1, 2, 4, MU_APPLY>), dim3(nb), dim3(256), 0, st_, tab_, ws_);
+      if (side == 1) lmh_launch((k_mu_small<MU_APPLY>), dim3(nb), dim3(256), 0, st_, tab_, ws_);
+      else if (side == 2) lmh_launch((k_mu_gemm<1, 2, 4, MU_APPLY>), dim3(nb), dim3(256), 0, st_, tab_, ws_);
       else lmh_launch((k_mu_gemm<2, 2, 2, MU_APPLY>), dim3(nb), dim3(256), 0, st_, tab_, ws_);
     }
   }
@@ -832,21 +1013,15 @@ static void mu_run(const lmh_muon_job* jobs, const mu_plan& pl, int steps, float
   for (int kind = 0; kind < 2; ++kind) {
     const std::vector<const mu_group*>& G = gs[kind];
     if (G.empty()) continue;
-    // m x m products: 64 x 64 tiles while those of 128 x 128 would leave places free
-    int64_t tiles = 0, xtiles = 0, xstages = 0;
-    for (const mu_group* g : G) {
-      const int64_t t = (int64_t)g->count * (g->pm / 128) * (g->pm / 128 + 1) / 2;
-      tiles += t;
-      xtiles += (int64_t)g->count * (g->pm / 128) * (g->pn / 128);
-      xstages += t * (g->pn / 32);
-    }
-    const int tw = pl.tw == 2 && tiles >= 256 ? 2 : 1;
-    const int tw_apply = pl.tw == 2 && xtiles >= 128 ? 2 : 1, tw_gram = pl.tw == 2 && xstages >= 4096 ? 2 : 1;
+    mu_counts counts;
+    for (const mu_group* g : G) counts.add(g->pm, g->pn, g->count);
+    const int most = 2 * pl.tw;
+    const int side = std::min(most, counts.square()), side_x = std::min(most, counts.apply()), side_gram = std::min(most, counts.gram());
     int flip = 0;
     for (int done = 0; done < steps;) {
       const int left = steps - done, len = kind == 0 ? 1 : left == 4 ? 2 : std::min(left, 3);
       // A = X X' and b I + c A
-      run.symmetric(G, tw_gram, [](const mu_group& g, mu_runner::product* p) {
+      run.symmetric(G, side_gram, [](const mu_group& g, mu_runner::product* p) {
         const float s = 1.f / (MU_SX * MU_SX);
         p[0] = {g.x, g.x, g.a, g.c, g.pn / 16, MU_SG * s, 0.f, MU_C * MU_SC * s, MU_B * MU_SC};
         return 1;
@@ -854,14 +1029,14 @@ static void mu_run(const lmh_muon_job* jobs, const mu_plan& pl, int steps, float
       int q = 0;                       // of a run of several steps: their product so far in q[q]
       for (int k = 0; k < len; ++k) {
         // p = (b I + c A) A + a I; the first of several is their product too
-        run.symmetric(G, tw, [&](const mu_group& g, mu_runner::product* p) {
+        run.symmetric(G, side, [&](const mu_group& g, mu_runner::product* p) {
           const float s = 1.f / (MU_SC * MU_SG);
           p[0] = {g.c, g.a, g.p, k == 0 && len > 1 ? g.q[0] : -1, g.pm / 16, MU_SP * s, MU_A * MU_SP, MU_SQ * s, MU_A * MU_SQ};
           return 1;
         });
         if (len == 1) break;
         // z = p A unless this is the last of them, Q <- p Q unless it is the first
-        run.symmetric(G, tw, [&](const mu_group& g, mu_runner::product* p) {
+        run.symmetric(G, side, [&](const mu_group& g, mu_runner::product* p) {
           int n = 0;
           if (k + 1 < len) p[n++] = {g.p, g.a, g.z, -1, g.pm / 16, MU_SG / (MU_SP * MU_SG), 0.f, 0.f, 0.f};
           if (k > 0) p[n++] = {g.p, g.q[q], g.q[1 - q], -1, g.pm / 16, MU_SQ / (MU_SP * MU_SQ), 0.f, 0.f, 0.f};
@@ -869,7 +1044,7 @@ static void mu_run(const lmh_muon_job* jobs, const mu_plan& pl, int steps, float
         });
         if (k > 0) q = 1 - q;
         if (k + 1 < len) {
-          run.symmetric(G, tw, [&](const mu_group& g, mu_runner::product* p) {      // A <- z p
+          run.symmetric(G, side, [&](const mu_group& g, mu_runner::product* p) {      // A <- z p
             const float s = 1.f / (MU_SG * MU_SP);
             p[0] = {g.z, g.p, g.a, g.c, g.pm / 16, MU_SG * s, 0.f, MU_C * MU_SC * s, MU_B * MU_SC};
             return 1;
@@ -885,16 +1060,17 @@ static void mu_run(const lmh_muon_job* jobs, const mu_plan& pl, int steps, float
         t->s0 = len > 1 ? 1.f / MU_SQ : 1.f / MU_SP;
       };
       if (done < steps) {
-        run.apply(G, tw_apply, operands);
+        run.apply(G, side_x, operands);
         flip = 1 - flip;
       } else {
         run.with_jobs(jobs, G, [&](const mu_group& g, mu_task* t) {
           operands(g, t);
           t->s0 /= MU_SX;
           t->aux = g.pm / 16;
-          return (g.pm / (64 * tw_apply)) * (g.pn / (64 * tw_apply));
+          return (g.pm / (32 * side_x)) * (g.pn / (32 * side_x));
         }, [&](dim3 nb, const mu_table& tab, const mu_jobs& pj) {
-          if (tw_apply == 1) lmh_launch((k_mu_last<T, 1, 2, 4, OPT>), nb, dim3(256), 0, st, tab, pj, ws, lr);
+          if (side_x == 1) lmh_launch((k_mu_small_last<T, OPT>), nb, dim3(256), 0, st, tab, pj, ws, lr);
+          else if (side_x == 2) lmh_launch((k_mu_last<T, 1, 2, 4, OPT>), nb, dim3(256), 0, st, tab, pj, ws, lr);
           else lmh_launch((k_mu_last<T, 2, 2, 2, OPT>), nb, dim3(256), 0, st, tab, pj, ws, lr);
         });
       }
