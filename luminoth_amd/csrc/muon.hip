@@ -48,6 +48,9 @@
 // the 42 matrices of a ResNet-50 detector, 328 tiles, 13.3 us a launch both)
 #define MU_SMALL 160
 #define MU_SMALL_X 256        // ... of the products with X
+// Two tiles of 128 x 128 in one of 256 x 128: a unit of 16 k then takes 12 KB of LDS reads and 6 KB of writes a wave for 24 matrix
+// instructions instead of 8 + 4 for 12 - with those LDS has as many cycles of work as the matrix cores - (4096 x 4096: 373 -> 350 us a
+// product = 1180 TFLOP/s of f16 instructions).  Where rounds of blocks cost more than that gains, 128 x 128 stays.
 #define MU_NORM_BLOCKS 256
 #define MU_NORM_ELEMS 2048    // at least this many per block of k_mu_norm
 
@@ -292,11 +295,13 @@ __device__ __forceinline__ void mu_triangle(int t, int tm, int* ti, int* tj) {
   }
 }
 
-// The accumulator of 32-blocks (rb, cb) of a symmetric result, scaled into its one or two buffers, and mirrored unless the
-// whole tile lies on the diagonal.
-__device__ __forceinline__ void mu_store_symmetric(const mu_task& g, char* ws, int job, const float* acc, int rb, int cb, bool mirror,
-                                                   int lane, uint32_t* turn, int only = -1) {
+// The accumulator of 32-blocks (rb, cb) of a symmetric result, scaled into its one or two buffers (`only`: one of them), and mirrored
+// unless its tile of SQ x SQ blocks lies on the diagonal (all of it is computed).
+template <int SQ>
+__device__ __forceinline__ void mu_store_symmetric(const mu_task& g, char* ws, int job, const float* acc, int rb, int cb, int lane,
+                                                   uint32_t* turn, int only = -1) {
   const int l31 = lane & 31, h = lane >> 5, units = g.pm / 16;
+  const bool mirror = rb / SQ != cb / SQ;
 #pragma unroll
   for (int k = 0; k < 2; ++k) {
     const int d = k ? g.d1 : g.d0;
@@ -312,14 +317,14 @@ __device__ __forceinline__ void mu_store_symmetric(const mu_task& g, char* ws, i
 
 enum { MU_SYM = 0, MU_APPLY = 1, MU_LAST = 2 };
 
-// One tile of (64 TW)^2 of C = L . R' (rows of L and R along k), 4 waves of (32 TW)^2; a ring of DEPTH stages of 16 KU k in LDS.
+// One tile of 64 TA x 64 TB of C = L . R' (rows of L and R along k), 4 waves of 32 TA x 32 TB; a ring of DEPTH stages of 16 KU k in LDS.
 //  MU_SYM: m x m, tiles of the upper triangle; kinds of operands by r: k runs over aux 16-units.
 //  MU_APPLY: l = X' (n x m), r = a polynomial (m x m) -> d0 = X (rows m), d1 = X' (rows n).
 //  MU_LAST: the same product into the result (a wide matrix the other way round: lanes then run along stored rows).
-template <typename T, int TW, int KU, int DEPTH, int MODE, bool OPT>
+template <typename T, int TA, int TB, int KU, int DEPTH, int MODE, bool OPT>
 __device__ __forceinline__ void mu_gemm_tile(const mu_table& tab, const mu_jobs* jobs, char* ws, float lr) {
-  constexpr int BT = 64 * TW, RB = 2 * TW, SU = KU * 2048, STAGE = RB * SU, NL = TW * KU;      // bytes of one operand's stage, its loads by a wave
-  __shared__ __attribute__((aligned(16))) char smem[2 * DEPTH * STAGE];
+  constexpr int RBA = 2 * TA, RBB = 2 * TB, SU = KU * 2048, STAGE = (RBA + RBB) * SU, NL = (TA + TB) * KU;     // bytes of a stage, a wave's loads
+  __shared__ __attribute__((aligned(16))) char smem[DEPTH * STAGE];
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, wr = wave >> 1, wc = wave & 1, l31 = lane & 31, h = lane >> 5;
   // every eighth block runs on the same die: of 64 blocks, those of a die take eight tiles behind each other, which share operands
   // in its L2
@@ -328,7 +333,9 @@ __device__ __forceinline__ void mu_gemm_tile(const mu_table& tab, const mu_jobs*
   const int gi = mu_find(tab, blk);
   const mu_task& g = tab.t[gi];
   int u = blk - tab.blk0[gi], split = 0, ti, tj, job;
-  const int tm = g.pm / BT, tn = g.pn / BT, per = MODE == MU_SYM ? tm * (tm + 1) / 2 : tm * tn;
+  const bool turned = MODE == MU_LAST && !g.tall;
+  const int rows32 = MODE == MU_SYM || turned ? g.pm / 32 : g.pn / 32, cols32 = turned ? g.pn / 32 : g.pm / 32;      // of the result
+  const int tm = (rows32 + RBA - 1) / RBA, tn = cols32 / RBB, per = MODE == MU_SYM ? tm * (tm + 1) / 2 : tm * tn;
   int t;
   if (MODE == MU_SYM && g.whole == 0) {      // all tiles split: a matrix's tiles of one part of k are neighbours
     const unsigned both = (unsigned)per * g.splits, in = (unsigned)u % both;
@@ -345,12 +352,13 @@ __device__ __forceinline__ void mu_gemm_tile(const mu_table& tab, const mu_jobs*
     job = (unsigned)u / (unsigned)per;
     t = u - job * per;
   }
-  const bool turned = MODE == MU_LAST && !g.tall;
   if (MODE == MU_SYM) {
     mu_triangle(t, tm, &ti, &tj);
   } else {
-    // (row, column) among tn x tm tiles: in strips of eight rows, a strip column by column; few columns: row by row
-    const int step = tm > 8 ? 8 : 1, strip = t / (step * tm), in = t - strip * step * tm, high = min(step, tn - strip * step);
+    // among the tiles along n and those along m: in strips of eight of the former, a strip one by one of the latter; few of those:
+    // the other way round
+    const int ta = turned ? tn : tm, tb = turned ? tm : tn;
+    const int step = tb > 8 ? 8 : 1, strip = t / (step * tb), in = t - strip * step * tb, high = min(step, ta - strip * step);
     const int row = strip * step + in % high, col = in / high;
     ti = turned ? col : row;
     tj = turned ? row : col;
@@ -365,28 +373,29 @@ __device__ __forceinline__ void mu_gemm_tile(const mu_table& tab, const mu_jobs*
     k0 = (int)(all * split / parts);
     stages = (int)(all * (split + 1) / parts) - k0;
   }
-  f32x16 acc[TW][TW];
+  f32x16 acc[TA][TB];
 #pragma unroll
-  for (int a = 0; a < TW; ++a)
+  for (int a = 0; a < TA; ++a)
 #pragma unroll
-    for (int b = 0; b < TW; ++b)
+    for (int b = 0; b < TB; ++b)
 #pragma unroll
       for (int i = 0; i < 16; ++i) acc[a][b][i] = 0.f;
 
   typedef __attribute__((address_space(3))) void* lds_ptr;
   typedef const __attribute__((address_space(1))) void* glb_ptr;
-  // a stage: RB row blocks x KU units x 2 KB of each operand; wave w brings in KBs w, w + 4, ...
-  const char* gl = L + (int64_t)ti * RB * kunits * 2048 + (int64_t)k0 * SU + lane * 16;
-  const char* gr = R + (int64_t)tj * RB * kunits * 2048 + (int64_t)k0 * SU + lane * 16;
-  auto issue = [&](int s, int b) {
-    char* dst = smem + b * 2 * STAGE;
+  // a stage: RBA row blocks of the left operand and RBB of the right one x KU units x 2 KB; wave w brings in KBs w, w + 4, ...  (Rows
+  // behind the last: that one again; their products are dropped.)
+  const char* src[NL];
 #pragma unroll
-    for (int i = 0; i < NL; ++i) {
-      const int piece = i * 4 + wave;
-      const int64_t at = (int64_t)(piece / (2 * KU)) * kunits * 2048 + (int64_t)s * SU + piece % (2 * KU) * 1024;
-      __builtin_amdgcn_global_load_lds((glb_ptr)(gl + at), (lds_ptr)(dst + piece * 1024), 16, 0, 0);
-      __builtin_amdgcn_global_load_lds((glb_ptr)(gr + at), (lds_ptr)(dst + STAGE + piece * 1024), 16, 0, 0);
-    }
+  for (int i = 0; i < NL; ++i) {
+    const int piece = i * 4 + wave, rb = piece / (2 * KU);
+    const int64_t row = rb < RBA ? min(ti * RBA + rb, rows32 - 1) : tj * RBB + rb - RBA;
+    src[i] = (rb < RBA ? L : R) + row * kunits * 2048 + (int64_t)k0 * SU + piece % (2 * KU) * 1024 + lane * 16;
+  }
+  auto issue = [&](int s, int b) {
+#pragma unroll
+    for (int i = 0; i < NL; ++i)
+      __builtin_amdgcn_global_load_lds((glb_ptr)(src[i] + (int64_t)s * SU), (lds_ptr)(smem + b * STAGE + (i * 4 + wave) * 1024), 16, 0, 0);
   };
 #pragma unroll
   for (int s = 0; s < DEPTH - 1; ++s)
@@ -395,48 +404,49 @@ __device__ __forceinline__ void mu_gemm_tile(const mu_table& tab, const mu_jobs*
   for (int s = 0; s < stages; ++s) {
     // this wave's pieces of stage s have landed (DEPTH - 2 later stages may still be on their way); behind the barrier
     // everybody's have, and everybody is done with the stage whose place the next issue takes
-    if (DEPTH > 2 && stages - 1 - s >= DEPTH - 2) asm volatile("s_waitcnt vmcnt(%0)" ::"n"((DEPTH - 2) * 2 * NL) : "memory");
+    if (DEPTH > 2 && stages - 1 - s >= DEPTH - 2) asm volatile("s_waitcnt vmcnt(%0)" ::"n"((DEPTH - 2) * NL) : "memory");
     else asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
     asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
     if (s + DEPTH - 1 < stages) issue(s + DEPTH - 1, cur == 0 ? DEPTH - 1 : cur - 1);
-    const char* Ls = smem + cur * 2 * STAGE + wr * TW * SU + lane * 16;
-    const char* Rs = smem + cur * 2 * STAGE + STAGE + wc * TW * SU + lane * 16;
+    const char* Ls = smem + cur * STAGE + wr * TA * SU + lane * 16;
+    const char* Rs = smem + cur * STAGE + RBA * SU + wc * TB * SU + lane * 16;
 #pragma unroll
     for (int k = 0; k < KU; ++k) {
-      f16x8 lh[TW], ll[TW], rh[TW], rl[TW];
+      f16x8 lh[TA], ll[TA], rh[TB], rl[TB];
 #pragma unroll
-      for (int a = 0; a < TW; ++a) {
-        lh[a] = *reinterpret_cast<const f16x8*>(Ls + a * SU + k * 2048);
-        rl[a] = *reinterpret_cast<const f16x8*>(Rs + a * SU + k * 2048 + 1024);
-        ll[a] = *reinterpret_cast<const f16x8*>(Ls + a * SU + k * 2048 + 1024);
-        rh[a] = *reinterpret_cast<const f16x8*>(Rs + a * SU + k * 2048);
-      }
+      for (int a = 0; a < TA; ++a) lh[a] = *reinterpret_cast<const f16x8*>(Ls + a * SU + k * 2048);
 #pragma unroll
-      for (int a = 0; a < TW; ++a)
+      for (int b = 0; b < TB; ++b) rl[b] = *reinterpret_cast<const f16x8*>(Rs + b * SU + k * 2048 + 1024);
 #pragma unroll
-        for (int b = 0; b < TW; ++b) acc[a][b] = __builtin_amdgcn_mfma_f32_32x32x16_f16(lh[a], rl[b], acc[a][b], 0, 0, 0);
+      for (int a = 0; a < TA; ++a) ll[a] = *reinterpret_cast<const f16x8*>(Ls + a * SU + k * 2048 + 1024);
 #pragma unroll
-      for (int a = 0; a < TW; ++a)
+      for (int b = 0; b < TB; ++b) rh[b] = *reinterpret_cast<const f16x8*>(Rs + b * SU + k * 2048);
 #pragma unroll
-        for (int b = 0; b < TW; ++b) acc[a][b] = __builtin_amdgcn_mfma_f32_32x32x16_f16(ll[a], rh[b], acc[a][b], 0, 0, 0);
+      for (int a = 0; a < TA; ++a)
 #pragma unroll
-      for (int a = 0; a < TW; ++a)
+        for (int b = 0; b < TB; ++b) acc[a][b] = __builtin_amdgcn_mfma_f32_32x32x16_f16(lh[a], rl[b], acc[a][b], 0, 0, 0);
 #pragma unroll
-        for (int b = 0; b < TW; ++b) acc[a][b] = __builtin_amdgcn_mfma_f32_32x32x16_f16(lh[a], rh[b], acc[a][b], 0, 0, 0);
+      for (int a = 0; a < TA; ++a)
+#pragma unroll
+        for (int b = 0; b < TB; ++b) acc[a][b] = __builtin_amdgcn_mfma_f32_32x32x16_f16(ll[a], rh[b], acc[a][b], 0, 0, 0);
+#pragma unroll
+      for (int a = 0; a < TA; ++a)
+#pragma unroll
+        for (int b = 0; b < TB; ++b) acc[a][b] = __builtin_amdgcn_mfma_f32_32x32x16_f16(lh[a], rh[b], acc[a][b], 0, 0, 0);
     }
     cur = cur + 1 == DEPTH ? 0 : cur + 1;
   }
 
   if constexpr (MODE == MU_SYM) {
     if (part) {
-      float* s = (float*)(ws + (int64_t)g.slab * 256) + ((int64_t)(u - g.whole) * g.splits + split) * BT * BT;
+      float* s = (float*)(ws + (int64_t)g.slab * 256) + ((int64_t)(u - g.whole) * g.splits + split) * (RBA * RBB * 1024);
 #pragma unroll
-      for (int a = 0; a < TW; ++a)
+      for (int a = 0; a < TA; ++a)
 #pragma unroll
-        for (int b = 0; b < TW; ++b)
+        for (int b = 0; b < TB; ++b)
 #pragma unroll
           for (int q = 0; q < 4; ++q)
-            *reinterpret_cast<float4*>(s + ((wave * TW + a) * TW + b) * 1024 + q * 256 + lane * 4) =
+            *reinterpret_cast<float4*>(s + ((wave * TA + a) * TB + b) * 1024 + q * 256 + lane * 4) =
                 make_float4(acc[a][b][4 * q], acc[a][b][4 * q + 1], acc[a][b][4 * q + 2], acc[a][b][4 * q + 3]);
       return;
     }
@@ -447,10 +457,10 @@ __device__ __forceinline__ void mu_gemm_tile(const mu_table& tab, const mu_jobs*
     const int rows = g.tall ? g.n : g.m, cols = g.tall ? g.m : g.n;
     const float scale = OPT ? lr * p.scale * g.s0 : g.s0;
 #pragma unroll
-    for (int a = 0; a < TW; ++a)
+    for (int a = 0; a < TA; ++a)
 #pragma unroll
-      for (int b = 0; b < TW; ++b) {
-        const int c = tj * BT + (wc * TW + b) * 32 + l31, r0 = ti * BT + (wr * TW + a) * 32 + 4 * h;
+      for (int b = 0; b < TB; ++b) {
+        const int c = (tj * RBB + wc * TB + b) * 32 + l31, r0 = (ti * RBA + wr * TA + a) * 32 + 4 * h;
         if constexpr (OPT) {                 // sixteen loads on their way, then the stores
           float w[16];
           int64_t at[16];
@@ -476,10 +486,11 @@ __device__ __forceinline__ void mu_gemm_tile(const mu_table& tab, const mu_jobs*
   __syncthreads();                           // the stages' LDS is free
   uint32_t* turn = (uint32_t*)smem + wave * 32 * MU_PITCH;
 #pragma unroll
-  for (int a = 0; a < TW; ++a)
+  for (int a = 0; a < TA; ++a)
 #pragma unroll
-    for (int b = 0; b < TW; ++b) {
-      const int rb = ti * RB + wr * TW + a, cb = tj * RB + wc * TW + b;      // 32-blocks of the result
+    for (int b = 0; b < TB; ++b) {
+      const int rb = ti * RBA + wr * TA + a, cb = tj * RBB + wc * TB + b;    // 32-blocks of the result
+      if (rb >= rows32) continue;
       float v[16];
       if constexpr (MODE == MU_APPLY) {      // rows of the result: n, columns: m
 #pragma unroll
@@ -489,20 +500,20 @@ __device__ __forceinline__ void mu_gemm_tile(const mu_table& tab, const mu_jobs*
       } else {
 #pragma unroll
         for (int i = 0; i < 16; ++i) v[i] = acc[a][b][i];
-        mu_store_symmetric(g, ws, job, v, rb, cb, ti != tj, lane, turn);
+        mu_store_symmetric<RBB>(g, ws, job, v, rb, cb, lane, turn);
       }
     }
 }
 
-template <int TW, int KU, int DEPTH, int MODE>
-__global__ void __launch_bounds__(256)
+template <int TA, int TB, int KU, int DEPTH, int MODE>
+__global__ void __launch_bounds__(256, 2)
 k_mu_gemm(mu_table tab, char* ws) {
-  mu_gemm_tile<f32_t, TW, KU, DEPTH, MODE, false>(tab, nullptr, ws, 0.f);
+  mu_gemm_tile<f32_t, TA, TB, KU, DEPTH, MODE, false>(tab, nullptr, ws, 0.f);
 }
-template <typename T, int TW, int KU, int DEPTH, bool OPT>
-__global__ void __launch_bounds__(256)
+template <typename T, int TA, int TB, int KU, int DEPTH, bool OPT>
+__global__ void __launch_bounds__(256, 2)
 k_mu_last(mu_table tab, mu_jobs jobs, char* ws, float lr) {
-  mu_gemm_tile<T, TW, KU, DEPTH, MU_LAST, OPT>(tab, &jobs, ws, lr);
+  mu_gemm_tile<T, TA, TB, KU, DEPTH, MU_LAST, OPT>(tab, &jobs, ws, lr);
 }
 
 // Few tiles: one of 32 x 32 by four waves, a quarter of k each.  What bounds such a launch is how fast a compute unit gets its operands
@@ -614,7 +625,7 @@ __device__ __forceinline__ void mu_small_tile(const mu_table& tab, const mu_jobs
       for (int q = 0; q < 4; ++q) *reinterpret_cast<float4*>(s + q * 256 + lane * 4) = make_float4(v[4 * q], v[4 * q + 1], v[4 * q + 2], v[4 * q + 3]);
       return;
     }
-    mu_store_symmetric(g, ws, job, v, ti, tj, ti != tj, lane, turn, wave);
+    mu_store_symmetric<1>(g, ws, job, v, ti, tj, lane, turn, wave);
   } else if constexpr (MODE == MU_APPLY) {
     if (wave) return;
 #pragma unroll
@@ -649,25 +660,26 @@ k_mu_small_last(mu_table tab, mu_jobs jobs, char* ws, float lr) {
   mu_small_tile<T, MU_LAST, OPT>(tab, &jobs, ws, lr);
 }
 
-// Joins the parts of split tiles (SIDE 32-blocks wide), one 32 x 32 block of a tile each wave (blk0 counts tiles).
-template <int SIDE>
+// Joins the parts of split tiles (WAVES: four with TW x TW 32-blocks each, or one), one 32 x 32 block of a tile each wave (blk0 counts
+// tiles).
+template <int TW, int WAVES>
 __global__ void __launch_bounds__(64)
 k_mu_join(mu_table tab, char* ws) {
-  constexpr int BT = 32 * SIDE, SUB = SIDE * SIDE, TW = SIDE == 4 ? 2 : 1;
+  constexpr int W = WAVES == 4 ? 2 : 1, RB = W * TW, SUB = RB * RB;
   __shared__ __attribute__((aligned(16))) uint32_t turn[32 * MU_PITCH];
   const int lane = threadIdx.x, tile = blockIdx.x / SUB, sub = blockIdx.x % SUB;
   const int gi = mu_find(tab, tile);
   const mu_task& g = tab.t[gi];
   const int q0 = tile - tab.blk0[gi], u = g.whole + q0;
-  const int tm = g.pm / BT, per = tm * (tm + 1) / 2, job = u / per;
+  const int tm = g.pm / 32 / RB, per = tm * (tm + 1) / 2, job = u / per;
   int ti, tj;
   mu_triangle(u - job * per, tm, &ti, &tj);
-  const float* s = (const float*)(ws + (int64_t)g.slab * 256) + (int64_t)q0 * g.splits * BT * BT + sub * 1024 + lane * 4;
+  const float* s = (const float*)(ws + (int64_t)g.slab * 256) + (int64_t)q0 * g.splits * (SUB * 1024) + sub * 1024 + lane * 4;
   float v[16];
 #pragma unroll
   for (int i = 0; i < 16; ++i) v[i] = 0.f;
 #pragma unroll 4
-  for (int k = 0; k < g.splits; ++k, s += BT * BT)
+  for (int k = 0; k < g.splits; ++k, s += SUB * 1024)
 #pragma unroll
     for (int q = 0; q < 4; ++q) {
       const float4 f = *reinterpret_cast<const float4*>(s + q * 256);
@@ -677,12 +689,11 @@ k_mu_join(mu_table tab, char* ws) {
       v[4 * q + 3] += f.w;
     }
   const int wave = sub / (TW * TW), a = sub / TW % TW, b = sub % TW;
-  const int rb = ti * SIDE + (wave >> 1) * TW + a, cb = tj * SIDE + (wave & 1) * TW + b;
-  mu_store_symmetric(g, ws, job, v, rb, cb, ti != tj, lane, turn);
+  mu_store_symmetric<RB>(g, ws, job, v, ti * RB + wave / W * TW + a, tj * RB + wave % W * TW + b, lane, turn);
 }
 
 // ------------------------------------------------------------------------------------------------------- host ----
-#define MU_SLOTS 512      // blocks of 128 x 128 tiles (64 KB of LDS) the chip holds at a time
+#define MU_SLOTS 512      // blocks of 128 x 128 or 256 x 128 tiles (64 and 72 KB of LDS) the chip holds at a time
 
 static int64_t mu_up(int64_t v, int64_t a) { return (v + a - 1) / a * a; }
 
@@ -722,20 +733,26 @@ static mu_cut mu_cut_of(int64_t tiles, int stages, int64_t all_stages, int64_t a
 
 // Tiles (of 128 x 128 and 64 x 64) of the m x m products and of those with X, and what sides (of 32) they have.
 struct mu_counts {
-  int64_t tiles = 0, xtiles = 0, xstages = 0, tiles64 = 0, xtiles64 = 0;
+  int64_t tiles = 0, xtiles = 0, xtall = 0, xstages = 0, tiles64 = 0, xtiles64 = 0;
   void add(int64_t pm, int64_t pn, int64_t count) {
     const int64_t t = count * (pm / 128) * (pm / 128 + 1) / 2;
     tiles += t;
     xtiles += count * (pm / 128) * (pn / 128);
+    xtall += count * (pm / 128) * ((pn / 128 + 1) / 2);
     xstages += t * (pn / 32);
     tiles64 += count * (pm / 64) * (pm / 64 + 1) / 2;
     xtiles64 += count * (pm / 64) * (pn / 64);
   }
   // 64 x 64 while tiles of 128 x 128 would leave places free
   int square() const { return tiles64 <= MU_SMALL ? 1 : tiles < 256 ? 2 : 4; }
-  int apply() const { return xtiles64 <= MU_SMALL_X ? 1 : xtiles < 128 ? 2 : 4; }
+  int apply() const {
+    if (xtiles64 <= MU_SMALL_X) return 1;
+    if (xtiles < 128) return 2;
+    const int64_t rounds = (xtiles + MU_SLOTS - 1) / MU_SLOTS, tall = (xtall + MU_SLOTS - 1) / MU_SLOTS;
+    return 188 * tall < 100 * rounds ? 8 : 4;
+  }
   int gram() const { return tiles64 <= MU_SMALL ? 1 : xstages < 4096 ? 2 : 4; }
-  bool large() const { return square() == 4 || apply() == 4 || gram() == 4; }
+  bool large() const { return square() >= 4 || apply() >= 4 || gram() >= 4; }
 };
 
 static void mu_make_plan(const lmh_muon_job* jobs, int count, mu_plan* pl) {
@@ -821,6 +838,14 @@ extern "C" size_t lmh_muon_workspace_bytes(const lmh_muon_job* jobs, int count) 
   } catch (...) {
     return 0;
   }
+}
+
+// Tiles of one product with X: `side` 32-blocks each way; 8: eight along the result's rows and four along its columns.  (The last product's
+// rows are those of the matrix as it is stored.)
+static int mu_x_tiles(const mu_group& g, int side, bool last) {
+  if (side < 8) return g.pm / (32 * side) * (g.pn / (32 * side));
+  const int rows = last && !g.tall ? g.pm : g.pn, cols = last && !g.tall ? g.pn : g.pm;
+  return (rows + 255) / 256 * (cols / 128);
 }
 
 class mu_runner {
@@ -919,29 +944,29 @@ class mu_runner {
       }
       // few blocks: one to a compute unit, with more stages on their way
       if (side == 1) lmh_launch((k_mu_small<MU_SYM>), dim3(blocks), dim3(256), 0, st_, tab_, ws_);
-      else if (side == 2) lmh_launch((k_mu_gemm<1, 2, 4, MU_SYM>), dim3(blocks), dim3(256), 0, st_, tab_, ws_);
-      else if (blocks <= MU_SLOTS / 2) lmh_launch((k_mu_gemm<2, 2, 4, MU_SYM>), dim3(blocks), dim3(256), 0, st_, tab_, ws_);
-      else lmh_launch((k_mu_gemm<2, 2, 2, MU_SYM>), dim3(blocks), dim3(256), 0, st_, tab_, ws_);
+      else if (side == 2) lmh_launch((k_mu_gemm<1, 1, 2, 4, MU_SYM>), dim3(blocks), dim3(256), 0, st_, tab_, ws_);
+      else if (blocks <= MU_SLOTS / 2) lmh_launch((k_mu_gemm<2, 2, 2, 4, MU_SYM>), dim3(blocks), dim3(256), 0, st_, tab_, ws_);
+      else lmh_launch((k_mu_gemm<2, 2, 2, 2, MU_SYM>), dim3(blocks), dim3(256), 0, st_, tab_, ws_);
       if (joins) {
-        if (side == 1) lmh_launch((k_mu_join<1>), dim3(joins), dim3(64), 0, st_, join, ws_);
-        else if (side == 2) lmh_launch((k_mu_join<2>), dim3(joins * 4), dim3(64), 0, st_, join, ws_);
-        else lmh_launch((k_mu_join<4>), dim3(joins * 16), dim3(64), 0, st_, join, ws_);
+        if (side == 1) lmh_launch((k_mu_join<1, 1>), dim3(joins), dim3(64), 0, st_, join, ws_);
+        else if (side == 2) lmh_launch((k_mu_join<1, 4>), dim3(joins * 4), dim3(64), 0, st_, join, ws_);
+        else lmh_launch((k_mu_join<2, 4>), dim3(joins * 16), dim3(64), 0, st_, join, ws_);
       }
     }
   }
   // X <- polynomial X
   template <typename F>
   void apply(const std::vector<const mu_group*>& gs, int side, F operands) {
-    const int bt = 32 * side;
     for (size_t lo = 0; lo < gs.size(); lo += MU_MAX_GROUPS) {
       const int nb = tasks(gs, lo, std::min(gs.size(), lo + MU_MAX_GROUPS), [&](const mu_group& g, mu_task* t) {
         operands(g, t);
         t->aux = g.pm / 16;
-        return (g.pm / bt) * (g.pn / bt) * g.count;
+        return mu_x_tiles(g, side, false) * g.count;
       });
       if (side == 1) lmh_launch((k_mu_small<MU_APPLY>), dim3(nb), dim3(256), 0, st_, tab_, ws_);
-      else if (side == 2) lmh_launch((k_mu_gemm<1, 2, 4, MU_APPLY>), dim3(nb), dim3(256), 0, st_, tab_, ws_);
-      else lmh_launch((k_mu_gemm<2, 2, 2, MU_APPLY>), dim3(nb), dim3(256), 0, st_, tab_, ws_);
+      else if (side == 2) lmh_launch((k_mu_gemm<1, 1, 2, 4, MU_APPLY>), dim3(nb), dim3(256), 0, st_, tab_, ws_);
+      else if (side == 8) lmh_launch((k_mu_gemm<4, 2, 1, 3, MU_APPLY>), dim3(nb), dim3(256), 0, st_, tab_, ws_);
+      else lmh_launch((k_mu_gemm<2, 2, 2, 2, MU_APPLY>), dim3(nb), dim3(256), 0, st_, tab_, ws_);
     }
   }
   // Launches that take the caller's pointers: at most MU_MAX_JOBS matrices of MU_MAX_GROUPS shapes each.
@@ -1015,7 +1040,7 @@ static void mu_run(const lmh_muon_job* jobs, const mu_plan& pl, int steps, float
     if (G.empty()) continue;
     mu_counts counts;
     for (const mu_group* g : G) counts.add(g->pm, g->pn, g->count);
-    const int most = 2 * pl.tw;
+    const int most = pl.tw == 2 ? 8 : 2;
     const int side = std::min(most, counts.square()), side_x = std::min(most, counts.apply()), side_gram = std::min(most, counts.gram());
     int flip = 0;
     for (int done = 0; done < steps;) {
@@ -1067,11 +1092,12 @@ static void mu_run(const lmh_muon_job* jobs, const mu_plan& pl, int steps, float
           operands(g, t);
           t->s0 /= MU_SX;
           t->aux = g.pm / 16;
-          return (g.pm / (32 * side_x)) * (g.pn / (32 * side_x));
+          return mu_x_tiles(g, side_x, true);
         }, [&](dim3 nb, const mu_table& tab, const mu_jobs& pj) {
           if (side_x == 1) lmh_launch((k_mu_small_last<T, OPT>), nb, dim3(256), 0, st, tab, pj, ws, lr);
-          else if (side_x == 2) lmh_launch((k_mu_last<T, 1, 2, 4, OPT>), nb, dim3(256), 0, st, tab, pj, ws, lr);
-          else lmh_launch((k_mu_last<T, 2, 2, 2, OPT>), nb, dim3(256), 0, st, tab, pj, ws, lr);
+          else if (side_x == 2) lmh_launch((k_mu_last<T, 1, 1, 2, 4, OPT>), nb, dim3(256), 0, st, tab, pj, ws, lr);
+          else if (side_x == 8) lmh_launch((k_mu_last<T, 4, 2, 1, 3, OPT>), nb, dim3(256), 0, st, tab, pj, ws, lr);
+          else lmh_launch((k_mu_last<T, 2, 2, 2, 2, OPT>), nb, dim3(256), 0, st, tab, pj, ws, lr);
         });
       }
     }
