@@ -50,7 +50,8 @@
 #define MU_SMALL_X 256        // ... of the products with X
 // Two tiles of 128 x 128 in one of 256 x 128: a unit of 16 k then takes 12 KB of LDS reads and 6 KB of writes a wave for 24 matrix
 // instructions instead of 8 + 4 for 12 - with those LDS has as many cycles of work as the matrix cores - (4096 x 4096: 373 -> 350 us a
-// product = 1180 TFLOP/s of f16 instructions).  Where rounds of blocks cost more than that gains, 128 x 128 stays.
+// product = 1180 TFLOP/s of f16 instructions).  Where rounds of blocks cost more than that gains, or k is short and the rest of a
+// block's work counts (42 matrices of m = 128 to 512: 50 -> 53 us), 128 x 128 stays.
 #define MU_NORM_BLOCKS 256
 #define MU_NORM_ELEMS 2048    // at least this many per block of k_mu_norm
 
@@ -733,11 +734,12 @@ static mu_cut mu_cut_of(int64_t tiles, int stages, int64_t all_stages, int64_t a
 
 // Tiles (of 128 x 128 and 64 x 64) of the m x m products and of those with X, and what sides (of 32) they have.
 struct mu_counts {
-  int64_t tiles = 0, xtiles = 0, xtall = 0, xstages = 0, tiles64 = 0, xtiles64 = 0;
+  int64_t tiles = 0, xtiles = 0, xtall = 0, xdepth = 0, xstages = 0, tiles64 = 0, xtiles64 = 0;
   void add(int64_t pm, int64_t pn, int64_t count) {
     const int64_t t = count * (pm / 128) * (pm / 128 + 1) / 2;
     tiles += t;
     xtiles += count * (pm / 128) * (pn / 128);
+    xdepth += count * (pm / 128) * (pn / 128) * pm;
     xtall += count * (pm / 128) * ((pn / 128 + 1) / 2);
     xstages += t * (pn / 32);
     tiles64 += count * (pm / 64) * (pm / 64 + 1) / 2;
@@ -749,7 +751,7 @@ struct mu_counts {
     if (xtiles64 <= MU_SMALL_X) return 1;
     if (xtiles < 128) return 2;
     const int64_t rounds = (xtiles + MU_SLOTS - 1) / MU_SLOTS, tall = (xtall + MU_SLOTS - 1) / MU_SLOTS;
-    return 188 * tall < 100 * rounds ? 8 : 4;
+    return 188 * tall < 100 * rounds && xdepth >= 1024 * xtiles ? 8 : 4;
   }
   int gram() const { return tiles64 <= MU_SMALL ? 1 : xstages < 4096 ? 2 : 4; }
   bool large() const { return square() >= 4 || apply() >= 4 || gram() >= 4; }
