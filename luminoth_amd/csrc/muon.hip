@@ -28,6 +28,7 @@
 // along k; their parts are joined, in order, by a launch of their own.
 #include <algorithm>
 #include <tuple>
+#include <type_traits>
 #include <vector>
 
 #include "rowops.h"
@@ -52,7 +53,7 @@
 // instructions instead of 8 + 4 for 12 - with those LDS has as many cycles of work as the matrix cores - (4096 x 4096: 373 -> 350 us a
 // product = 1180 TFLOP/s of f16 instructions).  Where rounds of blocks cost more than that gains, or k is short and the rest of a
 // block's work counts (42 matrices of m = 128 to 512: 50 -> 53 us), 128 x 128 stays.
-#define MU_NORM_BLOCKS 256
+#define MU_NORM_BLOCKS 512
 #define MU_NORM_ELEMS 2048    // at least this many per block of k_mu_norm
 
 typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
@@ -147,10 +148,18 @@ k_mu_norm(mu_table tab, mu_jobs jobs, char* ws, float mu, int nesterov, float gs
   } else {
     constexpr int VEC = row_type<T>::VEC;
     const T* g = (const T*)p.g;
-    for (int64_t i = ((int64_t)b * 256 + threadIdx.x) * VEC; i < n; i += stride * VEC) {
-      const raw16 r = load_cols(g + i, 0, (int)(n - i < VEC ? n - i : VEC));
+    for (int64_t i = ((int64_t)b * 256 + threadIdx.x) * VEC; i < n; i += 4 * stride * VEC) {
+      raw16 r[4];                          // (four loads on their way)
 #pragma unroll
-      for (int e = 0; e < VEC; ++e) acc += (double)elem<T>(r, e) * (double)elem<T>(r, e);
+      for (int u = 0; u < 4; ++u) {
+        const int64_t at = i + u * stride * VEC;
+        r[u] = raw16{0, 0, 0, 0};
+        if (at < n) r[u] = load_cols(g + at, 0, (int)(n - at < VEC ? n - at : VEC));
+      }
+#pragma unroll
+      for (int u = 0; u < 4; ++u)
+#pragma unroll
+        for (int e = 0; e < VEC; ++e) acc += (double)elem<T>(r[u], e) * (double)elem<T>(r[u], e);
     }
   }
   for (int o = 32; o > 0; o >>= 1) acc += __shfl_xor(acc, o);
@@ -172,15 +181,12 @@ k_mu_planes(mu_table tab, mu_jobs jobs, char* ws, float eps) {
   const int local = blockIdx.x - tab.blk0[gi], per = (prow / 64) * (pcol / 64), job = local / per, t = local % per;
   const int r0 = (t / (pcol / 64)) * 64, c0 = (t % (pcol / 64)) * 64;
   const void* src = OPT ? (const void*)mu_at(ws, g, job, g.l) : jobs.p[g.first + job].g;
-  float x[16];
+  typedef typename std::conditional<OPT, f32_t, T>::type S;
+  S raw[16];                               // (sixteen loads on their way; behind the matrix: its last row and column, not used)
 #pragma unroll
   for (int i = 0; i < 16; ++i) {
-    const int r = i * 4 + (threadIdx.x >> 6), c = threadIdx.x & 63;
-    x[i] = 0.f;
-    if (r0 + r < rows && c0 + c < cols) {
-      const int64_t at = (int64_t)(r0 + r) * cols + c0 + c;
-      x[i] = OPT ? ((const float*)src)[at] : to_f32(((const T*)src)[at]);
-    }
+    const int r = min(r0 + i * 4 + (int)(threadIdx.x >> 6), rows - 1), c = min(c0 + (int)(threadIdx.x & 63), cols - 1);
+    raw[i] = ((const S*)src)[(int64_t)r * cols + c];
   }
   if (threadIdx.x < 64) {                  // the matrix's partial sums, in a fixed order
     const double* part = (const double*)mu_at(ws, g, job, g.norm);
@@ -194,7 +200,10 @@ k_mu_planes(mu_table tab, mu_jobs jobs, char* ws, float eps) {
   if (norm < (double)eps) norm = (double)eps;            // (not a number stays one)
   const double inv = (double)MU_SX / norm;               // (may lie outside fp32's range, X does not)
 #pragma unroll
-  for (int i = 0; i < 16; ++i) tile[i * 4 + (threadIdx.x >> 6)][threadIdx.x & 63] = (float)((double)x[i] * inv);
+  for (int i = 0; i < 16; ++i) {
+    const int r = i * 4 + (threadIdx.x >> 6), c = threadIdx.x & 63;
+    tile[r][c] = r0 + r < rows && c0 + c < cols ? (float)((double)to_f32(raw[i]) * inv) : 0.f;
+  }
   __syncthreads();
   // stored rows as rows (k = stored columns): X for a wide matrix, X' for a tall one; and the other way round
   char* by_row = mu_at(ws, g, job, g.tall ? g.d1 : g.d0);
