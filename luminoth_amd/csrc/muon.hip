@@ -28,7 +28,7 @@
 // along k; their parts are joined, in order, by a launch of their own.
 //
 // Measured (five steps): 4096 x 4096 fp32 3.95 ms, products with X 350 us = 1180 TFLOP/s of f16 instructions, symmetric ones 206 us = 1040;
-// 1024 x 320 bf16 117 us in 19 launches; the 42 matrices of a ResNet-50 detector, a whole optimizer step, 454 us in 22.
+// 1024 x 320 bf16 100 us in 19 launches; the 42 matrices of a ResNet-50 detector, a whole optimizer step, 454 us in 22.
 #include <algorithm>
 #include <tuple>
 #include <type_traits>
@@ -74,19 +74,23 @@ struct mu_task {
   float s0, g0, s1, g1;            // what is stored: accumulator * s + (on the diagonal) g
 };
 // blk0: the tasks' first blocks, behind each other: the arguments lie in host memory, where a search that goes from task to task
-// waits for every one of them (10 us of a 14 us launch)
-struct mu_table {
-  int32_t blk0[MU_MAX_GROUPS];     // (unused: the largest integer)
+// waits for every one of them (10 us of a 14 us launch).  One task alone has a table of its own, without a search
+// (0.8 us a launch: 1024 x 320 114 -> 100 us, 100 x 400 89 -> 73).
+template <int N> struct mu_table_of {
+  int32_t blk0[N];                 // (unused: the largest integer)
   int32_t tasks;
-  mu_task t[MU_MAX_GROUPS];
+  mu_task t[N];
 };
 struct mu_ptrs { const void* g; float* v; void* out; const float* factor; float wd, scale; };      // out: the weights, or the result
-struct mu_jobs { mu_ptrs p[MU_MAX_JOBS]; };
+template <int N> struct mu_jobs_of { mu_ptrs p[N]; };
+typedef mu_table_of<MU_MAX_GROUPS> mu_table;
+typedef mu_jobs_of<MU_MAX_JOBS> mu_jobs;
 
-__device__ __forceinline__ int mu_find(const mu_table& t, int blk) {
+template <int N> __device__ __forceinline__ int mu_find(const mu_table_of<N>& t, int blk) {
+  if (N == 1) return 0;
   int i = -1;
 #pragma unroll
-  for (int k = 0; k < MU_MAX_GROUPS; ++k) i += blk >= t.blk0[k];
+  for (int k = 0; k < N; ++k) i += blk >= t.blk0[k];
   return i;
 }
 __device__ __forceinline__ char* mu_at(char* ws, const mu_task& t, int job, int buffer) {
@@ -101,14 +105,14 @@ __device__ __forceinline__ void mu_split(float x, uint16_t* hi, uint16_t* lo) {
 
 // ---- momentum and the partial sums of the squares ----------------------------------------------------------
 // aux: blocks per matrix; d0: the matrix that is orthogonalised, row-major fp32 (the optimizer's; the plain call reads its input)
-template <typename T, bool OPT>
+template <typename T, bool OPT, int N>
 __global__ void __launch_bounds__(256)
-k_mu_norm(mu_table tab, mu_jobs jobs, char* ws, float mu, int nesterov, float gscale) {
+k_mu_norm(mu_table_of<N> tab, mu_jobs_of<(N == 1 ? 1 : MU_MAX_JOBS)> jobs, char* ws, float mu, int nesterov, float gscale) {
   __shared__ double red[4];
   const int ti = mu_find(tab, blockIdx.x);
   const mu_task& t = tab.t[ti];
-  const int local = blockIdx.x - tab.blk0[ti], job = local / t.aux, b = local % t.aux;
-  const mu_ptrs& p = jobs.p[t.first + job];
+  const int local = N == 1 ? blockIdx.x : blockIdx.x - tab.blk0[ti], job = N == 1 ? 0 : local / t.aux, b = N == 1 ? local : local % t.aux;
+  const mu_ptrs& p = jobs.p[N == 1 ? 0 : t.first + job];
   const int64_t n = (int64_t)t.m * t.n, stride = (int64_t)t.aux * 256;
   double acc = 0.0;
   if (OPT) {
@@ -173,17 +177,17 @@ k_mu_norm(mu_table tab, mu_jobs jobs, char* ws, float mu, int nesterov, float gs
 
 // ---- X and X' as planes --------------------------------------------------------------------------------------
 // One block: 64 x 64 of the matrix as it is stored (rows x cols), padding included.  l: fp32 input (OPT), d0: X, d1: X'
-template <typename T, bool OPT>
+template <typename T, bool OPT, int N>
 __global__ void __launch_bounds__(256)
-k_mu_planes(mu_table tab, mu_jobs jobs, char* ws, float eps) {
+k_mu_planes(mu_table_of<N> tab, mu_jobs_of<(N == 1 ? 1 : MU_MAX_JOBS)> jobs, char* ws, float eps) {
   __shared__ float tile[64][65];
   __shared__ double total;
   const int gi = mu_find(tab, blockIdx.x);
   const mu_task& g = tab.t[gi];
   const int rows = g.tall ? g.n : g.m, cols = g.tall ? g.m : g.n, prow = g.tall ? g.pn : g.pm, pcol = g.tall ? g.pm : g.pn;
-  const int local = blockIdx.x - tab.blk0[gi], per = (prow / 64) * (pcol / 64), job = local / per, t = local % per;
+  const int per = (prow / 64) * (pcol / 64), local = N == 1 ? blockIdx.x : blockIdx.x - tab.blk0[gi], job = N == 1 ? 0 : local / per, t = local - job * per;
   const int r0 = (t / (pcol / 64)) * 64, c0 = (t % (pcol / 64)) * 64;
-  const void* src = OPT ? (const void*)mu_at(ws, g, job, g.l) : jobs.p[g.first + job].g;
+  const void* src = OPT ? (const void*)mu_at(ws, g, job, g.l) : jobs.p[N == 1 ? 0 : g.first + job].g;
   typedef typename std::conditional<OPT, f32_t, T>::type S;
   S raw[16];                               // (sixteen loads on their way; behind the matrix: its last row and column, not used)
 #pragma unroll
@@ -519,12 +523,12 @@ __device__ __forceinline__ void mu_gemm_tile(const mu_table& tab, const mu_jobs*
 }
 
 template <int TA, int TB, int KU, int DEPTH, int MODE>
-__global__ void __launch_bounds__(256, 2)
+__global__ void __launch_bounds__(256, DEPTH * (TA + TB) * KU > 20 ? 1 : 2)      // (LDS: 4 KB of that product)
 k_mu_gemm(mu_table tab, char* ws) {
   mu_gemm_tile<f32_t, TA, TB, KU, DEPTH, MODE, false>(tab, nullptr, ws, 0.f);
 }
 template <typename T, int TA, int TB, int KU, int DEPTH, bool OPT>
-__global__ void __launch_bounds__(256, 2)
+__global__ void __launch_bounds__(256, DEPTH * (TA + TB) * KU > 20 ? 1 : 2)      // (LDS: 4 KB of that product)
 k_mu_last(mu_table tab, mu_jobs jobs, char* ws, float lr) {
   mu_gemm_tile<T, TA, TB, KU, DEPTH, MU_LAST, OPT>(tab, &jobs, ws, lr);
 }
@@ -533,8 +537,8 @@ k_mu_last(mu_table tab, mu_jobs jobs, char* ws, float lr) {
 // from beyond its die's L2 (some 40 GB/s: another die wrote them; a stage of 32 k of a 64 x 64 tile took 0.42 us, whether two or
 // seven more were on their way), so more units with less each: operands come straight to registers (eight units of 16 k on
 // their way in a wave), without LDS and barriers, and the quarters are added in LDS, in order.
-template <typename T, int MODE, bool OPT>
-__device__ __forceinline__ void mu_small_tile(const mu_table& tab, const mu_jobs* jobs, char* ws, float lr) {
+template <typename T, int MODE, bool OPT, int N, typename J>
+__device__ __forceinline__ void mu_small_tile(const mu_table_of<N>& tab, const J* jobs, char* ws, float lr) {
   constexpr int CHUNK = 4;
   __shared__ __attribute__((aligned(16))) float quarter[4][1024];
   __shared__ __attribute__((aligned(16))) uint32_t turns[2][32 * MU_PITCH];
@@ -544,7 +548,7 @@ __device__ __forceinline__ void mu_small_tile(const mu_table& tab, const mu_jobs
   if (blk < (int)(gridDim.x / (8 * RUN) * (8 * RUN))) blk = blk / (8 * RUN) * (8 * RUN) + (blk & 7) * RUN + (blk >> 3) % RUN;
   const int gi = mu_find(tab, blk);
   const mu_task& g = tab.t[gi];
-  int u = blk - tab.blk0[gi], split = 0, ti, tj;
+  int u = N == 1 ? blk : blk - tab.blk0[gi], split = 0, ti, tj;
   const int tm = g.pm / 32, tn = g.pn / 32, per = MODE == MU_SYM ? tm * (tm + 1) / 2 : tm * tn;
   const bool part = MODE == MU_SYM && g.whole == 0;
   int job, t;
@@ -662,14 +666,14 @@ __device__ __forceinline__ void mu_small_tile(const mu_table& tab, const mu_jobs
     }
   }
 }
-template <int MODE>
+template <int MODE, int N>
 __global__ void __launch_bounds__(256)
-k_mu_small(mu_table tab, char* ws) {
-  mu_small_tile<f32_t, MODE, false>(tab, nullptr, ws, 0.f);
+k_mu_small(mu_table_of<N> tab, char* ws) {
+  mu_small_tile<f32_t, MODE, false>(tab, (const mu_jobs*)nullptr, ws, 0.f);
 }
-template <typename T, bool OPT>
+template <typename T, bool OPT, int N>
 __global__ void __launch_bounds__(256)
-k_mu_small_last(mu_table tab, mu_jobs jobs, char* ws, float lr) {
+k_mu_small_last(mu_table_of<N> tab, mu_jobs_of<(N == 1 ? 1 : MU_MAX_JOBS)> jobs, char* ws, float lr) {
   mu_small_tile<T, MU_LAST, OPT>(tab, &jobs, ws, lr);
 }
 
@@ -862,6 +866,10 @@ static int mu_x_tiles(const mu_group& g, int side, bool last) {
   return (rows + 255) / 256 * (cols / 128);
 }
 
+// A launch of one task, or of one matrix: its table and job alone.
+static bool mu_alone(const mu_table& t) { return t.tasks == 1 && t.t[0].count == 1; }
+static mu_table_of<1> mu_single(const mu_table& t) { return {{0}, 1, {t.t[0]}}; }
+
 class mu_runner {
  public:
   mu_runner(const mu_plan& pl, char* ws, hipStream_t st) : pl_(pl), ws_(ws), st_(st) { memset(&tab_, 0, sizeof(tab_)); }
@@ -957,7 +965,8 @@ class mu_runner {
         }
       }
       // few blocks: one to a compute unit, with more stages on their way
-      if (side == 1) lmh_launch((k_mu_small<MU_SYM>), dim3(blocks), dim3(256), 0, st_, tab_, ws_);
+      if (side == 1 && tab_.tasks == 1) lmh_launch((k_mu_small<MU_SYM, 1>), dim3(blocks), dim3(256), 0, st_, mu_single(tab_), ws_);
+      else if (side == 1) lmh_launch((k_mu_small<MU_SYM, MU_MAX_GROUPS>), dim3(blocks), dim3(256), 0, st_, tab_, ws_);
       else if (side == 2) lmh_launch((k_mu_gemm<1, 1, 2, 4, MU_SYM>), dim3(blocks), dim3(256), 0, st_, tab_, ws_);
       else if (blocks <= MU_SLOTS / 2) lmh_launch((k_mu_gemm<2, 2, 2, 4, MU_SYM>), dim3(blocks), dim3(256), 0, st_, tab_, ws_);
       else lmh_launch((k_mu_gemm<2, 2, 2, 2, MU_SYM>), dim3(blocks), dim3(256), 0, st_, tab_, ws_);
@@ -977,7 +986,8 @@ class mu_runner {
         t->aux = g.pm / 16;
         return mu_x_tiles(g, side, false) * g.count;
       });
-      if (side == 1) lmh_launch((k_mu_small<MU_APPLY>), dim3(nb), dim3(256), 0, st_, tab_, ws_);
+      if (side == 1 && tab_.tasks == 1) lmh_launch((k_mu_small<MU_APPLY, 1>), dim3(nb), dim3(256), 0, st_, mu_single(tab_), ws_);
+      else if (side == 1) lmh_launch((k_mu_small<MU_APPLY, MU_MAX_GROUPS>), dim3(nb), dim3(256), 0, st_, tab_, ws_);
       else if (side == 2) lmh_launch((k_mu_gemm<1, 1, 2, 4, MU_APPLY>), dim3(nb), dim3(256), 0, st_, tab_, ws_);
       else if (side == 8) lmh_launch((k_mu_gemm<4, 2, 1, 3, MU_APPLY>), dim3(nb), dim3(256), 0, st_, tab_, ws_);
       else lmh_launch((k_mu_gemm<2, 2, 2, 2, MU_APPLY>), dim3(nb), dim3(256), 0, st_, tab_, ws_);
@@ -1038,7 +1048,8 @@ static void mu_run(const lmh_muon_job* jobs, const mu_plan& pl, int steps, float
     t->d0 = g.xt[1];                   // (free until the first product with X has been taken)
     return g.norm_blocks;
   }, [&](dim3 nb, const mu_table& tab, const mu_jobs& pj) {
-    lmh_launch((k_mu_norm<T, OPT>), nb, dim3(256), 0, st, tab, pj, ws, mu, nesterov, gscale);
+    if (mu_alone(tab)) lmh_launch((k_mu_norm<T, OPT, 1>), nb, dim3(256), 0, st, mu_single(tab), mu_jobs_of<1>{{pj.p[0]}}, ws, mu, nesterov, gscale);
+    else lmh_launch((k_mu_norm<T, OPT, MU_MAX_GROUPS>), nb, dim3(256), 0, st, tab, pj, ws, mu, nesterov, gscale);
   });
   run.with_jobs(jobs, all, [](const mu_group& g, mu_task* t) {
     t->aux = g.norm_blocks;
@@ -1047,7 +1058,8 @@ static void mu_run(const lmh_muon_job* jobs, const mu_plan& pl, int steps, float
     t->d1 = g.xt[0];
     return (g.pm / 64) * (g.pn / 64);
   }, [&](dim3 nb, const mu_table& tab, const mu_jobs& pj) {
-    lmh_launch((k_mu_planes<T, OPT>), nb, dim3(256), 0, st, tab, pj, ws, eps);
+    if (mu_alone(tab)) lmh_launch((k_mu_planes<T, OPT, 1>), nb, dim3(256), 0, st, mu_single(tab), mu_jobs_of<1>{{pj.p[0]}}, ws, eps);
+    else lmh_launch((k_mu_planes<T, OPT, MU_MAX_GROUPS>), nb, dim3(256), 0, st, tab, pj, ws, eps);
   });
   for (int kind = 0; kind < 2; ++kind) {
     const std::vector<const mu_group*>& G = gs[kind];
@@ -1108,7 +1120,9 @@ static void mu_run(const lmh_muon_job* jobs, const mu_plan& pl, int steps, float
           t->aux = g.pm / 16;
           return mu_x_tiles(g, side_x, true);
         }, [&](dim3 nb, const mu_table& tab, const mu_jobs& pj) {
-          if (side_x == 1) lmh_launch((k_mu_small_last<T, OPT>), nb, dim3(256), 0, st, tab, pj, ws, lr);
+          if (side_x == 1 && mu_alone(tab))
+            lmh_launch((k_mu_small_last<T, OPT, 1>), nb, dim3(256), 0, st, mu_single(tab), mu_jobs_of<1>{{pj.p[0]}}, ws, lr);
+          else if (side_x == 1) lmh_launch((k_mu_small_last<T, OPT, MU_MAX_GROUPS>), nb, dim3(256), 0, st, tab, pj, ws, lr);
           else if (side_x == 2) lmh_launch((k_mu_last<T, 1, 1, 2, 4, OPT>), nb, dim3(256), 0, st, tab, pj, ws, lr);
           else if (side_x == 8) lmh_launch((k_mu_last<T, 4, 2, 1, 3, OPT>), nb, dim3(256), 0, st, tab, pj, ws, lr);
           else lmh_launch((k_mu_last<T, 2, 2, 2, 2, OPT>), nb, dim3(256), 0, st, tab, pj, ws, lr);
