@@ -1481,9 +1481,13 @@ def muon_fits(rows, cols):
 
 def _matrix_of(t, what):
     """(..., out) weights as the matrix (inputs, out): HWIO kernels flattened like a Linear's (in, out)."""
-    _refuse(t.dim() < 2 or t.numel() == 0, '%s: matrices expected, got shape %s', what, tuple(t.shape))
-    rows, cols = t.numel() // t.shape[-1], t.shape[-1]
-    _refuse(not muon_fits(rows, cols), '%s: at most %d rows and columns and 2^30 values, got %d x %d', what, MUON_MAX_DIM, rows, cols)
+    shape, values = t.shape, t.numel()
+    if len(shape) < 2 or values == 0:
+        raise _lib.LuminothHipError('%s: matrices expected, got shape %s' % (what, tuple(shape)))
+    cols = shape[-1]
+    rows = values // cols
+    if not muon_fits(rows, cols):
+        raise _lib.LuminothHipError('%s: at most %d rows and columns and 2^30 values, got %d x %d' % (what, MUON_MAX_DIM, rows, cols))
     return rows, cols
 
 
@@ -1498,18 +1502,19 @@ def orthogonalize(mats, steps=5, eps=1e-7):
         return []
     dtype = _row_dtype(mats[0], 'orthogonalize')
     jobs = (_lib.MuonJob * len(mats))()
-    out = []
+    out, kind = [], mats[0].dtype
     for j, u in zip(jobs, mats):
-        _refuse(u.dtype != mats[0].dtype, 'orthogonalize: matrices of one type expected, got %s and %s', mats[0].dtype, u.dtype)
+        _refuse(u.dtype is not kind, 'orthogonalize: matrices of one type expected, got %s and %s', kind, u.dtype)
         j.rows, j.cols = _matrix_of(u, 'orthogonalize')
     dev = _same_device(*mats)
     if dev != _get_device():
         with torch.cuda.device(dev):
             return orthogonalize(mats, steps, eps)
     for j, u in zip(jobs, mats):
-        o = _new(u.shape, u.dtype, u.device)
+        j.g = _flat(u, 'orthogonalize')
+        o = _new_like(u)
         out.append(o)
-        j.g, j.out = _p(u).value, _p(o).value
+        j.out = _pr(o)
     ws = _new((lib.lmh_muon_workspace_bytes(jobs, len(mats)),), torch.uint8, mats[0].device)
     check(lib.lmh_orthogonalize(jobs, len(mats), dtype, int(steps), float(eps), _p(ws), ctypes.c_size_t(ws.numel()), _stream()),
           'lmh_orthogonalize')
@@ -1533,6 +1538,7 @@ class MuonJobs(object):
         self.jobs, self.count = (_lib.MuonJob * n)(), n
         for t in self.tensors:
             _refuse(t.dtype != torch.float32, 'muon: float32 expected, got %s', t.dtype)
+            _refuse(not t.is_contiguous(), 'muon: contiguous tensors expected, got strides %s', t.stride())
         for i, (j, w, g, v) in enumerate(zip(self.jobs, params, grads, moms)):
             _refuse(w.shape != g.shape or w.shape != v.shape, 'muon: weights, gradient and momentum of one shape expected, got %s, %s, %s',
                     tuple(w.shape), tuple(g.shape), tuple(v.shape))

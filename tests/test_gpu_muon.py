@@ -203,3 +203,25 @@ def test_one_gradient_for_two_weights():
     K.muon_step(w2, [g.clone(), g.clone()], v2, lr=0.1)
     for a, b in zip(w + v, w2 + v2):
         assert torch.equal(a, b)
+
+
+def test_matrices_that_are_not_contiguous_are_refused():
+    from luminoth_amd import _lib
+    u = make(48, 32).cuda()
+    with pytest.raises(_lib.LuminothHipError, match='contiguous'):
+        K.orthogonalize([u.t()])
+    with pytest.raises(_lib.LuminothHipError, match='contiguous'):
+        K.muon_step([u.t()], [u.t()], [torch.zeros_like(u).t()], lr=0.1)
+
+
+def test_one_shape_and_many():
+    """A launch of one shape has a table of its own: one matrix, several of one shape, and the same ones among others."""
+    a, b, c = make(90, 170), make(90, 170, seed=1), make(40, 60)
+    for mats in ([a], [a, b], [a, b, c]):
+        for m, o in zip(mats, K.orthogonalize([m.cuda() for m in mats])):
+            close(o, m)
+    w, v = [m.cuda() for m in (a, b)], [torch.zeros(90, 170, device='cuda') for _ in range(2)]
+    K.muon_step(w, [m.cuda() for m in (b, a)], v, lr=1.0, momentum=0.0, nesterov=False, scale=[1.0, 1.0])
+    for got, start, g in zip(w, (a, b), (b, a)):
+        err = float(torch.linalg.norm(got.cpu().double() - (start.double() - ns(g))))
+        assert err <= bound(g) + 2.0 ** -24 * float(torch.linalg.norm(got.cpu().double()))
