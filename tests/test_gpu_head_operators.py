@@ -211,3 +211,41 @@ def test_a_classifier_with_all_three():
     for a, b in zip(dev, ref):
         # each step moves a weight by lr 0.2 sqrt(80) O: O is off by 2e-5 of its gradient's norm, 485 times over where O is small
         assert float(torch.linalg.norm(a.detach().cpu().double() - b.detach())) <= 3 * 0.02 * 0.2 * 9 * 485 * 2e-5 + 1e-5
+
+
+def test_calls_from_two_threads():
+    """Two threads with a stream each, the same operators at the same time: the bits of the calls alone."""
+    import threading
+    g = torch.Generator().manual_seed(11)
+    inputs = [(torch.randn((300, 1500), generator=g).cuda(), torch.randn((6, 50000), generator=g).bfloat16().cuda(),
+               torch.randint(0, 50000, (6,), generator=g).cuda(), [torch.randn((200, 310), generator=g).cuda() for _ in range(2)]) for _ in range(2)]
+
+    def calls(x, logits, targets, mats):
+        y, mean, rstd = K.layer_norm_fwd(x)
+        dg, db = torch.empty(1500, device='cuda'), torch.empty(1500, device='cuda')
+        out = [y, K.layer_norm_bwd(x, x, mean, rstd, None, dg, db), dg, db]
+        out += list(K.log_probs_fwd(logits, targets, 5))
+        out.append(K.log_probs_bwd(logits, targets, out[-1], out[-4], torch.ones(6, device='cuda')))
+        return out + K.orthogonalize(mats)
+    want = [calls(*a) for a in inputs]
+    torch.cuda.synchronize()
+    got, failed = [[], []], []
+
+    def work(i):
+        try:
+            with torch.cuda.stream(torch.cuda.Stream()):
+                for _ in range(20):
+                    got[i].append(calls(*inputs[i]))
+                torch.cuda.current_stream().synchronize()
+        except Exception as e:                              # (pytest sees only its own thread)
+            failed.append(e)
+    threads = [threading.Thread(target=work, args=(i,)) for i in range(2)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert not failed, failed
+    for i in range(2):
+        for results in got[i]:
+            for a, b in zip(want[i], results):
+                assert torch.equal(a, b)

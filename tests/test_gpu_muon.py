@@ -165,7 +165,7 @@ def test_same_bits_streams_and_graph():
                 assert torch.equal(a, b)
 
 
-@pytest.mark.parametrize('rows,cols', [(4100, 4200), (4000, 9000), (2900, 8800), (8800, 2900)])
+@pytest.mark.parametrize('rows,cols', [(1000, 2100), (1500, 1600), (5000, 1400), (4100, 4200), (4000, 9000), (2900, 8800), (8800, 2900)])
 def test_large_matrices(rows, cols):
     """More tiles than one round of blocks takes: the last ones are split along k and joined; products with X in tiles of 256 rows,
     of which the last has 128; the reference on the device too."""
