@@ -214,6 +214,15 @@ def test_matrices_that_are_not_contiguous_are_refused():
         K.muon_step([u.t()], [u.t()], [torch.zeros_like(u).t()], lr=0.1)
 
 
+@pytest.mark.parametrize('steps', [1, 2, 3, 4, 5])
+def test_short_sides(steps):
+    """All steps in A in one launch: lists of at most 64 and of at most 128 rows, padded ones among them."""
+    for sizes in ([(64, 64), (40, 50), (300, 7)], [(128, 300), (33, 900), (100, 260), (800, 65)]):
+        mats = [make(*s) for s in sizes]
+        for m, o in zip(mats, K.orthogonalize([m.cuda() for m in mats], steps=steps)):
+            close(o, m, steps=steps)
+
+
 def test_one_shape_and_many():
     """A launch of one shape has a table of its own: one matrix, several of one shape, and the same ones among others."""
     a, b, c = make(90, 170), make(90, 170, seed=1), make(40, 60)
