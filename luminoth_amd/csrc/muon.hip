@@ -15,7 +15,11 @@
 // Long matrices (n >= 2 m).  The steps are polynomials in A, which commute: A <- p A p and Q <- p Q take m x m products only, and
 // X <- Q X comes every second or third step: of 15 m m n multiplications in five steps 6 are left.  A's error grows by up to
 // a^2 = 11.9 a step where A is small (there p hardly depends on it: |b| / a of it), so A is taken anew from X after three
-// steps at most.  Shorter matrices go X by X: A has nothing to save there.
+// steps at most.  Relative errors after five steps, of random matrices, against float64 (the same in fp32, step by step in X: 0.9e-6 for
+// 20 x 41, 1.4 for 100 x 220, 2.2 for 250 x 600, 3.4 for 1000 x 2100): one step at a time 1.0, 0.8, 1.1, 1.5e-6; two 2.1, 1.9, 1.2,
+// 1.8; three 2.9, 2.8, 2.3, 1.9.  So lists with a short side of 256 take three, of 128 two, and smaller ones, whose launches are as many
+// either way, one (a small matrix beside large ones goes their way, at up to 5e-6).  Shorter matrices go X by X too: A has nothing to
+// save there.
 //
 // Layout.  An operand lies in memory as the matrix instruction takes it ("planes"): [32 rows][16 k] units of hi then lo, 64
 // lanes x 16 bytes each, k units of one row block after each other.  Tiles go to LDS with lane-linear 16-byte DMA and come
@@ -56,7 +60,6 @@
 // instructions instead of 8 + 4 for 12 - with those LDS has as many cycles of work as the matrix cores - (4096 x 4096: 373 -> 350 us a
 // product = 1180 TFLOP/s of f16 instructions).  Where rounds of blocks cost more than that gains, or k is short and the rest of a
 // block's work counts (42 matrices of m = 128 to 512: 50 -> 53 us), 128 x 128 stays.
-#define MU_CHAIN_ROWS 128      // k_mu_chain
 #define MU_NORM_BLOCKS 512
 #define MU_NORM_ELEMS 2048    // at least this many per block of k_mu_norm
 
@@ -678,87 +681,6 @@ k_mu_small_last(mu_table_of<N> tab, mu_jobs_of<(N == 1 ? 1 : MU_MAX_JOBS)> jobs,
   mu_small_tile<T, MU_LAST, OPT>(tab, &jobs, ws, lr);
 }
 
-// All steps of a segment in A for matrices of at most 32 SIDE rows (t.aux: steps; reads A, leaves P (one step) or their product Q), one
-// block each, a wave for each 32 x 32 block: A and P as planes in LDS, A in the accumulators too:
-//   p = a I + b A + c A A,   Q <- p Q,   z = p A,   A <- z p
-// A launch a product takes some 5 us each; here a product takes 1.1 us up to 64 rows and 3.5 up to 128 (64 x 600, all steps: 70 -> 44 us,
-// 128 x 2000 88 -> 80, 200 of 128 x 512 577 -> 530).  Blocks above the diagonal alone, mirrored through LDS: 48, 78 and 530.
-template <int SIDE>
-__global__ void __launch_bounds__(64 * SIDE * SIDE)
-k_mu_chain(mu_table tab, char* ws) {
-  __shared__ __attribute__((aligned(16))) char Al[SIDE * SIDE * 4096];       // A, then z
-  __shared__ __attribute__((aligned(16))) char Pl[SIDE * SIDE * 4096];
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, l31 = lane & 31, h = lane >> 5, rb = wave / SIDE, cb = wave % SIDE;
-  const int gi = mu_find(tab, blockIdx.x);
-  const mu_task& g = tab.t[gi];
-  const int job = blockIdx.x - tab.blk0[gi], units = g.pm / 16, steps = g.aux;
-  const bool live = rb * 2 < units && cb * 2 < units;          // (all waves meet all barriers)
-  char* q0 = mu_at(ws, g, job, g.d0);
-  char* q1 = mu_at(ws, g, job, g.d1);
-  const raw16* from = reinterpret_cast<const raw16*>(mu_at(ws, g, job, g.l));
-  for (int i = threadIdx.x; i < g.pm * g.pm / 4; i += 64 * SIDE * SIDE) reinterpret_cast<raw16*>(Al)[i] = from[i];
-  __syncthreads();
-  const int at = (cb * units + rb * 2) * 2048;                 // of this wave's result (symmetric: its columns as rows)
-  float av[16];
-#pragma unroll
-  for (int j = 0; j < 4; ++j) {
-    typedef _Float16 f16x4 __attribute__((ext_vector_type(4)));
-    const char* p = Al + (live ? at : 0) + (j >> 1) * 2048 + (l31 + 32 * (j & 1)) * 16 + h * 8;
-    const f16x4 hi = *reinterpret_cast<const f16x4*>(p), lo = *reinterpret_cast<const f16x4*>(p + 1024);
-#pragma unroll
-    for (int e = 0; e < 4; ++e) av[4 * j + e] = ((float)hi[e] + (float)lo[e]) * (1.f / MU_SG);
-  }
-  auto product = [&](const char* L, const char* R, float scale, float* out) {
-    f32x16 acc;
-#pragma unroll
-    for (int i = 0; i < 16; ++i) acc[i] = 0.f;
-    const char* l = L + rb * units * 2048 + lane * 16;
-    const char* r = R + cb * units * 2048 + lane * 16;
-    for (int u = 0; u < units; u += 4, l += 8192, r += 8192)      // (units: four or eight)
-#pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        const f16x8 lh = *reinterpret_cast<const f16x8*>(l + e * 2048), ll = *reinterpret_cast<const f16x8*>(l + e * 2048 + 1024);
-        const f16x8 rh = *reinterpret_cast<const f16x8*>(r + e * 2048), rl = *reinterpret_cast<const f16x8*>(r + e * 2048 + 1024);
-        acc = __builtin_amdgcn_mfma_f32_32x32x16_f16(lh, rl, acc, 0, 0, 0);
-        acc = __builtin_amdgcn_mfma_f32_32x32x16_f16(ll, rh, acc, 0, 0, 0);
-        acc = __builtin_amdgcn_mfma_f32_32x32x16_f16(lh, rh, acc, 0, 0, 0);
-      }
-#pragma unroll
-    for (int i = 0; i < 16; ++i) out[i] = acc[i] * scale;
-  };
-  auto store = [&](const float* v, float scale, char* to) {
-    float x[16];
-#pragma unroll
-    for (int i = 0; i < 16; ++i) x[i] = v[i] * scale;
-    mu_store(x, to + at, nullptr, lane, nullptr);
-  };
-  for (int k = 0; k < steps; ++k) {
-    float v[16];
-    if (live) {
-      product(Al, Al, MU_C / (MU_SG * MU_SG), v);
-#pragma unroll
-      for (int i = 0; i < 16; ++i) v[i] += MU_B * av[i] + (rb == cb && (i & 3) + 8 * (i >> 2) + 4 * h == l31 ? MU_A : 0.f);
-      store(v, MU_SP, Pl);
-      if (k == 0) store(v, steps == 1 ? MU_SP : MU_SQ, q0);
-    }
-    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");           // (Q, which other waves read)
-    __syncthreads();
-    if (k > 0 && live) {
-      product(Pl, k & 1 ? q0 : q1, 1.f / (MU_SP * MU_SQ), v);
-      store(v, MU_SQ, k & 1 ? q1 : q0);
-    }
-    if (k + 1 == steps) break;
-    if (live) product(Pl, Al, 1.f / (MU_SP * MU_SG), v);
-    __syncthreads();
-    if (live) store(v, MU_SG, Al);
-    __syncthreads();
-    if (live) product(Al, Pl, 1.f / (MU_SG * MU_SP), av);
-    __syncthreads();
-    if (live) store(av, MU_SG, Al);
-    __syncthreads();
-  }
-}
-
 // Joins the parts of split tiles (WAVES: four with TW x TW 32-blocks each, or one), one 32 x 32 block of a tile each wave (blk0 counts
 // tiles).
 template <int TW, int WAVES>
@@ -806,6 +728,7 @@ struct mu_plan {
   std::vector<int> order;              // the caller's jobs, sorted by shape
   std::vector<mu_group> groups;
   int tw;                              // tiles of the products with X: 64 tw
+  int segment;                         // steps in A behind each other, at most
   int64_t slab, slab_units, units;
 };
 
@@ -873,14 +796,14 @@ static void mu_make_plan(const lmh_muon_job* jobs, int count, mu_plan* pl) {
     all.add(mu_up(m, 128), mu_up(n, 128), 1);
   }
   if (!all.large()) pl->tw = 1;
-  // short sides: the steps in A are one launch (k_mu_chain; up to 64 rows the fastest way for square ones too: 50 x 60 60 -> 40 us, but
-  // 100 x 120 63 -> 65).  One long matrix, and the others but for large ones go its way: the number of multiplications is the same
-  // for m = n, and two kinds would take their launches one after the other
-  bool all_long = false, short_sides = true;
+  // one long matrix, and the others but for large ones go its way: the number of multiplications is the same for m = n, and two
+  // kinds would take their launches one after the other
+  bool all_long = false;
   for (int i = 0; i < count; ++i)
     if (std::max(jobs[i].rows, jobs[i].cols) >= 2 * std::min(jobs[i].rows, jobs[i].cols)) all_long = true;
-  for (int i = 0; i < count; ++i)
-    if (std::min(jobs[i].rows, jobs[i].cols) > MU_CHAIN_ROWS / 2) short_sides = false;
+  int largest = 0;
+  for (int i = 0; i < count; ++i) largest = std::max(largest, std::min(jobs[i].rows, jobs[i].cols));
+  pl->segment = largest >= 256 ? 3 : largest >= 128 ? 2 : 1;
   const int bt = 64 * pl->tw;
   int64_t off = 0;
   pl->groups.clear();
@@ -896,7 +819,7 @@ static void mu_make_plan(const lmh_muon_job* jobs, int count, mu_plan* pl) {
     g.pn = (int)mu_up(g.n, bt);
     g.count = e - s;
     g.first = s;
-    g.longish = short_sides || (all_long && g.pm <= 2048) || g.n >= 2 * g.m;
+    g.longish = pl->segment > 1 && ((all_long && g.pm <= 2048) || g.n >= 2 * g.m);
     const int mn = (int)((int64_t)g.pm * g.pn / 64), mm = (int)((int64_t)g.pm * g.pm / 64);      // 4 bytes a value, units of 256
     int at = 0;
     auto take = [&](int n) { const int r = at; at += n; return r; };
@@ -1078,22 +1001,6 @@ class mu_runner {
       else lmh_launch((k_mu_gemm<2, 2, 2, 2, MU_APPLY>), dim3(nb), dim3(256), 0, st_, tab_, ws_);
     }
   }
-  // The steps of a segment in A of matrices of short sides: `steps` of them, into P (one) or into the product Q[(steps - 1) & 1].
-  void chain(const std::vector<const mu_group*>& gs, int steps) {
-    int most = 0;
-    for (const mu_group* g : gs) most = std::max(most, g->pm);
-    for (size_t lo = 0; lo < gs.size(); lo += MU_MAX_GROUPS) {
-      const int nb = tasks(gs, lo, std::min(gs.size(), lo + MU_MAX_GROUPS), [&](const mu_group& g, mu_task* t) {
-        t->aux = steps;
-        t->l = g.a;
-        t->d0 = steps == 1 ? g.p : g.q[0];
-        t->d1 = g.q[1];
-        return g.count;
-      });
-      if (most <= 64) lmh_launch((k_mu_chain<2>), dim3(nb), dim3(256), 0, st_, tab_, ws_);
-      else lmh_launch((k_mu_chain<4>), dim3(nb), dim3(1024), 0, st_, tab_, ws_);
-    }
-  }
   // Launches that take the caller's pointers: at most MU_MAX_JOBS matrices of MU_MAX_GROUPS shapes each.
   template <typename F, typename L>
   void with_jobs(const lmh_muon_job* jobs, const std::vector<const mu_group*>& gs, F fill, L launch) {
@@ -1169,11 +1076,9 @@ static void mu_run(const lmh_muon_job* jobs, const mu_plan& pl, int steps, float
     for (const mu_group* g : G) counts.add(g->pm, g->pn, g->count);
     const int most = pl.tw == 2 ? 8 : 2;
     const int side = std::min(most, counts.square()), side_x = std::min(most, counts.apply()), side_gram = std::min(most, counts.gram());
-    bool chained = kind == 1;
-    for (const mu_group* g : G) chained = chained && g->m <= MU_CHAIN_ROWS;
     int flip = 0;
     for (int done = 0; done < steps;) {
-      const int left = steps - done, len = kind == 0 ? 1 : left == 4 ? 2 : std::min(left, 3);
+      const int left = steps - done, len = kind == 0 ? 1 : left == 4 ? 2 : std::min(left, pl.segment);
       // A = X X' and b I + c A
       run.symmetric(G, side_gram, [](const mu_group& g, mu_runner::product* p) {
         const float s = 1.f / (MU_SX * MU_SX);
@@ -1181,11 +1086,7 @@ static void mu_run(const lmh_muon_job* jobs, const mu_plan& pl, int steps, float
         return 1;
       });
       int q = 0;                       // of a run of several steps: their product so far in q[q]
-      if (chained) {
-        run.chain(G, len);
-        q = (len - 1) & 1;
-      }
-      for (int k = 0; k < len && !chained; ++k) {
+      for (int k = 0; k < len; ++k) {
         // p = (b I + c A) A + a I; the first of several is their product too
         run.symmetric(G, side, [&](const mu_group& g, mu_runner::product* p) {
           const float s = 1.f / (MU_SC * MU_SG);

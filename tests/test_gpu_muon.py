@@ -216,11 +216,33 @@ def test_matrices_that_are_not_contiguous_are_refused():
 
 @pytest.mark.parametrize('steps', [1, 2, 3, 4, 5])
 def test_short_sides(steps):
-    """All steps in A in one launch: lists of at most 64 and of at most 128 rows, padded ones among them."""
+    """Lists of short sides, padded ones among them: up to 64 rows, and up to 128."""
     for sizes in ([(64, 64), (40, 50), (300, 7)], [(128, 300), (33, 900), (100, 260), (800, 65)]):
         mats = [make(*s) for s in sizes]
         for m, o in zip(mats, K.orthogonalize([m.cuda() for m in mats], steps=steps)):
             close(o, m, steps=steps)
+
+
+@pytest.mark.parametrize('rows,cols', [(16, 33), (20, 41), (16, 100), (40, 40), (60, 120), (100, 220), (64, 600), (127, 300), (128, 260), (200, 420),
+                                       (256, 520), (320, 1024), (500, 500)])
+def test_as_exact_as_fp32(rows, cols):
+    """The error against float64 is that of the steps in X in fp32, within a factor of two, in the mean over eight matrices.
+    u = 2^-24, a rounding's root mean square is u / sqrt(3) = 0.58 u: a product in fp32 is off by its sum's and its result's, 0.82 u
+    |L| |R| together; here by those, by both operands' (their second halves end at u) and by the product of the second halves that is
+    left out (u / 3): 1.2 u, 1.5 times as much, and what follows a product is the same on both sides.  Eight matrices of 16 directions
+    and more: each side's mean is known to 1 / sqrt(128) = 9 %, their quotient to 12 %, two of those make 1.5 a 1.9.  Several steps in A
+    without a fresh one would be off by 3 to 5 times as much where the matrix is small."""
+    plain, own = 0.0, 0.0
+    for seed in range(8):
+        u = torch.randn((rows, cols), generator=torch.Generator().manual_seed(seed)).cuda()
+        x = u / torch.linalg.norm(u)
+        for _ in range(5):
+            g = x @ x.t()
+            x = COEF[0] * x + (COEF[1] * g + COEF[2] * (g @ g)) @ x
+        want = ns(u)
+        plain += float(torch.linalg.norm(x.double() - want) / torch.linalg.norm(want)) / 8
+        own += float(torch.linalg.norm(K.orthogonalize([u])[0].double() - want) / torch.linalg.norm(want)) / 8
+    assert own <= 2 * plain, (own, plain)
 
 
 def test_one_shape_and_many():
