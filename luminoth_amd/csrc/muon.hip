@@ -527,12 +527,12 @@ __device__ __forceinline__ void mu_gemm_tile(const mu_table& tab, const mu_jobs*
 }
 
 template <int TA, int TB, int KU, int DEPTH, int MODE>
-__global__ void __launch_bounds__(256, DEPTH * (TA + TB) * KU > 20 ? 1 : 2)      // (LDS: 4 KB of that product)
+__global__ void __launch_bounds__(256, 2)
 k_mu_gemm(mu_table tab, char* ws) {
   mu_gemm_tile<f32_t, TA, TB, KU, DEPTH, MODE, false>(tab, nullptr, ws, 0.f);
 }
 template <typename T, int TA, int TB, int KU, int DEPTH, bool OPT>
-__global__ void __launch_bounds__(256, DEPTH * (TA + TB) * KU > 20 ? 1 : 2)      // (LDS: 4 KB of that product)
+__global__ void __launch_bounds__(256, 2)
 k_mu_last(mu_table tab, mu_jobs jobs, char* ws, float lr) {
   mu_gemm_tile<T, TA, TB, KU, DEPTH, MU_LAST, OPT>(tab, &jobs, ws, lr);
 }
@@ -972,11 +972,9 @@ class mu_runner {
           joins += (int)(n - c.whole);
         }
       }
-      // few blocks: one to a compute unit, with more stages on their way
       if (side == 1 && tab_.tasks == 1) lmh_launch((k_mu_small<MU_SYM, 1>), dim3(blocks), dim3(256), 0, st_, mu_single(tab_), ws_);
       else if (side == 1) lmh_launch((k_mu_small<MU_SYM, MU_MAX_GROUPS>), dim3(blocks), dim3(256), 0, st_, tab_, ws_);
       else if (side == 2) lmh_launch((k_mu_gemm<1, 1, 2, 4, MU_SYM>), dim3(blocks), dim3(256), 0, st_, tab_, ws_);
-      else if (blocks <= MU_SLOTS / 2) lmh_launch((k_mu_gemm<2, 2, 2, 4, MU_SYM>), dim3(blocks), dim3(256), 0, st_, tab_, ws_);
       else lmh_launch((k_mu_gemm<2, 2, 2, 2, MU_SYM>), dim3(blocks), dim3(256), 0, st_, tab_, ws_);
       if (joins) {
         if (side == 1) lmh_launch((k_mu_join<1, 1>), dim3(joins), dim3(64), 0, st_, join, ws_);
