@@ -17,9 +17,13 @@
 // a^2 = 11.9 a step where A is small (there p hardly depends on it: |b| / a of it), so A is taken anew from X after three
 // steps at most.  Relative errors after five steps, of random matrices, against float64 (the same in fp32, step by step in X: 0.9e-6 for
 // 20 x 41, 1.4 for 100 x 220, 2.2 for 250 x 600, 3.4 for 1000 x 2100): one step at a time 1.0, 0.8, 1.1, 1.5e-6; two 2.1, 1.9, 1.2,
-// 1.8; three 2.9, 2.8, 2.3, 1.9.  So lists with a short side of 256 take three, of 128 two, and smaller ones, whose launches are as many
-// either way, one (a small matrix beside large ones goes their way, at up to 5e-6).  Shorter matrices go X by X too: A has nothing to
-// save there.
+// 1.8; three 2.9, 2.8, 2.3, 1.9.  So a matrix takes three with a short side of 256, two with one of 128, and X by X goes what is smaller
+// or not long (there A has little or nothing to save).  That goes by its own sides, whatever else is in the list: three steps for all
+// of a list with one large matrix had squares of 16 beside it off by 5.6e-6, 7 times as much as fp32 (now 0.8e-6).  The three kinds
+// advance side by side, a launch for all of them, and the five products with X of one meet the others' where they can: the 42
+// matrices of a ResNet-50 detector take 28 launches, 491 us (three steps for all of them: 22 and 444; one: 589).  One matrix of few tiles
+// takes as long either way (1024 x 320 100 us with three and with one, 200 x 420 82 and 77), eight of them do not (320 x 1024 199 and
+// 219).
 //
 // Layout.  An operand lies in memory as the matrix instruction takes it ("planes"): [32 rows][16 k] units of hi then lo, 64
 // lanes x 16 bytes each, k units of one row block after each other.  Tiles go to LDS with lane-linear 16-byte DMA and come
@@ -32,7 +36,7 @@
 // along k; their parts are joined, in order, by a launch of their own.
 //
 // Measured (five steps): 4096 x 4096 fp32 3.95 ms, products with X 350 us = 1180 TFLOP/s of f16 instructions, symmetric ones 206 us = 1040;
-// 1024 x 320 bf16 100 us in 19 launches; the 42 matrices of a ResNet-50 detector, a whole optimizer step, 454 us in 22.
+// 1024 x 320 bf16 100 us in 19 launches; the 42 matrices of a ResNet-50 detector, a whole optimizer step, 491 us in 28.
 #include <algorithm>
 #include <tuple>
 #include <type_traits>
@@ -720,7 +724,7 @@ static int64_t mu_up(int64_t v, int64_t a) { return (v + a - 1) / a * a; }
 
 struct mu_group {
   int m, n, pm, pn, count, first, tall;
-  bool longish;                        // steps in A alone, X every second or third
+  int segment;                         // steps in A behind each other, at most (1: X by X)
   int64_t off, stride;                 // units of 256 bytes
   int x, xt[2], a, c, p, z, q[2], norm, norm_blocks;
 };
@@ -728,7 +732,6 @@ struct mu_plan {
   std::vector<int> order;              // the caller's jobs, sorted by shape
   std::vector<mu_group> groups;
   int tw;                              // tiles of the products with X: 64 tw
-  int segment;                         // steps in A behind each other, at most
   int64_t slab, slab_units, units;
 };
 
@@ -753,30 +756,34 @@ static mu_cut mu_cut_of(int64_t tiles, int stages, int64_t all_stages, int64_t a
   return c;
 }
 
-// Tiles (of 128 x 128 and 64 x 64) of the m x m products and of those with X, and what sides (of 32) they have.
+// Tiles (of 128 x 128 and 64 x 64) of the symmetric products of a launch (X X' and those of m x m matrices) or of its products with X,
+// and what sides (of 32) its tiles have.
 struct mu_counts {
-  int64_t tiles = 0, xtiles = 0, xtall = 0, xdepth = 0, xstages = 0, tiles64 = 0, xtiles64 = 0;
-  void add(int64_t pm, int64_t pn, int64_t count) {
+  int64_t grams = 0, squares = 0, xtiles = 0, xtall = 0, xdepth = 0, stages = 0, tiles64 = 0, xtiles64 = 0;
+  void add_symmetric(int64_t pm, int64_t count, int64_t units, bool gram) {
     const int64_t t = count * (pm / 128) * (pm / 128 + 1) / 2;
-    tiles += t;
+    (gram ? grams : squares) += t;
+    if (gram) stages += t * (units / 2);
+    tiles64 += count * (pm / 64) * (pm / 64 + 1) / 2;
+  }
+  void add_apply(int64_t pm, int64_t pn, int64_t count) {
     xtiles += count * (pm / 128) * (pn / 128);
     xdepth += count * (pm / 128) * (pn / 128) * pm;
     xtall += count * (pm / 128) * ((pn / 128 + 1) / 2);
-    xstages += t * (pn / 32);
-    tiles64 += count * (pm / 64) * (pm / 64 + 1) / 2;
     xtiles64 += count * (pm / 64) * (pn / 64);
   }
   // 64 x 64 while tiles of 128 x 128 would leave places free
-  int square() const { return tiles64 <= MU_SMALL ? 1 : tiles < 256 ? 2 : 4; }
+  int symmetric() const { return tiles64 <= MU_SMALL ? 1 : squares >= 256 || stages >= 4096 ? 4 : 2; }
   int apply() const {
     if (xtiles64 <= MU_SMALL_X) return 1;
     if (xtiles < 128) return 2;
     const int64_t rounds = (xtiles + MU_SLOTS - 1) / MU_SLOTS, tall = (xtall + MU_SLOTS - 1) / MU_SLOTS;
     return 188 * tall < 100 * rounds && xdepth >= 1024 * xtiles ? 8 : 4;
   }
-  int gram() const { return tiles64 <= MU_SMALL ? 1 : xstages < 4096 ? 2 : 4; }
-  bool large() const { return square() >= 4 || apply() >= 4 || gram() >= 4; }
 };
+
+// By a matrix's own sides, whatever else is in the list: its error does not depend on its companions.
+static int mu_segment(int m, int n) { return n < 2 * m ? 1 : m >= 256 ? 3 : m >= 128 ? 2 : 1; }
 
 static void mu_make_plan(const lmh_muon_job* jobs, int count, mu_plan* pl) {
   pl->order.resize(count);
@@ -788,22 +795,16 @@ static void mu_make_plan(const lmh_muon_job* jobs, int count, mu_plan* pl) {
   };
   std::stable_sort(pl->order.begin(), pl->order.end(), [&](int a, int b) { return key(a) > key(b); });
   // rows and columns are padded to 128 where a tile of 128 x 128 may be taken (mu_counts), to 64 where none is
-  mu_counts all;
+  mu_counts gram, square;
   pl->tw = 1;
   for (int i = 0; i < count; ++i) {
     const int m = std::min(jobs[i].rows, jobs[i].cols), n = std::max(jobs[i].rows, jobs[i].cols);
     if (m > 64) pl->tw = 2;
-    all.add(mu_up(m, 128), mu_up(n, 128), 1);
+    gram.add_symmetric(mu_up(m, 128), 1, mu_up(n, 128) / 16, true);
+    square.add_symmetric(mu_up(m, 128), 1, mu_up(m, 128) / 16, false);
+    square.add_apply(mu_up(m, 128), mu_up(n, 128), 1);
   }
-  if (!all.large()) pl->tw = 1;
-  // one long matrix, and the others but for large ones go its way: the number of multiplications is the same for m = n, and two
-  // kinds would take their launches one after the other
-  bool all_long = false;
-  for (int i = 0; i < count; ++i)
-    if (std::max(jobs[i].rows, jobs[i].cols) >= 2 * std::min(jobs[i].rows, jobs[i].cols)) all_long = true;
-  int largest = 0;
-  for (int i = 0; i < count; ++i) largest = std::max(largest, std::min(jobs[i].rows, jobs[i].cols));
-  pl->segment = largest >= 256 ? 3 : largest >= 128 ? 2 : 1;
+  if (gram.symmetric() < 4 && square.symmetric() < 4 && square.apply() < 4) pl->tw = 1;
   const int bt = 64 * pl->tw;
   int64_t off = 0;
   pl->groups.clear();
@@ -819,7 +820,7 @@ static void mu_make_plan(const lmh_muon_job* jobs, int count, mu_plan* pl) {
     g.pn = (int)mu_up(g.n, bt);
     g.count = e - s;
     g.first = s;
-    g.longish = pl->segment > 1 && ((all_long && g.pm <= 2048) || g.n >= 2 * g.m);
+    g.segment = mu_segment(g.m, g.n);
     const int mn = (int)((int64_t)g.pm * g.pn / 64), mm = (int)((int64_t)g.pm * g.pm / 64);      // 4 bytes a value, units of 256
     int at = 0;
     auto take = [&](int n) { const int r = at; at += n; return r; };
@@ -829,9 +830,9 @@ static void mu_make_plan(const lmh_muon_job* jobs, int count, mu_plan* pl) {
     g.a = take(mm);
     g.c = take(mm);
     g.p = take(mm);
-    g.z = g.longish ? take(mm) : -1;
-    g.q[0] = g.longish ? take(mm) : -1;
-    g.q[1] = g.longish ? take(mm) : -1;
+    g.z = g.segment > 1 ? take(mm) : -1;
+    g.q[0] = g.segment > 1 ? take(mm) : -1;
+    g.q[1] = g.segment > 1 ? take(mm) : -1;
     g.norm_blocks = (int)std::min<int64_t>(MU_NORM_BLOCKS, ((int64_t)g.m * g.n + MU_NORM_ELEMS - 1) / MU_NORM_ELEMS);
     g.norm = take((int)((g.norm_blocks * sizeof(double) + 255) / 256));
     g.stride = at;
@@ -917,17 +918,15 @@ class mu_runner {
     for (int i = 0; i < MU_MAX_GROUPS; ++i) t->blk0[i] = 0x7fffffff;
   }
 
-  struct product { int l, r, d0, d1, units; float s0, g0, s1, g1; };
-  // Symmetric m x m products of the groups (`make` gives 0, 1 or 2 of a group), tiles of 64 tw.
-  template <typename F>
-  void symmetric(const std::vector<const mu_group*>& gs, int side, F make) {
-    const int bt = 32 * side;
-    std::vector<std::pair<const mu_group*, product>> all;
-    for (const mu_group* g : gs) {
-      product p[2];
-      const int n = make(*g, p);
-      for (int i = 0; i < n; ++i) all.push_back({g, p[i]});
+  struct product { int l, r, d0, d1, units; float s0, g0, s1, g1; bool gram; };
+  // Symmetric products of the groups, in tiles of at most 32 `most`.
+  void symmetric(const std::vector<std::pair<const mu_group*, product>>& all, int most) {
+    mu_counts counts;
+    for (size_t i = 0; i < all.size(); ++i) {
+      const mu_group& g = *all[i].first;          // (two products of one group count once: 1024 x 2048 274 us, 287 in the larger tiles)
+      if (!i || all[i - 1].first != &g) counts.add_symmetric(g.pm, g.count, all[i].second.units, all[i].second.gram);
     }
+    const int side = std::min(most, counts.symmetric()), bt = 32 * side;
     for (size_t lo = 0; lo < all.size(); lo += MU_MAX_GROUPS) {
       const size_t hi = std::min(all.size(), lo + MU_MAX_GROUPS);
       int64_t tiles = 0, stages = 0;
@@ -983,9 +982,15 @@ class mu_runner {
       }
     }
   }
+  static int apply_side(const std::vector<const mu_group*>& gs, int most) {
+    mu_counts counts;
+    for (const mu_group* g : gs) counts.add_apply(g->pm, g->pn, g->count);
+    return std::min(most, counts.apply());
+  }
   // X <- polynomial X
   template <typename F>
-  void apply(const std::vector<const mu_group*>& gs, int side, F operands) {
+  void apply(const std::vector<const mu_group*>& gs, int most, F operands) {
+    const int side = apply_side(gs, most);
     for (size_t lo = 0; lo < gs.size(); lo += MU_MAX_GROUPS) {
       const int nb = tasks(gs, lo, std::min(gs.size(), lo + MU_MAX_GROUPS), [&](const mu_group& g, mu_task* t) {
         operands(g, t);
@@ -1040,14 +1045,37 @@ class mu_runner {
   mu_table tab_;
 };
 
+// The launches of `steps` steps, `segment` of them at most in A behind each other.  flip: which X' is the present one; q: which Q.
+enum { MU_GRAM, MU_POLY, MU_MOVE, MU_NEXT, MU_X };
+struct mu_launch { int what, k, len, q, flip; };
+static std::vector<mu_launch> mu_launches(int steps, int segment) {
+  std::vector<mu_launch> l;
+  for (int done = 0, flip = 0; done < steps; flip = 1 - flip) {
+    const int left = steps - done, len = left == 4 ? std::min(2, segment) : std::min(left, segment);
+    int q = 0;                         // of a run of several steps: their product so far in q[q]
+    l.push_back({MU_GRAM, 0, len, q, flip});
+    for (int k = 0; k < len; ++k) {
+      l.push_back({MU_POLY, k, len, q, flip});
+      if (len == 1) break;
+      l.push_back({MU_MOVE, k, len, q, flip});
+      if (k > 0) q = 1 - q;
+      if (k + 1 < len) l.push_back({MU_NEXT, k, len, q, flip});
+    }
+    l.push_back({MU_X, 0, len, q, flip});
+    done += len;
+  }
+  return l;
+}
+
 template <typename T, bool OPT>
 static void mu_run(const lmh_muon_job* jobs, const mu_plan& pl, int steps, float eps, float gscale, float mu, int nesterov, float lr,
                    char* ws, hipStream_t st) {
   mu_runner run(pl, ws, st);
-  std::vector<const mu_group*> all, gs[2];           // by kind: step by step, long
+  std::vector<const mu_group*> all;
+  bool present[4] = {false, false, false, false};
   for (const mu_group& g : pl.groups) {
     all.push_back(&g);
-    gs[g.longish].push_back(&g);
+    present[g.segment] = true;
   }
   run.with_jobs(jobs, all, [](const mu_group& g, mu_task* t) {
     t->aux = g.norm_blocks;
@@ -1067,74 +1095,77 @@ static void mu_run(const lmh_muon_job* jobs, const mu_plan& pl, int steps, float
     if (mu_alone(tab)) lmh_launch((k_mu_planes<T, OPT, 1>), nb, dim3(256), 0, st, mu_single(tab), mu_jobs_of<1>{{pj.p[0]}}, ws, eps);
     else lmh_launch((k_mu_planes<T, OPT, MU_MAX_GROUPS>), nb, dim3(256), 0, st, tab, pj, ws, eps);
   });
-  for (int kind = 0; kind < 2; ++kind) {
-    const std::vector<const mu_group*>& G = gs[kind];
-    if (G.empty()) continue;
-    mu_counts counts;
-    for (const mu_group* g : G) counts.add(g->pm, g->pn, g->count);
-    const int most = pl.tw == 2 ? 8 : 2;
-    const int side = std::min(most, counts.square()), side_x = std::min(most, counts.apply()), side_gram = std::min(most, counts.gram());
-    int flip = 0;
-    for (int done = 0; done < steps;) {
-      const int left = steps - done, len = kind == 0 ? 1 : left == 4 ? 2 : std::min(left, pl.segment);
-      // A = X X' and b I + c A
-      run.symmetric(G, side_gram, [](const mu_group& g, mu_runner::product* p) {
-        const float s = 1.f / (MU_SX * MU_SX);
-        p[0] = {g.x, g.x, g.a, g.c, g.pn / 16, MU_SG * s, 0.f, MU_C * MU_SC * s, MU_B * MU_SC};
-        return 1;
-      });
-      int q = 0;                       // of a run of several steps: their product so far in q[q]
-      for (int k = 0; k < len; ++k) {
-        // p = (b I + c A) A + a I; the first of several is their product too
-        run.symmetric(G, side, [&](const mu_group& g, mu_runner::product* p) {
-          const float s = 1.f / (MU_SC * MU_SG);
-          p[0] = {g.c, g.a, g.p, k == 0 && len > 1 ? g.q[0] : -1, g.pm / 16, MU_SP * s, MU_A * MU_SP, MU_SQ * s, MU_A * MU_SQ};
-          return 1;
-        });
-        if (len == 1) break;
-        // z = p A unless this is the last of them, Q <- p Q unless it is the first
-        run.symmetric(G, side, [&](const mu_group& g, mu_runner::product* p) {
-          int n = 0;
-          if (k + 1 < len) p[n++] = {g.p, g.a, g.z, -1, g.pm / 16, MU_SG / (MU_SP * MU_SG), 0.f, 0.f, 0.f};
-          if (k > 0) p[n++] = {g.p, g.q[q], g.q[1 - q], -1, g.pm / 16, MU_SQ / (MU_SP * MU_SQ), 0.f, 0.f, 0.f};
-          return n;
-        });
-        if (k > 0) q = 1 - q;
-        if (k + 1 < len) {
-          run.symmetric(G, side, [&](const mu_group& g, mu_runner::product* p) {      // A <- z p
-            const float s = 1.f / (MU_SG * MU_SP);
-            p[0] = {g.z, g.p, g.a, g.c, g.pm / 16, MU_SG * s, 0.f, MU_C * MU_SC * s, MU_B * MU_SC};
-            return 1;
-          });
-        }
-      }
-      done += len;
-      auto operands = [&](const mu_group& g, mu_task* t) {
-        t->l = g.xt[flip];
-        t->r = len > 1 ? g.q[q] : g.p;
-        t->d0 = g.x;
-        t->d1 = g.xt[1 - flip];
-        t->s0 = len > 1 ? 1.f / MU_SQ : 1.f / MU_SP;
-      };
-      if (done < steps) {
-        run.apply(G, side_x, operands);
-        flip = 1 - flip;
-      } else {
-        run.with_jobs(jobs, G, [&](const mu_group& g, mu_task* t) {
-          operands(g, t);
-          t->s0 /= MU_SX;
-          t->aux = g.pm / 16;
-          return mu_x_tiles(g, side_x, true);
-        }, [&](dim3 nb, const mu_table& tab, const mu_jobs& pj) {
-          if (side_x == 1 && mu_alone(tab))
-            lmh_launch((k_mu_small_last<T, OPT, 1>), nb, dim3(256), 0, st, mu_single(tab), mu_jobs_of<1>{{pj.p[0]}}, ws, lr);
-          else if (side_x == 1) lmh_launch((k_mu_small_last<T, OPT, MU_MAX_GROUPS>), nb, dim3(256), 0, st, tab, pj, ws, lr);
-          else if (side_x == 2) lmh_launch((k_mu_last<T, 1, 1, 2, 4, OPT>), nb, dim3(256), 0, st, tab, pj, ws, lr);
-          else if (side_x == 8) lmh_launch((k_mu_last<T, 4, 2, 1, 3, OPT>), nb, dim3(256), 0, st, tab, pj, ws, lr);
-          else lmh_launch((k_mu_last<T, 2, 2, 2, 2, OPT>), nb, dim3(256), 0, st, tab, pj, ws, lr);
-        });
+  // Matrices of different segments go side by side, a launch of each in every round.  A product with X waits one round where the next
+  // but one launch of others is one too: they share it.
+  std::vector<mu_launch> seq[4];
+  size_t at[4] = {0, 0, 0, 0};
+  for (int s = 1; s < 4; ++s)
+    if (present[s]) seq[s] = mu_launches(steps, s);
+  const int most = pl.tw == 2 ? 8 : 2;
+  const float sgg = 1.f / (MU_SX * MU_SX), scg = 1.f / (MU_SC * MU_SG), sgp = 1.f / (MU_SG * MU_SP);
+  for (;;) {
+    bool now[4] = {false, false, false, false}, left = false;
+    for (int s = 1; s < 4; ++s) {
+      if (at[s] >= seq[s].size()) continue;
+      left = now[s] = true;
+      if (seq[s][at[s]].what != MU_X) continue;
+      for (int o = 1; o < 4; ++o)
+        if (at[o] + 1 < seq[o].size() && seq[o][at[o]].what != MU_X && seq[o][at[o] + 1].what == MU_X) now[s] = false;
+    }
+    if (!left) break;
+    std::vector<std::pair<const mu_group*, mu_runner::product>> products;
+    std::vector<const mu_group*> apply, last;
+    for (const mu_group* gp : all) {
+      const mu_group& g = *gp;
+      if (!now[g.segment]) continue;
+      const mu_launch& l = seq[g.segment][at[g.segment]];
+      const int units = g.pm / 16;
+      switch (l.what) {
+        case MU_GRAM:      // A = X X' and b I + c A
+          products.push_back({gp, {g.x, g.x, g.a, g.c, g.pn / 16, MU_SG * sgg, 0.f, MU_C * MU_SC * sgg, MU_B * MU_SC, true}});
+          break;
+        case MU_POLY:      // p = (b I + c A) A + a I; the first of several is their product too
+          products.push_back({gp, {g.c, g.a, g.p, l.k == 0 && l.len > 1 ? g.q[0] : -1, units, MU_SP * scg, MU_A * MU_SP, MU_SQ * scg,
+                                   MU_A * MU_SQ, false}});
+          break;
+        case MU_MOVE:      // z = p A unless this is the last of them, Q <- p Q unless it is the first
+          if (l.k + 1 < l.len) products.push_back({gp, {g.p, g.a, g.z, -1, units, MU_SG / (MU_SP * MU_SG), 0.f, 0.f, 0.f, false}});
+          if (l.k > 0) products.push_back({gp, {g.p, g.q[l.q], g.q[1 - l.q], -1, units, MU_SQ / (MU_SP * MU_SQ), 0.f, 0.f, 0.f, false}});
+          break;
+        case MU_NEXT:      // A <- z p
+          products.push_back({gp, {g.z, g.p, g.a, g.c, units, MU_SG * sgp, 0.f, MU_C * MU_SC * sgp, MU_B * MU_SC, false}});
+          break;
+        case MU_X:
+          (at[g.segment] + 1 == seq[g.segment].size() ? last : apply).push_back(gp);
       }
     }
+    if (!products.empty()) run.symmetric(products, most);
+    auto operands = [&](const mu_group& g, mu_task* t) {
+      const mu_launch& l = seq[g.segment][at[g.segment]];
+      t->l = g.xt[l.flip];
+      t->r = l.len > 1 ? g.q[l.q] : g.p;
+      t->d0 = g.x;
+      t->d1 = g.xt[1 - l.flip];
+      t->s0 = l.len > 1 ? 1.f / MU_SQ : 1.f / MU_SP;
+    };
+    if (!apply.empty()) run.apply(apply, most, operands);
+    if (!last.empty()) {
+      const int side = mu_runner::apply_side(last, most);
+      run.with_jobs(jobs, last, [&](const mu_group& g, mu_task* t) {
+        operands(g, t);
+        t->s0 /= MU_SX;
+        t->aux = g.pm / 16;
+        return mu_x_tiles(g, side, true);
+      }, [&](dim3 nb, const mu_table& tab, const mu_jobs& pj) {
+        if (side == 1 && mu_alone(tab))
+          lmh_launch((k_mu_small_last<T, OPT, 1>), nb, dim3(256), 0, st, mu_single(tab), mu_jobs_of<1>{{pj.p[0]}}, ws, lr);
+        else if (side == 1) lmh_launch((k_mu_small_last<T, OPT, MU_MAX_GROUPS>), nb, dim3(256), 0, st, tab, pj, ws, lr);
+        else if (side == 2) lmh_launch((k_mu_last<T, 1, 1, 2, 4, OPT>), nb, dim3(256), 0, st, tab, pj, ws, lr);
+        else if (side == 8) lmh_launch((k_mu_last<T, 4, 2, 1, 3, OPT>), nb, dim3(256), 0, st, tab, pj, ws, lr);
+        else lmh_launch((k_mu_last<T, 2, 2, 2, 2, OPT>), nb, dim3(256), 0, st, tab, pj, ws, lr);
+      });
+    }
+    for (int s = 1; s < 4; ++s) at[s] += now[s];
   }
 }
 
