@@ -25,7 +25,6 @@
 
 #define LP_MAX_TOP LMH_LOG_PROBS_MAX_TOP
 #define LP_SEG_VECS 4             // 64 registers: eight blocks a compute unit (8: 88 registers, 2-4 % slower)
-#define LP_JOIN_LDS 4096
 
 typedef unsigned long long u64;
 
@@ -308,8 +307,9 @@ k_log_probs(const T* __restrict__ x, int64_t ldx, const I* __restrict__ targets,
     }
     return;
   }
-  // many equal values or not-a-number among them: k times the largest key below the last one
-  u64 last = ~0ull;
+  // many equal values or not-a-number among them: k times the largest key below the last one (the first time: of all - not-a-number
+  // at class 0 has the largest there is)
+  u64 last = 0;
   for (int rank = 0; rank < k; ++rank) {
     u64 mx = 0;
     for (int col = first + lane * VEC; col < end; col += TPR * VEC) {
@@ -317,7 +317,7 @@ k_log_probs(const T* __restrict__ x, int64_t ldx, const I* __restrict__ targets,
 #pragma unroll
       for (int e = 0; e < VEC; ++e) {
         const u64 p = lp_pair(lp_key(elem<T>(r, e)), (uint32_t)(col + e));
-        if (col + e < end && p < last && p > mx) mx = p;
+        if (col + e < end && (rank == 0 || p < last) && p > mx) mx = p;
       }
     }
     mx = wave_max_u64(mx);
@@ -339,12 +339,11 @@ template <typename T, typename I>
 __global__ void __launch_bounds__(256)
 k_log_probs_join(const T* __restrict__ x, int64_t ldx, const I* __restrict__ targets, int64_t rows, int V, int k, int segs, lp_out out,
                  const float* __restrict__ stats, const u64* __restrict__ best) {
-  extern __shared__ u64 lists[];        // [segs][k] when that is at most LP_JOIN_LDS entries
+  extern __shared__ u64 lists[];        // [segs][k]: with alternatives a row has at most 64 parts
   const int64_t row = blockIdx.x;
   const int lane = threadIdx.x;
   const u64* b = best + row * segs * k;
-  const bool in_lds = segs <= 64 && segs * k <= LP_JOIN_LDS;
-  if (in_lds) {
+  if (k > 0) {
     for (int i = threadIdx.x; i < segs * k; i += blockDim.x) lists[i] = b[i];
     if (blockDim.x > 64) __syncthreads();
   }
@@ -377,28 +376,15 @@ k_log_probs_join(const T* __restrict__ x, int64_t ldx, const I* __restrict__ tar
     out.index[row * k + rank] = (int64_t)(uint32_t)~(uint32_t)pair;
     out.top[row * k + rank] = key == 0xffffffffu ? NAN : (lp_unkey(key) - m0) - log_s;
   };
-  u64 last = ~0ull, mine = 0;           // lane r keeps the alternative of rank r (k <= 64)
-  if (in_lds) {
-    int pos = 0;
-    u64 head = lane < segs ? lists[lane * k] : 0;
-    for (int rank = 0; rank < k; ++rank) {
-      const u64 mx = wave_max_u64(head);
-      if (lane == rank) mine = mx;
-      if (head == mx && lane < segs) {
-        ++pos;
-        head = pos < k ? lists[lane * k + pos] : 0;
-      }
-    }
-  } else {
-    for (int rank = 0; rank < k; ++rank) {      // the largest entry below the last one
-      u64 mx = 0;
-      for (int64_t i = lane; i < (int64_t)segs * k; i += 64) {
-        const u64 p = b[i];
-        if (p < last && p > mx) mx = p;
-      }
-      mx = wave_max_u64(mx);
-      if (lane == rank) mine = mx;
-      last = mx;
+  u64 mine = 0;                         // lane r keeps the alternative of rank r (k <= 64)
+  int pos = 0;
+  u64 head = lane < segs ? lists[lane * k] : 0;
+  for (int rank = 0; rank < k; ++rank) {
+    const u64 mx = wave_max_u64(head);
+    if (lane == rank) mine = mx;
+    if (head == mx && lane < segs) {
+      ++pos;
+      head = pos < k ? lists[lane * k + pos] : 0;
     }
   }
   if (lane < k) emit(lane, mine);
@@ -527,7 +513,7 @@ static void lp_fwd_launch(const void* x, int64_t ldx, const void* targets, int64
 #undef LP_FWD
   if (p.parts > 1)       // few entries: one wave a row
     lmh_launch((k_log_probs_join<T, I>), dim3((unsigned)rows), dim3(p.parts * k > 512 ? 256 : 64),
-               (unsigned)(p.parts <= 64 && p.parts * k <= LP_JOIN_LDS ? p.parts * k * sizeof(u64) : 0), st, (const T*)x, ldx, (const I*)targets, rows, V, k, p.parts, o,
+               (unsigned)(p.parts * k * sizeof(u64)), st, (const T*)x, ldx, (const I*)targets, rows, V, k, p.parts, o,
                (const float*)stats, (const u64*)best);
 }
 
