@@ -232,7 +232,10 @@ int lmh_layer_norm_bwd(const void* dy, int64_t lddy, const void* x, int64_t ldx,
  * not-a-number comes first).  A target < 0 is not asked for: logp 0, no gradient; one >= cols gives not-a-number.  Classes of
  * -inf have p = 0; in a row of -inf alone every log probability and lse are -inf, entropy and gradient 0.
  * Backward: dx = g_logp (1[target] - p) + sum_i g_top[i] (1[top_index[i]] - p) - g_entropy p (log p + entropy); g_logp, g_entropy
- * may be NULL, top = 0: no alternatives.  Fewer than 2^24 - 1 rows, and parts of long rows, a call. */
+ * may be NULL, top = 0: no alternatives.  lse: the forward's.  What its rounding lost is found again where that counts (|lse| >= 32: the
+ * row is read once more), so the gradient of logits far from zero is as exact as that of logits around it; an lse that is not
+ * this row's own, of a vocabulary of which these are some classes, is taken as it is.  Fewer than 2^24 - 1 rows, and parts of
+ * long rows, a call. */
 #define LMH_LOG_PROBS_MAX_TOP 64
 size_t lmh_log_probs_workspace_bytes(int64_t rows, int cols, int dtype, int top);
 int lmh_log_probs_fwd(const void* x, int64_t ldx, int dtype, const void* targets, int index64, int64_t rows, int cols, int top,

@@ -393,18 +393,27 @@ k_log_probs_join(const T* __restrict__ x, int64_t ldx, const I* __restrict__ tar
 // Gradient: a thread's vectors of one row, then the given classes' own entries, written whole (p, entropy and every
 // gradient given for that class, in the order target, alternative 0, 1, ...) by one thread each, behind a barrier.  A short row is
 // one wave's, a longer one is cut into `chunks` of one block each.
+//
+// lse = m + log S has been rounded to fp32: up to |lse| 2^-24 of log S is lost, and every p of the row would be off by that factor (logits
+// around 1e4: 5e-4).  Where that is more than 2^-20 (|lse| >= LP_LSE_EXACT) the block sums exp(x - lse) over the whole row, which is what was lost.
+// A sum that differs from 1 by more than the rounding belongs to an lse of other classes too (a vocabulary in shards): that counts as given.
+// That costs an exponential a class of the row in every block, so there one block takes the chunks of `join`, all of a row's while
+// LP_JOINED blocks are left: 4096 x 65536 bf16 with logits around 1000 301 us (187 around 0; every block for itself 710), 777 x 32003 fp32 53
+// (32; 141, 79 with 2048 blocks left), 100 x 131072 bf16 51 (11; 58).
+#define LP_LSE_EXACT 32.f
+#define LP_JOINED 512
 template <typename T, typename I, int TPR>
 __global__ void __launch_bounds__(256)
 k_log_probs_bwd(const T* __restrict__ x, int64_t ldx, const I* __restrict__ targets, const float* __restrict__ lse,
                 const float* __restrict__ entropy, const float* __restrict__ g_logp, const float* __restrict__ g_entropy,
                 const int64_t* __restrict__ index, const float* __restrict__ g_top, int64_t rows, int V, int k, int chunk, int chunks,
-                T* __restrict__ dx) {
+                int join, T* __restrict__ dx) {
   constexpr int VEC = row_type<T>::VEC;
   const int lane = threadIdx.x & (TPR - 1);
   const int64_t row = TPR == 64 ? (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6) : blockIdx.x / chunks;
   if (TPR == 64 && row >= rows) return;                         // (no barrier below)
-  const int first = TPR == 64 ? 0 : (int)(blockIdx.x % chunks) * chunk;
-  const int end = V - first < chunk ? V : first + chunk;
+  int first = TPR == 64 ? 0 : (int)(blockIdx.x % chunks) * chunk;
+  int end = V - first < chunk ? V : first + chunk;
   const T* xr = x + row * ldx;
   T* dr = dx + row * (int64_t)V;
   const float l = lse[row];
@@ -415,8 +424,29 @@ k_log_probs_bwd(const T* __restrict__ x, int64_t ldx, const I* __restrict__ targ
   float G = gt;
   for (int i = 0; i < k; ++i) G += g_top[row * k + i];
   const float h = g_entropy ? entropy[row] : 0.f, gh = g_entropy ? g_entropy[row] : 0.f;
+  float rest = 0.f;                                             // log S = (lse - m) + rest
+  if (fabsf(l) >= LP_LSE_EXACT && fabsf(l) < INFINITY) {        // (the same for all threads of a row)
+    __shared__ float red[4];
+    if (TPR > 64) {
+      // (another one from row to row: every eighth block runs on the same die)
+      const int c = (int)(blockIdx.x % chunks), c0 = c / join * join, n = min(join, chunks - c0);
+      if (c - c0 != (int)(((uint32_t)row * 2654435769u >> 8) % (uint32_t)n)) return;                     // (the whole block)
+      first = c0 * chunk;
+      end = V - first < (int64_t)chunk * n ? V : first + chunk * n;
+    }
+    float s = 0.f;
+#pragma unroll 4
+    for (int col = lane * VEC; col < V; col += TPR * VEC) {
+      const raw16 r = load_classes(xr, col, V);
+#pragma unroll
+      for (int e = 0; e < VEC; ++e) s += __expf(elem<T>(r, e) - l);
+    }
+    s = reduce_row<TPR>(s, op_add(), red);
+    const float lost = logf(s);
+    if (fabsf(lost) <= fabsf(l) * 0x1p-23f + 0x1p-19f) rest = lost;
+  }
   auto value = [&](float f) {
-    const float lp = f - l, p = __expf(lp);
+    const float lp = f - l - rest, p = __expf(lp);
     return p > 0.f || p != p ? -p * fmaf(gh, lp + h, G) : 0.f;
   };
   for (int col = first + lane * VEC; col < end; col += TPR * VEC) {
@@ -534,9 +564,10 @@ static void lp_bwd_launch(const void* x, int64_t ldx, const void* targets, const
                           hipStream_t st) {
   const int chunk = lp_bwd_chunk(rows, V, row_type<T>::VEC);
   const int chunks = (int)lp_bwd_chunks(rows, V, row_type<T>::VEC);
+  const int join = (int)std::max<int64_t>(1, std::min<int64_t>(chunks, rows * chunks / LP_JOINED));
 #define LP_BWD(TPR_, BLOCKS_)                                                                                               \
   lmh_launch((k_log_probs_bwd<T, I, TPR_>), dim3((unsigned)(BLOCKS_)), dim3(256), 0, st, (const T*)x, ldx, (const I*)targets, lse, entropy, \
-             g_logp, g_entropy, index, g_top, rows, V, k, chunk, chunks, (T*)dx)
+             g_logp, g_entropy, index, g_top, rows, V, k, chunk, chunks, join, (T*)dx)
   if (V <= 64 * row_type<T>::VEC * 2) LP_BWD(64, (rows + 3) / 4);
   else LP_BWD(256, rows * chunks);
 #undef LP_BWD

@@ -1409,7 +1409,8 @@ def log_probs_fwd(logits, targets=None, top_k=0):
 
 def log_probs_bwd(logits, targets, lse, entropy, g_logp=None, g_entropy=None, top_index=None, g_top=None):
     """-> gradient of the logits (their type, contiguous) from the gradients of log_probs_fwd's logp, entropy and top_logp (each
-    may be None)."""
+    may be None).  What lse lost by its rounding is found again in rows where that counts (|lse| >= 32; the row is read once
+    more); an lse of more classes than these is taken as it is."""
     lib = _lib.load()
     if top_index is None or g_top is None:
         top_index = g_top = None
