@@ -246,7 +246,8 @@ int lmh_log_probs_bwd(const void* x, int64_t ldx, int dtype, const void* targets
                       const float* g_top, int64_t rows, int cols, int top, void* dx, lmh_stream_t stream);
 /* Orthogonalised updates (the Muon optimizer, beside lmh_optimizer_step) for a list of matrices (rows, cols) at a time:
  * O(U) = `steps` Newton-Schulz steps X <- (a I + b A + c A A) X, A = X X' (a, b, c = 3.4445, -4.7750, 2.0315) on X = U / max(|U|_F,
- * eps), in products of fp32 accuracy.
+ * eps), in products of fp32 accuracy relative to the whole matrix: what is off is some 2^-24 of the result's norm, and a row that is
+ * 1e-4 of the largest or less has fewer right digits of its own than fp32 would give it (1e-6: four).
  * lmh_orthogonalize: out = O(g); g and out of `dtype`.
  * lmh_muon_step (fp32): g' = (g gscale + wd w) * factor, v = momentum v + g', U = nesterov ? g' + momentum v : v,
  * w -= lr scale O(U); `factor`: one float on the device (a clip factor of lmh_grad_clip_factors) or NULL.  Every w and v is

@@ -10,7 +10,11 @@
 // lo hi, hi hi; lo lo is below 2^-24) with fp32 accumulation: 3 instead of the 6 of a bf16 split, and 2500 / 3 TFLOP/s
 // against 157 of the fp32 instructions.  f16's range is enough because everything here is bounded in the spectral norm, which
 // bounds the entries: |X| <= 1.25, |A| <= 1.6, |b I + c A| <= 4.8, |p| <= 3.5, products of three p <= 41; fixed powers of two
-// put those just below 65504, so lo keeps its bits down to entries of 2^-24 of the bound.
+// put those below 65504, the largest that do.
+// What the fixed scale costs: lo ends at 2^-24, so an entry of X is off by up to 2^-40 whatever its size (a power of two less for the
+// others), and small rows lose bits that fp32 would keep: of 300 x 1000 with rows graded from 1 to 1e-6, in units of the row's own
+// norm, 7e-7 at 1e-4 of the largest, 6e-6 at 1e-5, 6e-5 at 1e-6 (fp32: 3e-7; with scales a quarter as large four times as much); rows
+// down to 1e-3 are as exact as in fp32.
 //
 // Long matrices (n >= 2 m).  The steps are polynomials in A, which commute: A <- p A p and Q <- p Q take m x m products only, and
 // X <- Q X comes every second or third step: of 15 m m n multiplications in five steps 6 are left.  A's error grows by up to
@@ -48,10 +52,10 @@
 #define MU_B -4.7750f
 #define MU_C 2.0315f
 // scales of what is stored as f16 pairs (powers of two)
-#define MU_SX 8192.f      // X
-#define MU_SG 8192.f      // A, p A
+#define MU_SX 32768.f     // X
+#define MU_SG 32768.f     // A, p A
 #define MU_SC 8192.f      // b I + c A, eigenvalues in [b, b + 1.6 c]
-#define MU_SP 8192.f      // p(A)
+#define MU_SP 16384.f     // p(A)
 #define MU_SQ 1024.f      // products of up to three of them
 #define MU_MAX_GROUPS 24  // of one launch (kernel arguments: under 4 KB together)
 #define MU_MAX_JOBS 44

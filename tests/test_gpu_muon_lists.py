@@ -76,3 +76,25 @@ def test_the_update_of_a_small_weight_beside_large_ones():
             plain[i] += float(torch.linalg.norm(ns(u, torch.float32).double() - want)) / size
             own[i] += float(torch.linalg.norm(-o.double() - want)) / size
     assert all(o <= 2 * p for o, p in zip(own, plain)), list(zip(shapes, own, plain))
+
+
+@pytest.mark.parametrize('rows,cols', [(64, 256), (128, 500), (1000, 300), (512, 512)])
+def test_rows_of_very_different_size(rows, cols):
+    """Rows (the short side's) graded from 1 to 1e-6 of the largest: every row's own error.  X is held as two f16 pieces with a scale of 2^15, so
+    below some size its entries are multiples of 2^-24 / 2^15 = 2^-39: a root mean square of 2^-39 / sqrt(12) an entry, sqrt(n) times that a row,
+    in the first X and in that of every step, each grown 3.4445 times a step from there on: 3.4445^5 (1 + 1/11.9 + ...)^0.5 = 506 of the
+    first.  What the polynomials' entries are off by adds some tenths of that.  Twice that, and four times what float32 is off by: the
+    expected quotient is 1.5 (above), and one row's error may lie in one direction, so a mean over four seeds of half a normal
+    distribution is known to 0.76 / 2 = 38 %, a quotient of two of them to 53 %, and three of those make 1.5 a 3.9."""
+    m, n = min(rows, cols), max(rows, cols)
+    grade = torch.logspace(0, -6, m)[:, None]
+    plain, own = torch.zeros(m), torch.zeros(m)
+    for seed in range(4):
+        u = (torch.randn((m, n), generator=torch.Generator().manual_seed(seed)) * grade).cuda()
+        want = ns(u, torch.float64)
+        got = K.orthogonalize([u if rows <= cols else u.t().contiguous()])[0]
+        got = got if rows <= cols else got.t()
+        plain += (ns(u, torch.float32).double() - want).norm(dim=1).cpu().float() / 4
+        own += (got.double() - want).norm(dim=1).cpu().float() / 4
+    tol = 4 * plain + 2 * 506 * n ** 0.5 * 2.0 ** -39 / 12 ** 0.5
+    assert (own <= tol).all(), float((own / tol).max())
