@@ -358,6 +358,12 @@ def free_port():
     return p
 
 
+def hardware_queues(exported):
+    """GPU_MAX_HW_QUEUES of a launched rank: 8 where nothing is exported, or HIP's own default of 4, which some machines export for
+    every process (fewer queues than the step has streams); any other value is the caller's choice and stays."""
+    return '8' if exported in (None, '', '4') else exported
+
+
 def main():
     ap = argparse.ArgumentParser()
     ap.add_argument('--gpus', type=int, default=1)
@@ -424,9 +430,7 @@ def main():
         # Every process started by a launcher (torch.distributed.run sets WORLD_SIZE, also for ONE rank) gets the same
         # mapping, so the N = 1 point of a scaling run and its N > 1 points differ in the exchange only; the plain
         # `python bench.py` headline keeps HIP's default (A/B of the two at N = 1: DESIGN.md 8).
-        # (a machine may export HIP's own default, 4: fewer queues than the step has streams)
-        if int(os.environ.get('GPU_MAX_HW_QUEUES') or 0) < 8:
-            os.environ['GPU_MAX_HW_QUEUES'] = '8'
+        os.environ['GPU_MAX_HW_QUEUES'] = hardware_queues(os.environ.get('GPU_MAX_HW_QUEUES'))
     rank = int(os.environ.get('RANK', '0'))
     local_rank = int(os.environ.get('LOCAL_RANK', '0'))
     if not torch.cuda.is_available():
