@@ -356,6 +356,10 @@ def allreduce_probe(flat_numel, device, reps=5, bucket_mb=12):
                                 'bus_GB/s': 2.0 * (world - 1) / world * t.numel() * 4 / med / 1e9,
                                 'correct': bool(abs(float(t[0]) - world) < 1e-3)})
         del t
+    # every rank has measured its own times, but the buckets of an exchange have to be the same on all of them: the slowest rank's
+    slowest = torch.tensor([times[k][0] for k in ('flat_gradient', 'bucket')], dtype=torch.float64, device=dev)
+    dist.all_reduce(slowest, op=dist.ReduceOp.MAX)
+    times = {k: (t, times[k][1]) for k, t in zip(('flat_gradient', 'bucket'), slowest.tolist())}
     (ts, bs), (tl, bl) = sorted(times.values(), key=lambda v: v[1])
     # a quarter of the gradient at most, whatever a collective costs: larger buckets leave nothing to exchange under the backward
     bucket, alpha, beta = bucket_bytes_from_probe(ts, bs, tl, bl, hi=min(64 << 20, max(4 << 20, int(flat_numel) >> 20 << 20)))
