@@ -318,6 +318,12 @@ def bucket_bytes_from_probe(t_small_s, small_bytes, t_large_s, large_bytes, lo=4
     return bucket, alpha, beta
 
 
+def bucket_that_overlaps(bucket_bytes, grad_bytes, lo=4 << 20):
+    """A bucket of more than half the gradient leaves nothing to exchange under the backward, however long the exchange takes: a
+    quarter of the gradient then (1 MB steps, `lo` at least).  Smaller buckets stay as the collective's cost asks for."""
+    return bucket_bytes if 2 * bucket_bytes <= grad_bytes else min(bucket_bytes, max(lo, grad_bytes // 4 >> 20 << 20))
+
+
 def allreduce_probe(flat_numel, device, reps=5, bucket_mb=12):
     """Times dist.all_reduce (sum, fp32) of a tensor as large as the model's flat gradient and of one `bucket_mb` MB bucket:
     one untimed round, then the median of `reps`; plus an all-reduce of ones — `ranks_seen` comes from the collective's own
@@ -361,11 +367,11 @@ def allreduce_probe(flat_numel, device, reps=5, bucket_mb=12):
     dist.all_reduce(slowest, op=dist.ReduceOp.MAX)
     times = {k: (t, times[k][1]) for k, t in zip(('flat_gradient', 'bucket'), slowest.tolist())}
     (ts, bs), (tl, bl) = sorted(times.values(), key=lambda v: v[1])
-    # a quarter of the gradient at most, whatever a collective costs: larger buckets leave nothing to exchange under the backward
-    bucket, alpha, beta = bucket_bytes_from_probe(ts, bs, tl, bl, hi=min(64 << 20, max(4 << 20, int(flat_numel) >> 20 << 20)))
+    bucket, alpha, beta = bucket_bytes_from_probe(ts, bs, tl, bl)
+    bucket = bucket_that_overlaps(bucket, int(flat_numel) * 4)
     out.update({'alpha_us': alpha * 1e6, 'beta_GB/s': beta / 1e9, 'bucket_bytes_from_probe': bucket,
                 'model': 't(bytes) = alpha + bytes / beta from the two messages; bucket = smallest size with alpha <= 25 % of '
-                         'its transfer time, 1 MB steps, clamped to [4, 64] MB and to a quarter of the gradient'})
+                         'its transfer time, 1 MB steps, clamped to [4, 64] MB; a quarter of the gradient where that is more than half of it'})
     return out
 
 

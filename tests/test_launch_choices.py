@@ -57,3 +57,11 @@ def test_ranks_agree_on_the_bucket_they_measured():
         assert p.exitcode == 0
     assert b0 == b1 and a0 == a1 and a1 >= 20e3, (b0, b1, a0, a1)
     assert min(ms1) >= 50 and ms0 != ms1
+
+
+@pytest.mark.parametrize('bucket,gradient,used', [(12, 112, 12), (56, 112, 56), (57, 112, 28), (64, 112, 28), (24, 60, 24), (31, 60, 15), (64, 1000, 64),
+                                                  (10, 40, 10), (8, 16, 8), (9, 16, 4), (4, 1, 4), (64, 9, 4)])
+def test_a_bucket_leaves_something_to_overlap(bucket, gradient, used):
+    """MB: only a bucket of more than half the gradient is cut, to a quarter; what a measured collective asks for below that stays"""
+    from luminoth_amd.utils.training import bucket_that_overlaps
+    assert bucket_that_overlaps(bucket << 20, gradient << 20) == used << 20
