@@ -66,3 +66,26 @@ def test_alternatives_of_a_diverged_head():
     x = torch.full((2, 300, 21), math.nan, device='cuda')
     index = K.log_probs_fwd(x, None, 21)[3]
     assert torch.equal(index.cpu(), torch.arange(21).expand(2, 300, 21))
+
+
+@pytest.mark.parametrize('rows,C,dtype', [(2100, 16389, torch.float32), (1400, 33001, torch.bfloat16), (4200, 16390, torch.float16), (3, 300007, torch.float32)])
+@pytest.mark.parametrize('k', [20, 33, 40, 64])
+def test_sums_with_and_without_alternatives(rows, C, dtype, k):
+    """More alternatives cut long rows into other parts, so sums are added in another order: log p, lse and entropy of both ways are each
+    within (100 + 4 E|z|) u of the exact ones (entropy: 110 E|z| + 4 E z^2 more; their own rounding on top), u = 2^-24, z = x - max."""
+    g = torch.Generator(device='cuda').manual_seed(C + k)
+    x = (torch.randn((rows, C), generator=g, device='cuda') * 3).to(dtype)
+    x[0] = torch.linspace(-9, 9, C, device='cuda')
+    x[1] = 1.5
+    x[2, : C - 5] = -math.inf
+    t = torch.randint(C - 5, C, (rows,), generator=g, device='cuda')
+    n = min(rows, 300)
+    a, b = ([v[:n].double() for v in (r[0], r[4], r[1])] for r in (K.log_probs_fwd(x, t, k), K.log_probs_fwd(x, t, 0)))
+    z = x[:n].double()
+    z = z - z.amax(-1, keepdim=True)
+    p = torch.softmax(z, -1)
+    z = torch.where(p > 0, z, torch.zeros_like(z))
+    ez, ezz = (p * z.abs()).sum(-1), (p * z * z).sum(-1)
+    u = 2.0 ** -24
+    for v, w, more in zip(a, b, (0, 0, 110 * ez + 4 * ezz)):
+        assert ((v - w).abs() <= 2 * u * (100 + 4 * ez + more) + 4 * u * w.abs()).all()
