@@ -525,7 +525,6 @@ class MuonOptimizer(MomentumOptimizer):
     LayerNorm parameters, matrices of one row or column or beyond the kernel's sizes, and variables whose name contains a
     string of `exclude` take Adam.  As with every optimizer here the L2 term is part of the gradient (total_loss holds it) and
     `train.clip_by_norm` acts on g + wd * w per variable."""
-    KIND = 5
 
     def __init__(self, model, train_config, momentum=0.95, use_nesterov=True, ns_steps=5, epsilon=1e-7, beta1=0.9, beta2=0.95,
                  adam_epsilon=1e-8, exclude=()):
