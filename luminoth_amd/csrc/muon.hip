@@ -25,7 +25,7 @@
 // or not long (there A has little or nothing to save).  That goes by its own sides, whatever else is in the list: three steps for all
 // of a list with one large matrix had squares of 16 beside it off by 5.6e-6, 7 times as much as fp32 (now 0.8e-6).  The three kinds
 // advance side by side, a launch for all of them, and the five products with X of one meet the others' where they can: the 42
-// matrices of a ResNet-50 detector take 28 launches, 491 us (three steps for all of them: 22 and 444; one: 589).  One matrix of few tiles
+// matrices of a ResNet-50 detector take 28 launches, 488 us (three steps for all of them: 22 and 444; one: 589).  One matrix of few tiles
 // takes as long either way (1024 x 320 100 us with three and with one, 200 x 420 82 and 77), eight of them do not (320 x 1024 199 and
 // 219).
 //
@@ -39,8 +39,8 @@
 // Products with too few tiles for the chip (a long k), and the tiles that a last round of blocks would leave over, are split
 // along k; their parts are joined, in order, by a launch of their own.
 //
-// Measured (five steps): 4096 x 4096 fp32 3.95 ms, products with X 350 us = 1180 TFLOP/s of f16 instructions, symmetric ones 206 us = 1040;
-// 1024 x 320 bf16 100 us in 19 launches; the 42 matrices of a ResNet-50 detector, a whole optimizer step, 491 us in 28.
+// Measured (five steps): 4096 x 4096 fp32 3.9-4.05 ms, products with X 356 us = 1160 TFLOP/s of f16 instructions, symmetric ones 205 us = 1040;
+// 1024 x 320 bf16 98-100 us in 19 launches; the 42 matrices of a ResNet-50 detector, a whole optimizer step, 488 us in 28.
 #include <algorithm>
 #include <tuple>
 #include <type_traits>
@@ -65,8 +65,8 @@
 #define MU_SMALL 160
 #define MU_SMALL_X 256        // ... of the products with X
 // Two tiles of 128 x 128 in one of 256 x 128: a unit of 16 k then takes 12 KB of LDS reads and 6 KB of writes a wave for 24 matrix
-// instructions instead of 8 + 4 for 12 - with those LDS has as many cycles of work as the matrix cores - (4096 x 4096: 373 -> 350 us a
-// product = 1180 TFLOP/s of f16 instructions).  Where rounds of blocks cost more than that gains, or k is short and the rest of a
+// instructions instead of 8 + 4 for 12 - with those LDS has as many cycles of work as the matrix cores - (4096 x 4096: 373 -> 356 us a
+// product = 1160 TFLOP/s of f16 instructions).  Where rounds of blocks cost more than that gains, or k is short and the rest of a
 // block's work counts (42 matrices of m = 128 to 512: 50 -> 53 us), 128 x 128 stays.
 #define MU_NORM_BLOCKS 512
 #define MU_NORM_ELEMS 2048    // at least this many per block of k_mu_norm
