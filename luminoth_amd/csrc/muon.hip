@@ -1054,6 +1054,7 @@ enum { MU_GRAM, MU_POLY, MU_MOVE, MU_NEXT, MU_X };
 struct mu_launch { int what, k, len, q, flip; };
 static std::vector<mu_launch> mu_launches(int steps, int segment) {
   std::vector<mu_launch> l;
+  l.reserve(5 * steps);
   for (int done = 0, flip = 0; done < steps; flip = 1 - flip) {
     const int left = steps - done, len = left == 4 ? std::min(2, segment) : std::min(left, segment);
     int q = 0;                         // of a run of several steps: their product so far in q[q]
@@ -1107,6 +1108,9 @@ static void mu_run(const lmh_muon_job* jobs, const mu_plan& pl, int steps, float
     if (present[s]) seq[s] = mu_launches(steps, s);
   const int most = pl.tw == 2 ? 8 : 2;
   const float sgg = 1.f / (MU_SX * MU_SX), scg = 1.f / (MU_SC * MU_SG), sgp = 1.f / (MU_SG * MU_SP);
+  std::vector<std::pair<const mu_group*, mu_runner::product>> products;
+  std::vector<const mu_group*> apply, last;
+  products.reserve(2 * all.size());
   for (;;) {
     bool now[4] = {false, false, false, false}, left = false;
     for (int s = 1; s < 4; ++s) {
@@ -1117,8 +1121,9 @@ static void mu_run(const lmh_muon_job* jobs, const mu_plan& pl, int steps, float
         if (at[o] + 1 < seq[o].size() && seq[o][at[o]].what != MU_X && seq[o][at[o] + 1].what == MU_X) now[s] = false;
     }
     if (!left) break;
-    std::vector<std::pair<const mu_group*, mu_runner::product>> products;
-    std::vector<const mu_group*> apply, last;
+    products.clear();
+    apply.clear();
+    last.clear();
     for (const mu_group* gp : all) {
       const mu_group& g = *gp;
       if (!now[g.segment]) continue;
